@@ -76,6 +76,8 @@ int mfb_graph_begin(void* stream);
 int mfb_graph_end(void* stream, void** graph_exec);
 int mfb_graph_launch(void* graph_exec, void* stream);
 int mfb_graph_destroy(void* graph_exec);
+/* 1 while `stream` records a graph (between mfb_graph_begin and mfb_graph_end, or any other stream capture). */
+int mfb_stream_is_capturing(void* stream, int* capturing);
 
 /* ---- fake quantization ----------------------------------------------------
  * Replaces Quantizer.effective (src/minifield_training/kernels/quantization.py:11-22,
@@ -198,7 +200,7 @@ int mfb_decode_attn_noalloc(const uint16_t* q, uint16_t* k_cache, uint16_t* v_ca
  * STE mask of the QAT weight gradient). This is the GEMM of full_linear
  * (src/minifield_training/kernels/linear.py:7-13) and its two transposes. */
 enum mfb_major { MFB_MAJOR_K = 0, MFB_MAJOR_MN = 1 };
-enum mfb_dtype { MFB_DTYPE_BF16 = 0, MFB_DTYPE_F32 = 1 };
+enum mfb_dtype { MFB_DTYPE_BF16 = 0, MFB_DTYPE_F32 = 1, MFB_DTYPE_F16 = 2 };
 int mfb_gemm_bf16(const uint16_t* A, int a_major, int lda, const uint16_t* B, int b_major, int ldb, void* C,
                   int ldc, int out_dtype, int M, int N, int K, float alpha, const uint8_t* mask, void* stream);
 /* The gate|up projection of the SwiGLU block with the SwiGLU product in its
@@ -383,6 +385,93 @@ int mfb_cast_bf16_f32(const uint16_t* x, float* y, long long n, void* stream);
  * (src/minifield_training/layers/attention.py:100-108,
  * layers/feed_forward.py:35). n a multiple of 8; 16-byte aligned buffers. */
 int mfb_add_bf16(const uint16_t* a, const uint16_t* b, uint16_t* out, long long n, void* stream);
+
+/* ---- Rotary positions with head norms, any layout -------------------------------
+ * mfb_qknorm_rope_fwd / _bwd above are the reference's own op (64-wide heads,
+ * whole head rotated in the half layout, bf16 rounding after each step). These
+ * are the general form, computed in FP32 and rounded once: D = 64 or 128,
+ * dtype MFB_DTYPE_BF16 or MFB_DTYPE_F16, qkv [M, ld_qkv] = [q heads | k heads |
+ * v heads] x D. Per q and k head x at position p:
+ *   u = wq|wk * x / sqrt(mean(x^2) + eps)     (u = x when wq and wk are NULL)
+ *   the first rotary_dim values of u (a multiple of 16, 0 to D) are rotated in
+ *   pairs by the angle p * freqs[i], i < rotary_dim/2: pair i is (i, i +
+ *   rotary_dim/2), or (2i, 2i+1) when `interleaved`; cos and sin are multiplied
+ *   by amplitude; the other values pass through.
+ * freqs are FP32 radians per position, positions any int32; angles are formed
+ * in FP64. v heads are copied (v may be NULL: not written). */
+int mfb_qk_rotary_fwd(const void* qkv, int ld_qkv, const float* wq, const float* wk, const int32_t* positions,
+                      const float* freqs, void* q, void* k, void* v, int M, int H, int Hk, int D, int rotary_dim,
+                      int interleaved, int dtype, float amplitude, float eps, void* stream);
+/* d_qkv [M, ld_qkv] from dq [M,H,D], dk and dv [M,Hk,D] (norms recomputed from
+ * qkv), and the gain gradients dwq, dwk [D] FP32, written or added to
+ * (accumulate); both NULL to leave them out. d_qkv may be qkv itself. */
+size_t mfb_qk_rotary_workspace_size(int D);
+int mfb_qk_rotary_bwd(const void* qkv, int ld_qkv, const float* wq, const float* wk, const int32_t* positions,
+                      const float* freqs, const void* dq, const void* dk, const void* dv, void* dqkv, float* dwq,
+                      float* dwk, int accumulate, int M, int H, int Hk, int D, int rotary_dim, int interleaved,
+                      int dtype, float amplitude, float eps, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Paged key/value cache -------------------------------------------------------
+ * Pools k_pages, v_pages [num_pages, page_size, Hk, D], or [num_pages, Hk,
+ * page_size, D] when head_major; page_size a power of two >= 8. Sequence b has
+ * seq_lens[b] tokens, the new ones included; token j lies in row j % page_size
+ * of page page_table[b][j / page_size] (page_table [B, max_pages]). Its new
+ * tokens are rows [cu_q[b], cu_q[b+1]) of the token arrays (cu_q [B+1], cu_q[0]
+ * = 0) and are the last of the sequence. Rows from cu_q[B] to N are padding and
+ * left as they were. The reference keeps fixed-capacity caches [B, capacity,
+ * Hk, 64] (src/minifield_training/models/lfm2_5/decode.py:96-117).
+ *
+ * Append: the norm and rotation of mfb_qk_rotary_fwd at each token's place in
+ * its sequence, q [N,H,D] written, k and v rows stored in the pages. A token
+ * whose page entry is outside [0, num_pages) or behind max_pages is not stored.
+ * Two sequences must not append to one page row in one call. */
+int mfb_paged_append(const void* qkv, int ld_qkv, const float* wq, const float* wk, const float* freqs,
+                     const int32_t* cu_q, const int32_t* seq_lens, const int32_t* page_table, void* q, void* k_pages,
+                     void* v_pages, int N, int B, int max_pages, int num_pages, int page_size, int H, int Hk, int D,
+                     int rotary_dim, int interleaved, int head_major, int dtype, float amplitude, float eps,
+                     void* stream);
+/* Attention of the new tokens q [N,H,D] over the cache, causal: token i of the
+ * sequence's n new ones sees the keys j <= seq_lens[b] - n + i. o [N,H,D]; lse
+ * [N,H] FP32 (natural log-sum-exp of the scaled scores) when not NULL. A token
+ * without keys gives zeros and lse -inf. max_q bounds the new tokens of any
+ * sequence (and picks the kernel: up to 16 query rows per KV head, max_q x
+ * H/Hk, run on a bandwidth-bound kernel, more on tcgen05 tiles). H/Hk <= 128.
+ * Keys and values behind a sequence's end may hold anything; those inside it
+ * must be finite (a non-finite value reaches queries up to 128 keys before
+ * it). Device arguments that contradict each other (cu_q outside [0, N], more
+ * than max_q new tokens, lengths outside the table, a used page id outside the
+ * pool: read as zeros) are clamped and recorded in the status word, never
+ * followed out of the buffers. The workspace holds the schedule and the
+ * partials; calls that share one must not overlap. */
+size_t mfb_paged_attn_workspace_size(int N, int B, int max_q, int H, int Hk, int D);
+int mfb_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* cu_q,
+                   const int32_t* seq_lens, const int32_t* page_table, void* o, float* lse, int N, int B, int max_q,
+                   int max_pages, int num_pages, int page_size, int H, int Hk, int D, int head_major, int dtype,
+                   float scale, void* workspace, size_t workspace_bytes, void* stream);
+/* Reads (and clears) the paged attention's device status word: 0 = ok, 1001 = a
+ * page id outside the pool, 1002 = lengths that contradict each other, else the
+ * id of a bounded pipeline wait that gave up. Synchronous. */
+int mfb_paged_attn_status(int* code);
+
+/* ---- Logit controls -------------------------------------------------------------
+ * out [B,V] FP32 from logits [B,V] (bf16, fp16 or FP32; FP32 may be out
+ * itself). With history [B, history_capacity] token ids, of which
+ * [0, history_len[b]) are used (NULL: all) and [prompt_len[b], history_len[b])
+ * were generated (NULL: from 0); ids outside [0, V) count for nothing. Per
+ * token t, each parameter NULL or one FP32 per row:
+ *   x = x > 0 ? x / repetition : x * repetition   if t occurs in the history
+ *   x -= frequency * (times generated) + presence * (generated at all)
+ *   x += bias_values[b][i] where bias_ids[b][i] == t (i < bias_count; of equal
+ *        ids the last entry counts, ids outside [0, V) none)
+ *   x = -inf where bit t % 32 of mask word t / 32 is 0
+ * mask [mask_count, ceil(V/32)]: row mask_rows[b], or b when mask_rows is NULL;
+ * an index outside [0, mask_count) leaves the row unmasked. history_capacity <
+ * 2^20, bias_count <= 2047, V <= 393216. */
+int mfb_logits_process(const void* logits, int dtype, const int32_t* history, int history_capacity,
+                       const int32_t* prompt_len, const int32_t* history_len, const float* repetition,
+                       const float* frequency, const float* presence, const int32_t* bias_ids,
+                       const float* bias_values, int bias_count, const uint32_t* mask, const int32_t* mask_rows,
+                       int mask_count, float* out, int B, int V, void* stream);
 
 /* ---- NCCL communicator (data-parallel exchange) -------------------------------
  * The psum of (loss, count, gradient tree) over the data axis of the

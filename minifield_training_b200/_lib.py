@@ -24,7 +24,7 @@ QUANT_KINDS = {
 MASK_CAUSAL, MASK_PREFIX, MASK_PACKED, MASK_BIDIR, MASK_CACHED = range(5)
 EMPTY_UNIFORM, EMPTY_ZERO = 0, 1
 MAJOR_K, MAJOR_MN = 0, 1
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_F16 = range(3)
 GEMM_PDL = 1
 
 P = ctypes.c_void_p
@@ -79,6 +79,7 @@ SIGNATURES = {
     "mfb_graph_end": (I, [P, ctypes.POINTER(ctypes.c_void_p)]),
     "mfb_graph_launch": (I, [P, P]),
     "mfb_graph_destroy": (I, [P]),
+    "mfb_stream_is_capturing": (I, [P, IP]),
     "mfb_adamw_workspace_size": (SZ, []),
     "mfb_adamw_commit": (I, [P, P, P, P, LL, LL, LL, P, P, P, P, F, F, F, F, F, F, P, P, SZ, P]),
     "mfb_adamw_shard_pass": (I, [I, P, P, P, P, LL, LL, LL, LL, LL, P, P, P, P, F, F, F, F, F, F, P, P, P, SZ, P]),
@@ -113,6 +114,14 @@ SIGNATURES = {
     "mfb_comm_destroy": (I, [P]),
     "mfb_conv_step": (I, [P, P, P, P, I, I, P]),
     "mfb_conv_causal": (I, [P, P, P, P, P, I, I, I, P]),
+    "mfb_qk_rotary_fwd": (I, [P, I] + [P] * 7 + [I] * 7 + [F, F, P]),
+    "mfb_qk_rotary_workspace_size": (SZ, [I]),
+    "mfb_qk_rotary_bwd": (I, [P, I] + [P] * 10 + [I] * 8 + [F, F, P, SZ, P]),
+    "mfb_paged_append": (I, [P, I] + [P] * 9 + [I] * 12 + [F, F, P]),
+    "mfb_paged_attn_workspace_size": (SZ, [I] * 6),
+    "mfb_paged_attn": (I, [P] * 8 + [I] * 11 + [F, P, SZ, P]),
+    "mfb_paged_attn_status": (I, [IP]),
+    "mfb_logits_process": (I, [P, I, P, I] + [P] * 7 + [I, P, P, I, P, I, I, P]),
 }
 
 _lib = None

@@ -195,6 +195,17 @@ int mfb_graph_launch(void* graph_exec, void* stream) {
   return MFB_OK;
 }
 
+int mfb_stream_is_capturing(void* stream, int* capturing) {
+  MFB_CHECK_ARG(capturing != nullptr, "capturing is NULL");
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing((cudaStream_t)stream, &st);
+  // The legacy default stream cannot record; asked while another stream does, it answers with this error.
+  if (e == cudaErrorStreamCaptureImplicit) cudaGetLastError();
+  else MFB_CUDA_TRY(e);
+  *capturing = e == cudaSuccess && st != cudaStreamCaptureStatusNone;
+  return MFB_OK;
+}
+
 int mfb_graph_destroy(void* graph_exec) {
   if (graph_exec) MFB_CUDA_TRY(cudaGraphExecDestroy((cudaGraphExec_t)graph_exec));
   return MFB_OK;

@@ -898,6 +898,24 @@ int make_tmap_bf16_heads(CUtensorMap* map, const void* base, uint64_t rows, int 
   return MFB_OK;
 }
 
+int make_tmap_16(CUtensorMap* map, const void* base, bool bf16, int rank, const uint64_t* dims,
+                 const uint64_t* strides, const uint32_t* box) {
+  auto fn = encode_fn();
+  if (!fn) return set_error(MFB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
+  cuuint64_t d[4] = {1, 1, 1, 1}, st[3] = {0, 0, 0};
+  cuuint32_t bx[4] = {1, 1, 1, 1}, estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    if (i + 1 < rank) st[i] = strides[i];
+  }
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                  const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(MFB_ERR_CUDA, "cuTensorMapEncodeTiled (rank %d) failed (%d)", rank, (int)r);
+  return MFB_OK;
+}
+
 int make_tmap_f32_rows_heads(CUtensorMap* map, const void* base, int heads, uint64_t T, uint64_t batch,
                              uint32_t box_rows) {
   auto fn = encode_fn();

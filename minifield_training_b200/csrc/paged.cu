@@ -1,0 +1,1223 @@
+// Attention of new tokens over a paged key/value cache: chunks of a prompt,
+// single decode tokens and ragged mixtures of both.
+//
+// Sequence b has seq_lens[b] cached tokens (the new ones included), token j in
+// row j % page_size of page page_table[b][j / page_size]; its new tokens are
+// rows [cu_q[b], cu_q[b + 1]) of q and sit at the end of the sequence. With
+// base = seq_lens[b] - (cu_q[b + 1] - cu_q[b]), query i attends to the keys
+// j <= base + i:
+//   o_i = sum_j p_ij v_j,  p_ij = softmax_j(scale q_i . k_j)
+// and a query without any key (base + i < 0) returns zeros.
+//
+// Floor: every live K/V row is read from HBM once per KV head; 4 D operations
+// per (query head, key) pair on the tensor cores and one exponential.
+//
+// Both kernels are persistent: a small schedule kernel lists the work items --
+// (sequence, KV heads, query rows) with their number of key tiles -- and cuts
+// the tiles of all items, in order, into equal contiguous shares, one per CTA.
+// A long context with few queries is thereby spread over the whole GPU and a
+// ragged batch stays balanced without the host knowing any length. Items cut
+// between CTAs leave FP32 partials (max, sum, output) in the workspace; the
+// last CTA to finish one (ticket, no waiting) joins them in CTA order.
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "tc.cuh"
+#include "types16.cuh"
+
+namespace mfb {
+namespace paged {
+
+constexpr int MAX_B = 8192;
+constexpr int MAX_SMS = 160;  // bounds the workspace: shares are at most 2 (few rows) or 1 (chunks) per SM
+
+__device__ int g_status;  // id of a bounded wait that gave up, or kBadPage / kBadLength
+constexpr int kBadPage = 1001, kBadLength = 1002;
+
+struct __align__(16) Item {
+  int b, hg;        // sequence, KV-head group
+  int tok0, ntok;   // query tokens: q rows tok0 .. tok0 + ntok - 1
+  int pos0;         // position of the first of them (negative: no keys yet)
+  int keys;         // keys the last one sees (0 if none)
+  int tiles, first; // key tiles (at least 1), and units before this item
+};
+
+struct Header {
+  int total, shares, items, pad;
+};
+
+struct Params {
+  const uint16_t* q;
+  uint16_t* o;
+  float* lse;
+  const int* cu_q;
+  const int* seq_lens;
+  const int* page_table;
+  Header* head;
+  Item* items;
+  int* starts;     // [grid] item holding each share's first unit
+  int* tickets;    // [items]
+  int* tickets_g;  // [2 * grid] first-level tickets of items cut into many parts
+  float* part_o;   // [slots][part_rows][D]
+  float2* part_ml; // [slots][part_rows]
+  int N, B, H, Hk, G, max_q, max_pages, num_pages, page_shift;
+  int tok_item;    // query tokens per item
+  int hc;          // KV heads per item
+  int unit;        // keys per unit
+  int min_units;   // units a share should hold at least
+  int grid, max_items, part_rows;
+  float scale_log2;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(v) : "r"(a));
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// Schedule: one block. Items of sequence b: head groups x query blocks.
+// ---------------------------------------------------------------------------
+constexpr int SCHED_THREADS = 1024;
+
+// Exclusive block scan of one int per thread; returns the prefix, total in *sum.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  __syncthreads();  // the previous scan's readers are done with warp_sums
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    warp_sums[lane] = w;
+  }
+  __syncthreads();
+  *sum = warp_sums[31];
+  return incl - v + (warp ? warp_sums[warp - 1] : 0);
+}
+
+// The share whose range [i * total / g, (i + 1) * total / g) holds unit x.
+__device__ __forceinline__ int share_of(int x, int total, int g) {
+  return (int)(((long long)(x + 1) * g + total - 1) / total) - 1;
+}
+__device__ __forceinline__ int share_begin(int i, int total, int g) { return (int)((long long)i * total / g); }
+
+// Query rows of sequence b inside q: arguments that contradict each other
+// (cu_q outside [0, N] or decreasing, more than max_q new tokens, lengths
+// outside the page table) are clamped, so no access leaves the buffers, and
+// recorded in the status word.
+__device__ __forceinline__ void sequence(const Params& p, int b, int* q0, int* nq, int* base, int* len) {
+  const int c0 = p.cu_q[b], c1 = p.cu_q[b + 1], s = p.seq_lens[b];
+  const int lo = min(max(c0, 0), p.N), hi = min(max(c1, lo), p.N);
+  const long long cap = (long long)p.max_pages << p.page_shift;
+  *q0 = lo;
+  *nq = min(hi - lo, p.max_q);
+  *len = (int)min((long long)max(s, 0), cap);
+  *base = *len - (hi - lo);
+  if (c0 != lo || c1 != hi || *nq != hi - lo || *len != s) atomicCAS(&g_status, 0, kBadLength);
+}
+
+__global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
+  allow_dependents();
+  extern __shared__ int item_base[];  // [B + 1] items before each sequence
+  __shared__ int warp_sums[32];
+  const int tid = threadIdx.x, groups = p.Hk / p.hc;
+  int carry = 0;
+  for (int b0 = 0; b0 < p.B; b0 += SCHED_THREADS) {
+    const int b = b0 + tid;
+    int q0, nq = 0, base, len, sum;
+    if (b < p.B) sequence(p, b, &q0, &nq, &base, &len);
+    const int pre = block_scan(cdiv(nq, p.tok_item) * groups, warp_sums, &sum);
+    if (b < p.B) item_base[b] = carry + pre;
+    carry += sum;
+  }
+  if (tid == 0) item_base[p.B] = carry;
+  __syncthreads();
+  const int items = min(carry, p.max_items);
+  auto make = [&](int i) {
+    int lo = 0, hi = p.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (item_base[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    int q0, nq, base, len;
+    sequence(p, lo, &q0, &nq, &base, &len);
+    const int blocks = cdiv(nq, p.tok_item), local = i - item_base[lo];
+    Item it;
+    it.b = lo;
+    it.hg = local / blocks;
+    const int t0 = (local % blocks) * p.tok_item;
+    it.tok0 = q0 + t0;
+    it.ntok = min(p.tok_item, nq - t0);
+    it.pos0 = base + t0;
+    it.keys = min(max(it.pos0 + it.ntok, 0), len);
+    it.tiles = max(1, cdiv(it.keys, p.unit));
+    it.first = 0;
+    return it;
+  };
+  // One pass of the items for their total, a second for prefixes and shares;
+  // with at most a block of items the first pass's item is kept.
+  Item mine{};
+  int total = 0;
+  for (int i0 = 0; i0 < items; i0 += SCHED_THREADS) {
+    const int i = i0 + tid;
+    int sum;
+    if (i < items) mine = make(i);
+    block_scan(i < items ? mine.tiles : 0, warp_sums, &sum);
+    total += sum;
+  }
+  const int g = max(1, min(p.grid, total / p.min_units));
+  carry = 0;
+  for (int i0 = 0; i0 < items; i0 += SCHED_THREADS) {
+    const int i = i0 + tid;
+    int sum;
+    if (i < items && items > SCHED_THREADS) mine = make(i);
+    const int pre = block_scan(i < items ? mine.tiles : 0, warp_sums, &sum);
+    if (i < items) {
+      mine.first = carry + pre;
+      p.items[i] = mine;
+      p.tickets[i] = 0;
+      // Shares whose first unit lies in this item.
+      const int end = mine.first + mine.tiles;
+      int s = share_of(mine.first, total, g);
+      if (share_begin(s, total, g) < mine.first) ++s;
+      for (; s < g && share_begin(s, total, g) < end; ++s) p.starts[s] = i;
+    }
+    carry += sum;
+  }
+  for (int i = tid; i < 2 * p.grid; i += SCHED_THREADS) p.tickets_g[i] = 0;
+  if (tid == 0) *p.head = Header{total, g, items, 0};
+}
+
+// ---------------------------------------------------------------------------
+// Joining the partials of a cut item. Segment (share c, which) owns a slot:
+// which = 0 where the share begins inside (or at) the item, 1 where the item
+// begins later in the share; only a share's first and last segment can be cut.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int slot_of(int c, int first_unit, int total, int g) {
+  return 2 * c + (share_begin(c, total, g) < first_unit ? 1 : 0);
+}
+
+// Joins `n` parts, part k in slot slot(k), for the float4 columns of `rows`
+// rows ([rows][D/4]) and hands each to emit(row, d4, m, l, o).
+template <int D, int NT, typename Slot, typename Emit>
+__device__ __forceinline__ void join(const Params& p, int n, int rows, int tid, Slot slot, Emit emit) {
+  for (int x = tid; x < rows * (D / 4); x += NT) {
+    const int row = x / (D / 4), d4 = x % (D / 4);
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < n; k += 8) {
+      float2 ml[8];
+      float4 ov[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        ml[u] = make_float2(-INFINITY, 0.f);
+        ov[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k + u < n) {
+          const long long at = (long long)slot(k + u) * p.part_rows + row;
+          ml[u] = __ldcg(p.part_ml + at);
+          ov[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + d4);
+        }
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) mn = fmaxf(mn, ml[u].x);
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float a = ex2(m - ref);
+      l *= a, acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = ex2(ml[u].x - ref);
+        l = fmaf(ml[u].y, w, l);
+        acc.x = fmaf(ov[u].x, w, acc.x);
+        acc.y = fmaf(ov[u].y, w, acc.y);
+        acc.z = fmaf(ov[u].z, w, acc.z);
+        acc.w = fmaf(ov[u].w, w, acc.w);
+      }
+      m = mn;
+    }
+    emit(row, d4, m, l, acc);
+  }
+}
+
+constexpr int JOIN = 16;  // shares joined per first-level group
+
+// Slot of group k of the item whose first share is c0, behind the segments'
+// slots. Items of several groups have more than JOIN shares each, so within
+// JOIN neighbouring shares at most one item has its first group and at most
+// one a later group.
+__device__ __forceinline__ int group_slot(const Params& p, int c0, int k) {
+  return 2 * p.grid + 2 * ((c0 + k * JOIN) / JOIN) + (k == 0 ? 1 : 0);
+}
+
+// This share's segment of a cut item is in its slot (written by the 256
+// threads of named barrier 1, which all call). Two levels: the last of each
+// JOIN neighbouring shares joins them into a slot of its group, the last such
+// group joins the groups and finishes the rows.
+template <int D, typename Finish>
+__device__ __forceinline__ void join_cut(const Params& p, const Item& w, int item, int share, int total, int g,
+                                         int rows, int tid, int* s_flag, Finish finish) {
+  const int c0 = share_of(w.first, total, g), c1 = share_of(w.first + w.tiles - 1, total, g);
+  const int k = (share - c0) / JOIN, grp0 = c0 + k * JOIN, gn = min(JOIN, c1 - grp0 + 1);
+  const int ngrp = cdiv(c1 - c0 + 1, JOIN);
+  auto meet = [] { asm volatile("bar.sync 1, 256;\n" ::: "memory"); };
+  __threadfence();
+  meet();
+  if (tid == 0) *s_flag = atomicAdd(p.tickets_g + slot_of(grp0, w.first, total, g), 1) == gn - 1;
+  meet();
+  if (*s_flag) {
+    __threadfence();
+    auto part = [&](int i) { return slot_of(grp0 + i, w.first, total, g); };
+    if (ngrp == 1) {
+      join<D, 256>(p, gn, rows, tid, part, finish);
+    } else {
+      const long long to = (long long)group_slot(p, c0, k) * p.part_rows;
+      join<D, 256>(p, gn, rows, tid, part, [&](int row, int d4, float m, float l, const float4& a) {
+        *reinterpret_cast<float4*>(p.part_o + (to + row) * D + d4 * 4) = a;
+        if (d4 == 0) p.part_ml[to + row] = make_float2(m, l);
+      });
+      __threadfence();
+      meet();
+      if (tid == 0) *s_flag = atomicAdd(p.tickets + item, 1) == ngrp - 1;
+      meet();
+      if (*s_flag) {
+        __threadfence();
+        join<D, 256>(p, ngrp, rows, tid, [&](int i) { return group_slot(p, c0, i); }, finish);
+      }
+    }
+  }
+  meet();  // s_flag may be written again
+}
+
+__device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY; }
+
+// Key tile boxes of one unit: rows of a page, at most the unit's.
+__device__ __forceinline__ int page_id(const Params& p, int b, int key) {
+  const int id = p.page_table[(long long)b * p.max_pages + (key >> p.page_shift)];
+  if ((unsigned)id < (unsigned)p.num_pages) return id;
+  atomicCAS(&g_status, 0, kBadPage);
+  return p.num_pages;  // outside the tensor: the load fills zeros
+}
+
+// 4-D tiled load, no multicast.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Few query rows per KV head (new tokens x group <= 16): bandwidth-bound.
+//
+// A unit is 128 / hc keys of hc KV heads: 16 KB of K and of V per 64 head
+// dims. A producer warp streams units through a ring (one TMA box per page
+// touched); eight compute warps take 16 keys of one head each on the
+// warp-level MMA (m16n8k16, the query rows as A: the kernel waits for memory,
+// not for these products), with an FP32 online softmax. Probabilities are
+// rounded to the cache's 16-bit type for the P.V product, as the fixed-capacity
+// decode does; their sum is taken before the rounding.
+// ---------------------------------------------------------------------------
+constexpr int DW = 8;                    // compute warps
+constexpr int D_THREADS = 32 * (DW + 1);
+
+struct DLayout {
+  uint32_t merge, bars, total;
+};
+__host__ __device__ inline DLayout dlayout(int D, int stages, int rows, int hc) {
+  DLayout L;
+  L.merge = (uint32_t)stages * 2u * 16384u * (uint32_t)(D / 64);
+  const uint32_t m = hc < 8 ? 8u * (uint32_t)rows * (uint32_t)(D + 4) * 4u : 0u;  // [warp][row]{o[D], m, l}
+  L.bars = L.merge + m;
+  L.total = 1024 + L.bars + 16u * (uint32_t)stages + 16u;
+  return L;
+}
+
+template <typename T, int D, bool R16>
+__global__ void __launch_bounds__(D_THREADS)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, Params p,
+                    int stages, int rows_max) {
+  constexpr int DH = D / 64;
+  constexpr uint32_t kStage = 2u * 16384u * DH;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t sb = smem_u32(smem);
+  const DLayout lay = dlayout(D, stages, rows_max, p.hc);
+  float* merge = reinterpret_cast<float*>(smem + lay.merge);
+  __shared__ int s_flag;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto full_bar = [&](int s) { return sb + lay.bars + 8u * s; };
+  auto empty_bar = [&](int s) { return sb + lay.bars + 8u * (stages + s); };
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) {
+      tc::mbar_init(full_bar(s), 1);
+      tc::mbar_init(empty_bar(s), DW);
+    }
+    tc::mbar_fence_init();
+    tc::tma_prefetch_desc(&tk);
+    tc::tma_prefetch_desc(&tv);
+  }
+  __syncthreads();
+  wait_prerequisites();
+  allow_dependents();
+  const Header head = *p.head;
+  const int total = head.total, g = head.shares, share = blockIdx.x;
+  if (share >= g || total == 0) return;
+  const int x0 = share_begin(share, total, g), x1 = share_begin(share + 1, total, g);
+  const int item0 = p.starts[share];
+  const int unit = p.unit, hc = p.hc;
+  const int br = min(unit, 1 << p.page_shift), nb = unit / br;  // box rows, boxes per unit
+
+  if (warp == DW) {
+    // Producer: lane i < nb looks up the page of box i one unit ahead; the
+    // boxes of K and V (and of both halves of 128-wide heads) are issued by
+    // the lanes in parallel, all counted on the stage's barrier.
+    int it = 0, item = item0;
+    bool ok = true;
+    for (int x = x0; ok && x < x1; ++item) {
+      const Item w = p.items[item];
+      const int u0 = x - w.first, u1 = min(w.tiles, x1 - w.first);
+      auto look = [&](int u) {
+        const int key = u * unit + lane * br;
+        return u < u1 && lane < nb && key < w.keys ? page_id(p, w.b, key) : 0;
+      };
+      int id = look(u0);
+      for (int u = u0; u < u1; ++u, ++it) {
+        const int st = it % stages;
+        const int next = look(u + 1);
+        if (!(ok = tc::mbar_wait_w(empty_bar(st), ((it / stages) & 1) ^ 1, &g_status, 1))) break;
+        const int live = min(nb, cdiv(max(w.keys - u * unit, 0), br));  // boxes that hold keys
+        const uint32_t box = (uint32_t)br * hc * 128u;
+        if (lane == 0) tc::mbar_expect_tx(full_bar(st), box * 2u * DH * live);
+        __syncwarp();
+        for (int j = lane; j - lane < live * 2 * DH; j += 32) {
+          const int bx = j % max(live, 1), rest = j / max(live, 1);  // rest: half, then K or V
+          const int pid = __shfl_sync(0xffffffffu, id, bx);
+          if (j < live * 2 * DH) {
+            const int half = rest % DH, kv = rest / DH;
+            const uint32_t dst = sb + st * kStage + kv * (kStage / 2) + half * 16384u + bx * box;
+            tma_load_4d(dst, kv ? &tv : &tk, half * 64, (u * unit + bx * br) & ((1 << p.page_shift) - 1), w.hg * hc,
+                        pid, full_bar(st));
+          }
+        }
+        id = next;
+      }
+      x = w.first + u1;
+    }
+    if (!ok)  // a wait gave up: let the copies in flight land before the CTA ends
+      for (int f = max(0, it - stages); f < it; ++f) tc::mbar_wait_w(full_bar(f % stages), (f / stages) & 1, &g_status, 3);
+    return;
+  }
+
+  // Compute warps: head hl of the item's hc, keys [16 sl, 16 sl + 16) of each unit.
+  const int hl = warp % hc, sl = warp / hc, slices = DW / hc;
+  const int g4 = lane >> 2, c4 = lane & 3;
+  // ldmatrix row offsets of this lane in a 64-dim half of a stage's K or V.
+  auto row_off = [&](int i) {
+    const int pos = sl * 16 + i;
+    return (uint32_t)((pos / br) * (br * hc * 128) + hl * br * 128 + (pos % br) * 128);
+  };
+  const int ki = (lane & 7) + ((lane >> 4) << 3), vi = (lane & 7) + ((lane >> 3) & 1) * 8;
+  const uint32_t koff = row_off(ki), voff = row_off(vi);
+  const int G = p.G;
+  int it = 0, item = item0;
+  bool ok = true;
+  for (int x = x0; x < x1; ++item) {
+    const Item w = p.items[item];
+    const int u0 = x - w.first, u1 = min(w.tiles, x1 - w.first);
+    const int rows = w.ntok * G, hk = w.hg * hc + hl;
+    uint32_t qa[D / 16][4];
+    int lim[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = g4 + 8 * e, t = r / G;
+      const bool live = r < rows && (R16 || e == 0);
+      lim[e] = live ? min(w.pos0 + t + 1, w.keys) : 0;
+      const uint16_t* qrow = p.q + ((long long)(w.tok0 + t) * p.H + hk * G + r % G) * D + 2 * c4;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qa[kk][e] = live ? *reinterpret_cast<const uint32_t*>(qrow + kk * 16) : 0u;
+        qa[kk][2 + e] = live ? *reinterpret_cast<const uint32_t*>(qrow + kk * 16 + 8) : 0u;
+      }
+    }
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int u = u0; u < u1; ++u, ++it) {
+      const int st = it % stages;
+      // After a wait that gave up the warp goes on without waiting, so that
+      // the named barriers below still meet.
+      if (ok) ok = tc::mbar_wait_w(full_bar(st), (it / stages) & 1, &g_status, 2);
+      if (ok) {
+        const uint32_t kt = sb + st * kStage, vt = kt + kStage / 2;
+        const int key0 = u * unit + sl * 16;
+        if (key0 < w.keys) {
+          float sc[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t f[4];
+            const int chunk = ((kk & 3) * 2 + ((lane >> 3) & 1)) ^ (ki & 7);
+            ldmatrix_x4(kt + (kk >> 2) * 16384 + koff + chunk * 16, f[0], f[1], f[2], f[3]);
+            Num16<T>::mma(sc[0], qa[kk], f);
+            Num16<T>::mma(sc[1], qa[kk], f + 2);
+          }
+          float v[2][4];  // [row half][key of this lane]
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+                v[e][2 * n + c] = key0 + n * 8 + 2 * c4 + c < lim[e] ? sc[n][2 * e + c] * p.scale_log2 : -INFINITY;
+          uint32_t pa[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int e = 0; e < (R16 ? 2 : 1); ++e) {
+            float mx = fmaxf(fmaxf(v[e][0], v[e][1]), fmaxf(v[e][2], v[e][3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float mn = fmaxf(m[e], mx);
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            const float a = ex2(m[e] - ref);
+            m[e] = mn;
+            float pr[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) pr[c] = ex2(v[e][c] - ref);
+            l[e] = fmaf(l[e], a, (pr[0] + pr[1]) + (pr[2] + pr[3]));
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) o[n][2 * e] *= a, o[n][2 * e + 1] *= a;
+            pa[e] = Num16<T>::pack2(pr[0], pr[1]);
+            pa[2 + e] = Num16<T>::pack2(pr[2], pr[3]);
+          }
+          // Rows of V past the sequence hold whatever the page (or the ring)
+          // held: zeros in their place, since 0 x NaN would not vanish.
+          const bool tail = key0 + 16 > w.keys;
+          uint32_t keep[2];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int k = key0 + n * 8 + 2 * c4;
+            keep[n] = (k < w.keys ? 0xFFFFu : 0u) | (k + 1 < w.keys ? 0xFFFF0000u : 0u);
+          }
+#pragma unroll
+          for (int nd = 0; nd < D / 16; ++nd) {
+            uint32_t f[4];
+            const int chunk = ((nd & 3) * 2 + (lane >> 4)) ^ (vi & 7);
+            ldmatrix_x4_trans(vt + (nd >> 2) * 16384 + voff + chunk * 16, f[0], f[1], f[2], f[3]);
+            if (tail) f[0] &= keep[0], f[1] &= keep[1], f[2] &= keep[0], f[3] &= keep[1];
+            Num16<T>::mma(o[2 * nd], pa, f);
+            Num16<T>::mma(o[2 * nd + 1], pa, f + 2);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(empty_bar(st));
+    }
+    x = w.first + u1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+    }
+    const int c0 = share_of(w.first, total, g), c1 = share_of(w.first + w.tiles - 1, total, g);
+    const bool cut = c0 != c1;
+    const int slot = slot_of(share, w.first, total, g);
+    auto finish = [&](int row, int h, int d4, float mm, float ll, const float4& a) {
+      const float inv = ll > 0.f ? 1.f / ll : 0.f;
+      const long long at = (long long)(w.tok0 + row / G) * p.H + (w.hg * hc + h) * G + row % G;
+      uint2 out;
+      out.x = Num16<T>::pack2(a.x * inv, a.y * inv);
+      out.y = Num16<T>::pack2(a.z * inv, a.w * inv);
+      *reinterpret_cast<uint2*>(p.o + at * D + d4 * 4) = out;
+      if (p.lse && d4 == 0) p.lse[at] = lse_of(mm, ll);
+    };
+    auto finish_row = [&](int rh, int d4, float mm, float ll, const float4& a) { finish(rh / hc, rh % hc, d4, mm, ll, a); };
+    if (slices == 1) {
+#pragma unroll
+      for (int e = 0; e < (R16 ? 2 : 1); ++e) {
+        const int r = g4 + 8 * e;
+        if (r >= rows) continue;
+        if (!cut) {
+          const float inv = l[e] > 0.f ? 1.f / l[e] : 0.f;
+          const long long at = (long long)(w.tok0 + r / G) * p.H + hk * G + r % G;
+          uint16_t* orow = p.o + at * D + 2 * c4;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<uint32_t*>(orow + n * 8) = Num16<T>::pack2(o[n][2 * e] * inv, o[n][2 * e + 1] * inv);
+          if (p.lse && c4 == 0) p.lse[at] = lse_of(m[e], l[e]);
+        } else {
+          const long long at = (long long)slot * p.part_rows + r * hc + hl;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(p.part_o + at * D + n * 8 + 2 * c4) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
+          if (c4 == 0) p.part_ml[at] = make_float2(m[e], l[e]);
+        }
+      }
+    } else {
+      // Join the warps that share a head through shared memory.
+#pragma unroll
+      for (int e = 0; e < (R16 ? 2 : 1); ++e) {
+        const int r = g4 + 8 * e;
+        if (r >= rows) continue;
+        float* dst = merge + (warp * rows_max + r) * (D + 4);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float2*>(dst + n * 8 + 2 * c4) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
+        if (c4 == 0) dst[D] = m[e], dst[D + 1] = l[e];
+      }
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");
+      for (int y = tid; y < rows * hc * (D / 4); y += 32 * DW) {
+        const int d4 = y % (D / 4), rh = y / (D / 4), r = rh / hc, h = rh % hc;
+        float mm = -INFINITY, ll = 0.f;
+        for (int s = 0; s < slices; ++s) mm = fmaxf(mm, merge[((s * hc + h) * rows_max + r) * (D + 4) + D]);
+        const float ref = mm == -INFINITY ? 0.f : mm;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < slices; ++s) {
+          const float* src = merge + ((s * hc + h) * rows_max + r) * (D + 4);
+          const float wgt = ex2(src[D] - ref);
+          const float4 v4 = *reinterpret_cast<const float4*>(src + d4 * 4);
+          ll = fmaf(src[D + 1], wgt, ll);
+          a.x = fmaf(v4.x, wgt, a.x), a.y = fmaf(v4.y, wgt, a.y);
+          a.z = fmaf(v4.z, wgt, a.z), a.w = fmaf(v4.w, wgt, a.w);
+        }
+        if (!cut) {
+          finish_row(rh, d4, mm, ll, a);
+        } else {
+          const long long at = (long long)slot * p.part_rows + r * hc + h;
+          *reinterpret_cast<float4*>(p.part_o + at * D + d4 * 4) = a;
+          if (d4 == 0) p.part_ml[at] = make_float2(mm, ll);
+        }
+      }
+      if (!cut) asm volatile("bar.sync 1, 256;\n" ::: "memory");  // before the area is written again
+    }
+    if (cut) join_cut<D>(p, w, item, share, total, g, rows * hc, tid, &s_flag, finish_row);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many query rows: tcgen05.
+//
+// An item is one KV head and up to 2 x 128 query rows, row r of a tile being
+// (token r / G, head r % G of the group): every query head of the group and
+// every token share the K/V tiles. Units are 128 keys.
+//   warp 0      producer: Q tiles per item, K and V tiles (one TMA box per
+//               page touched) through one ring, in the order they are used
+//   warp 1      TMEM owner and MMA issuer (whole warp, one elected lane)
+//   warps 2-9   softmax: two groups of four, a group per S accumulator, one
+//               query row (TMEM lane) per thread
+// S = Q K^T (TMEM), P = 2^(scale S - M) rounded to the cache's 16-bit type in
+// place of S, O += P V (TMEM); the sum of P is kept in FP32 before rounding.
+// M moves only when a row's maximum has risen by more than 2^8, the row's O
+// and sum then being rescaled.
+// Items of more than 128 rows give each group one of the two query tiles;
+// smaller ones give both groups the same queries and alternate key tiles
+// between them, so that softmax and tensor core overlap either way; the two
+// accumulators are then joined in the epilogue.
+// ---------------------------------------------------------------------------
+constexpr int T_THREADS = 320;
+
+template <int D>
+struct TShape {
+  static constexpr int DH = D / 64;
+  static constexpr uint32_t SLOT = 16384u * DH;  // one K or V tile
+  static constexpr int SLOTS = D == 64 ? 10 : 5;
+  static constexpr uint32_t Q = 0, RING = 2 * SLOT, ML = RING + SLOTS * SLOT;  // ML: (max, sum) of group 1's rows
+  static constexpr uint32_t BARS = ML + 1024;
+  static constexpr uint32_t TOTAL = 1024 + BARS + 8 * (2 * SLOTS + 13);
+};
+
+// Instruction descriptor of kind::f16 with FP32 accumulation; A and B bf16 or fp16.
+__host__ __device__ constexpr uint32_t idesc16(bool bf, int N, int b_mn) {
+  return (1u << 4) | ((bf ? 1u : 0u) << 7) | ((bf ? 1u : 0u) << 10) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(T_THREADS, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                 const __grid_constant__ CUtensorMap tv, Params p) {
+  using S = TShape<D>;
+  constexpr int DH = S::DH;
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t sb = smem_u32(smem), bars = sb + S::BARS;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (S::SLOTS + s); };
+  const uint32_t q_full = bars + 8u * (2 * S::SLOTS), q_empty = q_full + 8, tail_bar = q_full + 16;
+  auto s_full = [&](int g) { return q_full + 24 + 8u * g; };
+  auto p_full = [&](int g) { return q_full + 40 + 8u * g; };
+  auto o_full = [&](int g) { return q_full + 56 + 8u * g; };
+  const uint32_t o_free = q_full + 72, done_bar = q_full + 80;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 8 * (2 * S::SLOTS + 11));
+  __shared__ int s_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int* status = &g_status;
+
+  if (tid == 0) {
+    for (int s = 0; s < S::SLOTS; ++s) {
+      tc::mbar_init(full_bar(s), 1);
+      tc::mbar_init(empty_bar(s), 1);
+    }
+    tc::mbar_init(q_full, 1);
+    tc::mbar_init(q_empty, 1);
+    tc::mbar_init(tail_bar, 1);
+    for (int g = 0; g < 2; ++g) {
+      tc::mbar_init(s_full(g), 1);
+      tc::mbar_init(p_full(g), 128);
+      tc::mbar_init(o_full(g), 1);
+    }
+    tc::mbar_init(o_free, 256);
+    tc::mbar_init(done_bar, 1);
+    tc::mbar_fence_init();
+    tc::tma_prefetch_desc(&tq);
+    tc::tma_prefetch_desc(&tk);
+    tc::tma_prefetch_desc(&tv);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(smem_u32(tmem_slot), 512);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  wait_prerequisites();
+  allow_dependents();
+  const Header head = *p.head;
+  const int total = head.total, g_n = head.shares, share = blockIdx.x;
+  const bool idle = share >= g_n || total == 0;
+  const int x0 = idle ? 0 : share_begin(share, total, g_n), x1 = idle ? 0 : share_begin(share + 1, total, g_n);
+  const int item0 = idle ? 0 : p.starts[share];
+  const int G = p.G, tpt = 128 / G;  // tokens per query tile
+  const int page = 1 << p.page_shift, br = min(128, page), nb = 128 / br;
+
+  if (warp == 0) {
+    int slot = 0, slot_ph = 0, fills = 0, seg = 0, tails = 0, item = item0;
+    bool ok = true;
+    for (int x = x0; ok && x < x1; ++item, ++seg) {
+      const Item w = p.items[item];
+      const int j0 = x - w.first, j1 = min(w.tiles, x1 - w.first), n = j1 - j0;
+      const bool dual = w.ntok > tpt;
+      const int delay = dual ? 1 : 2;
+      if (!(ok = tc::mbar_wait_w(q_empty, (seg & 1) ^ 1, status, 11))) break;
+      if (lane == 0) {
+        const int tiles = dual ? 2 : 1;
+        tc::mbar_expect_tx(q_full, (uint32_t)(tiles * DH * tpt * G * 128));
+        for (int t = 0; t < tiles; ++t)
+          for (int h = 0; h < DH; ++h)
+            tc::tma_load_3d(sb + S::Q + t * S::SLOT + h * 16384u, &tq, h * 64, w.hg * G, w.tok0 + t * tpt, q_full);
+      }
+      __syncwarp();
+      auto look = [&](int j) {
+        const int key = j * 128 + lane * br;
+        return j < j1 && lane < nb && key < w.keys ? page_id(p, w.b, key) : 0;
+      };
+      // Page ids of the next K tile and of the tiles whose V is still to come.
+      int id_next = look(j0), id_v0 = 0, id_v1 = 0;
+      auto load = [&](const CUtensorMap* map, int j, int id, bool is_v) {
+        if (!(ok = tc::mbar_wait_w(empty_bar(slot), slot_ph ^ 1, status, 12))) return;
+        const int valid = min(128, w.keys - j * 128), live = cdiv(max(valid, 0), br);
+        const bool tail = is_v && valid < 128;
+        const uint32_t bar = tail ? tail_bar : full_bar(slot), dst = sb + S::RING + slot * S::SLOT;
+        if (lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(live * br * 128 * DH));
+        __syncwarp();
+        const int bx = lane % max(live, 1), half = lane / max(live, 1);
+        const int pid = __shfl_sync(0xffffffffu, id, bx);
+        if (half < DH && lane < live * DH)
+          tma_load_4d(dst + half * 16384u + bx * br * 128, map, half * 64, (j * 128 + bx * br) & (page - 1), w.hg, pid, bar);
+        if (tail) {
+          // Rows past the sequence hold whatever the page (or the ring) held;
+          // zeros in their place, since 0 x NaN would not vanish in P V.
+          ok = tc::mbar_wait_w(tail_bar, tails & 1, status, 13);
+          ++tails;
+          for (int i = max(valid, 0) * 8 + lane; i < 128 * 8; i += 32)
+            for (int h = 0; h < DH; ++h)
+              *reinterpret_cast<uint4*>(smem + S::RING + slot * S::SLOT + h * 16384u + i * 16) = make_uint4(0, 0, 0, 0);
+          tc::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(full_bar(slot));
+        }
+        ++fills;
+        if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+      };
+      for (int it = 0; ok && it < n + delay; ++it) {
+        const int id_k = id_next;
+        if (it + 1 < n) id_next = look(j0 + it + 1);
+        if (it >= delay) {
+          load(&tv, j0 + it - delay, dual ? id_v0 : id_v1, true);
+          if (!ok) break;
+        }
+        if (it < n) load(&tk, j0 + it, id_k, false);
+        id_v1 = id_v0;
+        id_v0 = id_k;
+      }
+      x = w.first + j1;
+    }
+    if (!ok)  // a wait gave up: let the copies in flight land before the CTA ends
+      for (int f = max(0, fills - S::SLOTS); f < fills; ++f)
+        tc::mbar_wait_w(full_bar(f % S::SLOTS), (f / S::SLOTS) & 1, status, 14);
+  } else if (warp == 1) {
+    const uint32_t idesc_s = idesc16(BF, 128, 0), idesc_o = idesc16(BF, D, 1);
+    int slot = 0, slot_ph = 0, seg = 0, item = item0;
+    int np[2] = {0, 0};  // P tiles consumed, per group
+    bool ok = true;
+    for (int x = x0; ok && x < x1; ++item, ++seg) {
+      const Item w = p.items[item];
+      const int j0 = x - w.first, j1 = min(w.tiles, x1 - w.first), n = j1 - j0;
+      const bool dual = w.ntok > tpt;
+      const int delay = dual ? 1 : 2;
+      if (!(ok = tc::mbar_wait_w(q_full, seg & 1, status, 21))) break;
+      tc::tc_fence_after();
+      for (int it = 0; ok && it < n + delay; ++it) {
+        const bool do_pv = it >= delay, do_qk = it < n;
+        int vs = 0, ks = 0;
+        if (do_pv) {
+          vs = slot;
+          if (!(ok = tc::mbar_wait_w(full_bar(vs), slot_ph, status, 22))) break;
+          if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+        }
+        if (do_qk) {
+          ks = slot;
+          if (!(ok = tc::mbar_wait_w(full_bar(ks), slot_ph, status, 23))) break;
+          if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+        }
+        tc::tc_fence_after();
+        // The output accumulators of the previous item are read out.
+        if (it == delay && !(ok = tc::mbar_wait_w(o_free, (seg & 1) ^ 1, status, 24))) break;
+        const int g_lo = dual ? 0 : (it & 1), g_hi = dual ? 1 : (it & 1);
+        for (int g = g_lo; ok && g <= g_hi; ++g) {
+          const uint32_t s_t = tmem + g * 128, o_t = tmem + 256 + g * D;
+          if (do_pv) {
+            if (!(ok = tc::mbar_wait_w(p_full(g), np[g] & 1, status, 25))) break;
+            ++np[g];
+            tc::tc_fence_after();
+            const uint32_t vb = sb + S::RING + vs * S::SLOT;
+            const bool first = dual ? it == 1 : it < 4;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              tc::mma_bf16_ts_w(o_t, s_t + k * 8, tc::smem_desc_sw128(vb + k * 2048, 16384, 1024), idesc_o,
+                                (first && k == 0) ? 0u : 1u);
+            if (it >= n) tc::mma_commit_w(o_full(g));  // the group's last product of the item
+          }
+          if (do_qk) {
+            const uint32_t qb = sb + S::Q + (dual ? g : 0) * S::SLOT, kb = sb + S::RING + ks * S::SLOT;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              tc::mma_bf16_w(s_t, tc::smem_desc_sw128(qb + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
+                             tc::smem_desc_sw128(kb + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
+            tc::mma_commit_w(s_full(g));
+          }
+        }
+        if (!ok) break;
+        if (do_pv) tc::mma_commit_w(empty_bar(vs));
+        if (do_qk) tc::mma_commit_w(empty_bar(ks));
+        if (it == n - 1) tc::mma_commit_w(q_empty);
+      }
+      x = w.first + j1;
+    }
+    tc::mma_commit_w(done_bar);
+    tc::mbar_wait_w(done_bar, 0, status, 26);
+  } else {
+    const int grp = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane, stid = tid - 64;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_t = tmem + lane_off + grp * 128, o_t = tmem + lane_off + 256 + grp * D;
+    float2* ml_s = reinterpret_cast<float2*>(smem + S::ML);
+    const float sl2 = p.scale_log2;
+    int ns = 0, item = item0;
+    int no[2] = {0, 0};  // items whose output each group has had
+    bool ok = true;
+    for (int x = x0; x < x1; ++item) {
+      const Item w = p.items[item];
+      const int j0 = x - w.first, j1 = min(w.tiles, x1 - w.first), n = j1 - j0;
+      const bool dual = w.ntok > tpt;
+      const int t = (dual ? grp * tpt : 0) + r / G;
+      const bool live = r < tpt * G && t < w.ntok;
+      const bool warp_live = __any_sync(0xffffffffu, live);
+      // Keys this row sees; rows that do not exist mask nothing and are never read.
+      const int limit = live ? min(w.pos0 + t + 1, w.keys) : 0x7fffffff;
+      float M = -INFINITY, l = 0.f;
+      for (int it = dual ? 0 : grp; it < n; it += dual ? 1 : 2, ++ns) {
+        if (ok) ok = tc::mbar_wait_w(s_full(grp), ns & 1, status, 31);
+        if (!ok) break;
+        if (warp_live) {
+          tc::tc_fence_after();
+          uint32_t v[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tc::tmem_ld_32x32b_x32(s_t + c * 32, v + c * 32);
+          tc::tmem_ld_wait();
+          const int lim = limit - (j0 + it) * 128;
+          if (__any_sync(0xffffffffu, lim < 128)) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) v[i] = i < lim ? v[i] : 0xFF800000u;
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 128; i += 4) {
+            mx[0] = fmaxf(mx[0], __uint_as_float(v[i]));
+            mx[1] = fmaxf(mx[1], __uint_as_float(v[i + 1]));
+            mx[2] = fmaxf(mx[2], __uint_as_float(v[i + 2]));
+            mx[3] = fmaxf(mx[3], __uint_as_float(v[i + 3]));
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+          // The group's previous product has landed: its commit precedes s_full's.
+          const bool up = top > M + 8.f;
+          if (__any_sync(0xffffffffu, up && M != -INFINITY)) {
+            const float a = (up && M != -INFINITY) ? ex2(M - top) : 1.f;
+            l *= a;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t ov[16];
+              tc::tmem_ld_32x32b_x16(o_t + c * 16, ov);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * a);
+              tc::tmem_st_32x32b_x16(o_t + c * 16, ov);
+            }
+          }
+          if (up) M = top;
+          const float neg = M == -INFINITY ? 0.f : -M;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float e0 = ex2(fmaf(__uint_as_float(v[c * 32 + i]), sl2, neg));
+              const float e1 = ex2(fmaf(__uint_as_float(v[c * 32 + i + 1]), sl2, neg));
+              sum[i & 2] += e0;
+              sum[(i & 2) + 1] += e1;
+              pk[i >> 1] = Num16<T>::pack2(e0, e1);
+            }
+            tc::tmem_st_32x32b_x16(s_t + c * 16, pk);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tc::tmem_st_wait();
+          tc::tc_fence_before();
+        }
+        tc::mbar_arrive(p_full(grp));
+      }
+      x = w.first + j1;
+
+      // Epilogue: this group's rows (dual), or both groups' accumulators of
+      // the same rows joined by group 0.
+      const bool has1 = dual || n > 1, cut = j0 > 0 || j1 < w.tiles;
+      float a0 = 1.f, a1 = 0.f;
+      if (!dual) {
+        if (grp == 1) ml_s[r] = make_float2(M, l);
+        asm volatile("bar.sync 1, 256;\n" ::: "memory");
+        const float2 o = ml_s[r];
+        asm volatile("bar.sync 1, 256;\n" ::: "memory");  // before the next item's are written
+        if (grp == 0 && has1) {
+          const float top = fmaxf(M, o.x), ref = top == -INFINITY ? 0.f : top;
+          a0 = ex2(M - ref);
+          a1 = ex2(o.x - ref);
+          l = l * a0 + o.y * a1;
+          M = top;
+        }
+      }
+      const bool store = live && (dual || grp == 0);
+      if ((dual || grp == 0) && ok) {
+        ok = tc::mbar_wait_w(o_full(grp), no[grp] & 1, status, 32);
+        if (ok && !dual && has1) ok = tc::mbar_wait_w(o_full(1), no[1] & 1, status, 33);
+        if (ok && warp_live) {
+          tc::tc_fence_after();
+          const float inv = cut ? 1.f : (l > 0.f ? 1.f / l : 0.f);
+          const float f0 = a0 * inv, f1 = a1 * inv;
+          const long long at = (long long)(w.tok0 + t) * p.H + w.hg * G + r % G;
+          const long long pr = (long long)slot_of(share, w.first, total, g_n) * p.part_rows + t * G + r % G;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t ov[32];
+            tc::tmem_ld_32x32b_x32(o_t + c * 32, ov);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * f0);
+            if (!dual && has1) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t o1[16];
+                tc::tmem_ld_32x32b_x16(o_t + D + c * 32 + h * 16, o1);
+                tc::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  ov[h * 16 + e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), f1, __uint_as_float(ov[h * 16 + e])));
+              }
+            }
+            if (!store) continue;
+            if (cut) {
+              float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + c * 32);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                dst[e] = make_float4(__uint_as_float(ov[4 * e]), __uint_as_float(ov[4 * e + 1]),
+                                     __uint_as_float(ov[4 * e + 2]), __uint_as_float(ov[4 * e + 3]));
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(p.o + at * D + c * 32);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(ov[8 * e + i]);
+                dst[e] = pack16x8<T>(f);
+              }
+            }
+          }
+          if (store && cut) p.part_ml[pr] = make_float2(M, l);
+          if (store && !cut && p.lse) p.lse[at] = lse_of(M, l);
+          tc::tc_fence_before();
+        }
+      }
+      ++no[0];
+      if (has1) ++no[1];
+      tc::mbar_arrive(o_free);
+      if (cut)
+        join_cut<D>(p, w, item, share, total, g_n, w.ntok * G, stid, &s_flag,
+                    [&](int row, int d4, float mm, float ll, const float4& a) {
+                      const float inv = ll > 0.f ? 1.f / ll : 0.f;
+                      const long long at = (long long)(w.tok0 + row / G) * p.H + w.hg * G + row % G;
+                      uint2 out;
+                      out.x = Num16<T>::pack2(a.x * inv, a.y * inv);
+                      out.y = Num16<T>::pack2(a.z * inv, a.w * inv);
+                      *reinterpret_cast<uint2*>(p.o + at * D + d4 * 4) = out;
+                      if (p.lse && d4 == 0) p.lse[at] = lse_of(mm, ll);
+                    });
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+constexpr size_t MAX_SMEM = 227 * 1024 - 64;  // dynamic part of a CTA's shared memory
+constexpr int FEW_ROWS = 16;  // query rows per KV head the warp-level kernel takes
+
+struct Plan {
+  bool few;
+  int hc, unit, tok_item, grid_cap, max_items, part_rows, slots;
+  size_t bytes;
+};
+
+Plan plan(int N, int B, int max_q, int H, int Hk, int D) {
+  Plan pl{};
+  const int G = H / Hk;
+  pl.few = (long long)max_q * G <= FEW_ROWS;
+  if (pl.few) {
+    pl.hc = Hk % 8 == 0 ? 8 : Hk % 4 == 0 ? 4 : Hk % 2 == 0 ? 2 : 1;
+    pl.unit = 128 / pl.hc;
+    pl.tok_item = max_q;
+    pl.grid_cap = 2 * MAX_SMS;
+    pl.max_items = B * (Hk / pl.hc);
+    pl.part_rows = max_q * G * pl.hc;
+  } else {
+    pl.hc = 1;
+    pl.unit = 128;
+    pl.tok_item = 2 * (128 / G);
+    pl.grid_cap = MAX_SMS;
+    pl.max_items = Hk * (N / pl.tok_item + B);
+    pl.part_rows = 256;
+  }
+  pl.slots = 2 * pl.grid_cap + 2 * (pl.grid_cap / JOIN + 1);
+  pl.bytes = 256 + align256(sizeof(Item) * (size_t)pl.max_items) + align256(sizeof(int) * (size_t)pl.max_items) +
+             align256(sizeof(int) * 3 * (size_t)pl.grid_cap) +
+             align256(sizeof(float) * (size_t)pl.slots * pl.part_rows * D) +
+             align256(sizeof(float2) * (size_t)pl.slots * pl.part_rows);
+  return pl;
+}
+
+void carve(Params& p, const Plan& pl, void* base, int D) {
+  char* c = static_cast<char*>(base);
+  auto take = [&](size_t n) {
+    char* r = c;
+    c += align256(n);
+    return r;
+  };
+  p.head = reinterpret_cast<Header*>(take(sizeof(Header)));
+  p.items = reinterpret_cast<Item*>(take(sizeof(Item) * (size_t)pl.max_items));
+  p.tickets = reinterpret_cast<int*>(take(sizeof(int) * (size_t)pl.max_items));
+  p.starts = reinterpret_cast<int*>(take(sizeof(int) * 3 * (size_t)pl.grid_cap));
+  p.tickets_g = p.starts + pl.grid_cap;
+  p.part_o = reinterpret_cast<float*>(take(sizeof(float) * (size_t)pl.slots * pl.part_rows * D));
+  p.part_ml = reinterpret_cast<float2*>(take(sizeof(float2) * (size_t)pl.slots * pl.part_rows));
+}
+
+// {dim, row of the page, KV head, page}; box {64, rows, heads, 1}.
+int make_tmap_pages(CUtensorMap* map, const void* base, bool bf, int D, int page_size, int Hk, int num_pages,
+                    bool head_major, int box_rows, int box_heads) {
+  const uint64_t token = (uint64_t)(head_major ? D : Hk * D) * 2, head = (uint64_t)(head_major ? page_size * D : D) * 2;
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page_size, (uint64_t)Hk, (uint64_t)num_pages};
+  const uint64_t strides[3] = {token, head, (uint64_t)page_size * Hk * D * 2};
+  const uint32_t box[4] = {64, (uint32_t)box_rows, (uint32_t)box_heads, 1};
+  return tc::make_tmap_16(map, base, bf, 4, dims, strides, box);
+}
+
+template <typename T, int D, bool R16>
+int run_few(Params& p, const Plan& pl, const CUtensorMap& tk, const CUtensorMap& tv, int sms, cudaStream_t s) {
+  const int rows = p.max_q * p.G;
+  int stages = 3;
+  while (stages > 2 && dlayout(D, stages, rows, pl.hc).total > MAX_SMEM) --stages;
+  const size_t smem = dlayout(D, stages, rows, pl.hc).total;
+  MFB_CUDA_TRY(cudaFuncSetAttribute(few_rows_kernel<T, D, R16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MAX_SMEM));
+  const int per_sm = 2 * smem + 4096 <= 228 * 1024 ? 2 : 1;
+  p.grid = std::min(per_sm * sms, pl.grid_cap);
+  schedule_kernel<<<1, SCHED_THREADS, sizeof(int) * (size_t)(p.B + 1), s>>>(p);
+  MFB_LAUNCH_CHECK("paged attention schedule");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.grid);
+  cfg.blockDim = dim3(D_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MFB_CUDA_TRY(cudaLaunchKernelEx(&cfg, few_rows_kernel<T, D, R16>, tk, tv, p, stages, rows));
+  return MFB_OK;
+}
+
+template <typename T, int D>
+int run(Params& p, const Plan& pl, const void* q, const void* kp, const void* vp, int page_size, bool head_major,
+        cudaStream_t s) {
+  constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+  int dev = 0, sms = 148, st;
+  MFB_CUDA_TRY(cudaGetDevice(&dev));
+  MFB_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  sms = std::min(sms, MAX_SMS);
+  CUtensorMap tk, tv, tq;
+  const int br = std::min(pl.unit, page_size);
+  if ((st = make_tmap_pages(&tk, kp, bf, D, page_size, p.Hk, p.num_pages, head_major, br, pl.hc))) return st;
+  if ((st = make_tmap_pages(&tv, vp, bf, D, page_size, p.Hk, p.num_pages, head_major, br, pl.hc))) return st;
+  if (pl.few) {
+    p.min_units = 4;
+    return p.max_q * p.G <= 8 ? run_few<T, D, false>(p, pl, tk, tv, sms, s) : run_few<T, D, true>(p, pl, tk, tv, sms, s);
+  }
+  p.min_units = 2;
+  const uint64_t dims[3] = {(uint64_t)D, (uint64_t)p.H, (uint64_t)p.N};
+  const uint64_t strides[2] = {(uint64_t)D * 2, (uint64_t)p.H * D * 2};
+  const uint32_t box[3] = {64, (uint32_t)p.G, (uint32_t)(128 / p.G)};
+  if ((st = tc::make_tmap_16(&tq, q, bf, 3, dims, strides, box))) return st;
+  constexpr size_t smem = TShape<D>::TOTAL;
+  static_assert(smem <= MAX_SMEM, "chunk kernel shared memory");
+  MFB_CUDA_TRY(cudaFuncSetAttribute(chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  p.grid = sms;
+  schedule_kernel<<<1, SCHED_THREADS, sizeof(int) * (size_t)(p.B + 1), s>>>(p);
+  MFB_LAUNCH_CHECK("paged attention schedule");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.grid);
+  cfg.blockDim = dim3(T_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MFB_CUDA_TRY(cudaLaunchKernelEx(&cfg, chunk_kernel<T, D>, tq, tk, tv, p));
+  return MFB_OK;
+}
+
+}  // namespace paged
+}  // namespace mfb
+
+using namespace mfb;
+
+extern "C" size_t mfb_paged_attn_workspace_size(int N, int B, int max_q, int H, int Hk, int D) {
+  if (N <= 0 || B <= 0 || B > paged::MAX_B || max_q <= 0 || H <= 0 || Hk <= 0 || H % Hk || H / Hk > 128 || D <= 0)
+    return 0;
+  return paged::plan(N, B, max_q, H, Hk, D).bytes;
+}
+
+extern "C" int mfb_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* cu_q,
+                              const int32_t* seq_lens, const int32_t* page_table, void* o, float* lse, int N, int B,
+                              int max_q, int max_pages, int num_pages, int page_size, int H, int Hk, int D,
+                              int head_major, int dtype, float scale, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  MFB_CHECK_ARG(N > 0 && B > 0 && max_q > 0 && max_pages > 0 && num_pages > 0,
+                "paged attention needs tokens, sequences and pages (N=%d B=%d max_q=%d)", N, B, max_q);
+  MFB_CHECK_ARG(B <= paged::MAX_B, "paged attention batch %d above the supported %d sequences", B, paged::MAX_B);
+  MFB_CHECK_ARG(H > 0 && Hk > 0 && H % Hk == 0, "Query heads must be divisible by KV heads (H=%d Hk=%d)", H, Hk);
+  MFB_CHECK_ARG(H / Hk <= 128 && Hk <= 1024, "paged attention supports up to 1024 KV heads of 128 query heads (H=%d Hk=%d)",
+                H, Hk);
+  MFB_CHECK_ARG(D == 64 || D == 128, "paged attention head_dim %d unsupported (64 or 128)", D);
+  MFB_CHECK_ARG(page_size >= 8 && (page_size & (page_size - 1)) == 0,
+                "page_size %d must be a power of two of at least 8", page_size);
+  MFB_CHECK_ARG((long long)page_size * Hk * D <= 1 << 30, "page of %d tokens too large", page_size);
+  MFB_CHECK_ARG((long long)max_pages * page_size < (1LL << 31) - 128, "page table spans %lld positions (below 2^31 supported)",
+                (long long)max_pages * page_size);
+  MFB_CHECK_ARG(dtype == MFB_DTYPE_BF16 || dtype == MFB_DTYPE_F16, "paged attention dtype must be bf16 or fp16");
+  MFB_CHECK_ARG(q && k_pages && v_pages && cu_q && seq_lens && page_table && o, "NULL paged attention argument");
+  MFB_CHECK_ARG((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o) & 15) == 0,
+                "q, the pages and o must be 16-byte aligned");
+  const paged::Plan pl = paged::plan(N, B, max_q, H, Hk, D);
+  if (!workspace || workspace_bytes < pl.bytes)
+    return set_error(MFB_ERR_WORKSPACE, "paged attention workspace needs %zu bytes", pl.bytes);
+  MFB_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");
+  paged::Params p{};
+  p.q = (const uint16_t*)q;
+  p.o = (uint16_t*)o;
+  p.lse = lse;
+  p.cu_q = cu_q;
+  p.seq_lens = seq_lens;
+  p.page_table = page_table;
+  p.N = N;
+  p.B = B;
+  p.H = H;
+  p.Hk = Hk;
+  p.G = H / Hk;
+  p.max_q = max_q;
+  p.max_pages = max_pages;
+  p.num_pages = num_pages;
+  while ((1 << p.page_shift) < page_size) ++p.page_shift;
+  p.tok_item = pl.tok_item;
+  p.hc = pl.hc;
+  p.unit = pl.unit;
+  p.max_items = pl.max_items;
+  p.part_rows = pl.part_rows;
+  p.scale_log2 = scale * kLog2e;
+  paged::carve(p, pl, workspace, D);
+  cudaStream_t s = (cudaStream_t)stream;
+  const bool hm = head_major != 0;
+  if (dtype == MFB_DTYPE_BF16)
+    return D == 64 ? paged::run<__nv_bfloat16, 64>(p, pl, q, k_pages, v_pages, page_size, hm, s)
+                   : paged::run<__nv_bfloat16, 128>(p, pl, q, k_pages, v_pages, page_size, hm, s);
+  return D == 64 ? paged::run<__half, 64>(p, pl, q, k_pages, v_pages, page_size, hm, s)
+                 : paged::run<__half, 128>(p, pl, q, k_pages, v_pages, page_size, hm, s);
+}
+
+extern "C" int mfb_paged_attn_status(int* code) {
+  MFB_CHECK_ARG(code != nullptr, "code is NULL");
+  int zero = 0;
+  MFB_CUDA_TRY(cudaMemcpyFromSymbol(code, paged::g_status, sizeof(int)));
+  if (*code) MFB_CUDA_TRY(cudaMemcpyToSymbol(paged::g_status, &zero, sizeof(int)));
+  return MFB_OK;
+}

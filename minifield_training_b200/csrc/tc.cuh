@@ -341,6 +341,11 @@ int make_tmap_bf16_box32(CUtensorMap* map, const void* base, uint64_t inner, uin
 // {dim, row, head} so that box {64, box_rows, heads} lands in shared memory as
 // [head][box_rows][64]: one 128-byte-swizzled tile per head.
 int make_tmap_bf16_heads(CUtensorMap* map, const void* base, uint64_t rows, int heads, uint32_t box_rows);
+// Tensor map of rank 3 or 4 over bf16 (or fp16) data, 128-byte swizzle: dims
+// and box innermost first (box[0] = 64 elements), strides in bytes of the
+// dimensions after the first. Loads outside the dims return zeros.
+int make_tmap_16(CUtensorMap* map, const void* base, bool bf16, int rank, const uint64_t* dims,
+                 const uint64_t* strides, const uint32_t* box);
 // 4-D FP32 tensor map over a [batch, T, heads, 64] array, addressed as
 // {dim, head, t, batch}; box {32, 1, box_rows, 1} (128-byte rows, 128-byte
 // swizzle). Boxes that run past T are clipped there, not into the next batch row.

@@ -16,6 +16,7 @@ from . import _lib
 
 DTYPES = {
     "bfloat16": np.dtype(ml_dtypes.bfloat16),
+    "float16": np.dtype(np.float16),
     "float32": np.dtype(np.float32),
     "int32": np.dtype(np.int32),
     "int8": np.dtype(np.int8),
@@ -197,6 +198,27 @@ _WORKSPACES = {}
 def workspace(tag: str, nbytes: int) -> DeviceArray:
     ws = _WORKSPACES.setdefault(tag, Workspace())
     return ws.get(nbytes)
+
+
+_STREAM_WORKSPACES = {}
+
+
+def stream_workspace(tag: str, nbytes: int, stream=None) -> DeviceArray:
+    """Grow-only scratch of one stream: calls on different streams never share it.
+
+    A call recorded into a CUDA graph is refused: the graph outlives the call
+    and may replay beside later ones, so it needs a workspace of its own.
+    """
+    flag = ctypes.c_int()
+    _lib.call("mfb_stream_is_capturing", stream, ctypes.byref(flag))
+    if flag.value:
+        raise ValueError(f"a captured {tag} call needs its own workspace (workspace=)")
+    key = (tag, getattr(stream, "value", stream))
+    entry = _STREAM_WORKSPACES.get(key)
+    if entry is None or entry[1] < nbytes:
+        size = max(int(nbytes), 2 * entry[1] if entry else 256)
+        entry = _STREAM_WORKSPACES[key] = (DeviceArray((size,), "uint8"), size)
+    return entry[0]
 
 
 class Event:

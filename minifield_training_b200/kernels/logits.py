@@ -1,0 +1,85 @@
+"""Controls on a step's logits before sampling: penalties for repeated tokens, biases, grammar masks.
+
+The reference hands raw FP32 logits to its caller
+(src/minifield_training/models/lfm2_5/decode.py:419-466). ``process_logits``
+applies the requests' controls in the pass that widens the logits to FP32.
+"""
+
+from .. import _lib
+from ..device import DeviceArray, as_device
+from .rotary import DTYPE_CODES, check_out
+
+
+def _per_row(x, rows, dtype, what, stream):
+    if x is None:
+        return None
+    x = as_device(x, dtype, stream)
+    if x.shape != (rows,):
+        raise ValueError(f"{what} must be [rows]")
+    return x.ptr, x
+
+
+def process_logits(logits, *, history=None, prompt_len=None, history_len=None, repetition=None, frequency=None,
+                   presence=None, bias_ids=None, bias_values=None, mask=None, mask_rows=None, out=None, stream=None):
+    """float32 [rows, vocab] logits under the rows' controls, each optional.
+
+    ``history`` (int32 [rows, n]) holds each row's token ids: the first
+    ``prompt_len`` of the prompt, then the generated ones, ``history_len`` in
+    all (defaults 0 and n; ids outside the vocabulary count for nothing). In
+    this order, for a token t of a row:
+
+    - ``repetition`` r (float32 [rows]): x / r if x > 0 else x * r, where t is in the history;
+    - ``frequency`` f, ``presence`` p: x - f * (times generated) - p * (generated at all);
+    - ``bias_ids``, ``bias_values`` (int32, float32 [rows, k]): x + the value at
+      t's id; of equal ids the last counts, ids outside the vocabulary pad;
+    - ``mask`` (int32 [grammars, ceil(vocab / 32)], bit t % 32 of word t // 32):
+      x = -inf where the bit is 0. ``mask_rows`` (int32 [rows]) picks each
+      row's grammar (default: row i's is i); an index outside leaves it free.
+
+    ``logits`` are bfloat16, float16 or float32; float32 logits may be ``out``.
+    """
+    if not isinstance(logits, DeviceArray):
+        logits = as_device(logits, "float32", stream)
+    if logits.ndim != 2 or logits.dtype not in DTYPE_CODES:
+        raise ValueError("logits must be [rows, vocab] in bfloat16, float16 or float32")
+    rows, vocab = logits.shape
+    out = check_out(out, (rows, vocab), "float32", "out")
+    capacity = biases = masks = 0
+    if history is not None:
+        history = as_device(history, "int32", stream)
+        if history.ndim != 2 or history.shape[0] != rows:
+            raise ValueError("history must be [rows, tokens]")
+        capacity = history.shape[1]
+    elif any(x is not None for x in (prompt_len, history_len, repetition, frequency, presence)):
+        raise ValueError("penalties and lengths need a history")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values must both be given or both be None")
+    if bias_ids is not None:
+        bias_ids, bias_values = as_device(bias_ids, "int32", stream), as_device(bias_values, "float32", stream)
+        if bias_ids.ndim != 2 or bias_ids.shape[0] != rows or bias_values.shape != bias_ids.shape:
+            raise ValueError("bias_ids and bias_values must be [rows, entries]")
+        biases = bias_ids.shape[1]
+    if mask is not None:
+        mask = as_device(mask, "int32", stream)
+        if mask.ndim != 2 or mask.shape[1] != (vocab + 31) // 32:
+            raise ValueError("mask must be [grammars, ceil(vocab / 32)]")
+        masks = mask.shape[0]
+        if mask_rows is None and masks < rows:
+            raise ValueError("a mask without mask_rows needs one row per logits row")
+    elif mask_rows is not None:
+        raise ValueError("mask_rows needs a mask")
+    held = [_per_row(x, rows, t, what, stream) for x, t, what in (
+        (prompt_len, "int32", "prompt_len"), (history_len, "int32", "history_len"),
+        (repetition, "float32", "repetition"), (frequency, "float32", "frequency"),
+        (presence, "float32", "presence"), (mask_rows, "int32", "mask_rows"))]
+    pl, hl, rep, freq, pres, mr = (x[0] if x is not None else None for x in held)
+    if rows and vocab:
+        _lib.call("mfb_logits_process", logits.ptr, DTYPE_CODES[logits.dtype],
+                  history.ptr if history is not None else None, capacity, pl, hl, rep, freq, pres,
+                  bias_ids.ptr if bias_ids is not None else None,
+                  bias_values.ptr if bias_values is not None else None, biases,
+                  mask.ptr if mask is not None else None, mr, masks, out.ptr, rows, vocab, stream)
+    return out
+
+
+__all__ = ["process_logits"]
