@@ -8,6 +8,7 @@ plays in the reference. Host NumPy arrays passed to the API are uploaded
 """
 
 import ctypes
+import math
 
 import ml_dtypes
 import numpy as np
@@ -54,7 +55,7 @@ class DeviceArray:
 
     @property
     def size(self) -> int:
-        return int(np.prod(self.shape, dtype=np.int64))
+        return math.prod(self.shape)
 
     @property
     def itemsize(self) -> int:
