@@ -36,16 +36,22 @@ constexpr int MAX_SMS = 160;  // bounds the workspace: shares are at most 2 (few
 __device__ int g_status;  // id of a bounded wait that gave up, or kBadPage / kBadLength
 constexpr int kBadPage = 1001, kBadLength = 1002;
 
+// A work item, and the record of a share: the item its first unit lies in.
 struct __align__(16) Item {
-  int b, hg;        // sequence, KV-head group
-  int tok0, ntok;   // query tokens: q rows tok0 .. tok0 + ntok - 1
-  int pos0;         // position of the first of them (negative: no keys yet)
-  int keys;         // keys the last one sees (0 if none)
-  int tiles, first; // key tiles (at least 1), and units before this item
+  int b, hg;         // sequence, KV-head group
+  int tok0, ntok;    // query tokens: q rows tok0 .. tok0 + ntok - 1
+  int pos0;          // position of the first of them (negative: no keys yet)
+  int keys;          // keys the last one sees (0 if none)
+  int tiles;         // units: key tiles, at least 1 (0: no query tokens)
+  int first;         // weight of the items before this one
+  int shift, index;  // a unit weighs 1 << shift; position in the list
+  int pad[2];
 };
 
+// The total weight is cut into `shares` ranges, the first `rest` of them one
+// longer than `base`. A unit belongs to the share its weight starts in.
 struct Header {
-  int total, shares, items, pad;
+  int total, shares, base, rest;
 };
 
 struct Params {
@@ -57,16 +63,16 @@ struct Params {
   const int* page_table;
   Header* head;
   Item* items;
-  int* starts;     // [grid] item holding each share's first unit
+  Item* starts;    // [grid] each share's first item
   int* tickets;    // [items]
   int* tickets_g;  // [2 * grid] first-level tickets of items cut into many parts
-  float* part_o;   // [slots][part_rows][D]
+  float* part_o;   // [slots][part_rows] x D
   float2* part_ml; // [slots][part_rows]
   int N, B, H, Hk, G, max_q, max_pages, num_pages, page_shift;
   int tok_item;    // query tokens per item
   int hc;          // KV heads per item
   int unit;        // keys per unit
-  int min_units;   // units a share should hold at least
+  int min_share;   // weight a share should hold at least
   int grid, max_items, part_rows;
   float scale_log2;
 };
@@ -114,11 +120,16 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* sum) {
   return incl - v + (warp ? warp_sums[warp - 1] : 0);
 }
 
-// The share whose range [i * total / g, (i + 1) * total / g) holds unit x.
-__device__ __forceinline__ int share_of(int x, int total, int g) {
-  return (int)(((long long)(x + 1) * g + total - 1) / total) - 1;
+__device__ __forceinline__ int share_begin(const Header& h, int i) { return i * h.base + min(i, h.rest); }
+__device__ __forceinline__ int share_of(const Header& h, int x) {
+  const int split = h.rest * (h.base + 1);
+  return x < split ? x / (h.base + 1) : h.rest + (x - split) / h.base;
 }
-__device__ __forceinline__ int share_begin(int i, int total, int g) { return (int)((long long)i * total / g); }
+// First unit of an item that belongs to the share beginning at weight x.
+__device__ __forceinline__ int unit_at(const Item& w, int x) {
+  return min(w.tiles, max(0, (x - w.first + (1 << w.shift) - 1) >> w.shift));
+}
+__device__ __forceinline__ int last_weight(const Item& w) { return w.first + ((w.tiles - 1) << w.shift); }
 
 // Query rows of sequence b inside q: arguments that contradict each other
 // (cu_q outside [0, N] or decreasing, more than max_q new tokens, lengths
@@ -135,128 +146,107 @@ __device__ __forceinline__ void sequence(const Params& p, int b, int* q0, int* n
   if (c0 != lo || c1 != hi || *nq != hi - lo || *len != s) atomicCAS(&g_status, 0, kBadLength);
 }
 
+// FEW: one item per sequence and head group (its new tokens fit one item);
+// otherwise a sequence has cdiv(new tokens, tok_item) blocks per head.
+template <bool FEW>
 __global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
   allow_dependents();
-  extern __shared__ int item_base[];  // [B + 1] items before each sequence
+  extern __shared__ int item_base[];  // [B + 1] items before each sequence (not FEW)
   __shared__ int warp_sums[32];
   const int tid = threadIdx.x, groups = p.Hk / p.hc;
-  int carry = 0;
-  for (int b0 = 0; b0 < p.B; b0 += SCHED_THREADS) {
-    const int b = b0 + tid;
-    int q0, nq = 0, base, len, sum;
-    if (b < p.B) sequence(p, b, &q0, &nq, &base, &len);
-    const int pre = block_scan(cdiv(nq, p.tok_item) * groups, warp_sums, &sum);
-    if (b < p.B) item_base[b] = carry + pre;
-    carry += sum;
-  }
-  if (tid == 0) item_base[p.B] = carry;
-  __syncthreads();
-  const int items = min(carry, p.max_items);
-  auto make = [&](int i) {
-    int lo = 0, hi = p.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (item_base[mid] <= i) lo = mid;
-      else hi = mid - 1;
+  for (int i = tid; i < 2 * p.grid; i += SCHED_THREADS) p.tickets_g[i] = 0;
+  int items = p.B * groups;
+  if (!FEW) {
+    int carry = 0;
+    for (int b0 = 0; b0 < p.B; b0 += SCHED_THREADS) {
+      const int b = b0 + tid;
+      int q0, nq = 0, base, len, sum;
+      if (b < p.B) sequence(p, b, &q0, &nq, &base, &len);
+      const int pre = block_scan(cdiv(nq, p.tok_item) * groups, warp_sums, &sum);
+      if (b < p.B) item_base[b] = carry + pre;
+      carry += sum;
     }
-    int q0, nq, base, len;
-    sequence(p, lo, &q0, &nq, &base, &len);
-    const int blocks = cdiv(nq, p.tok_item), local = i - item_base[lo];
+    items = min(carry, p.max_items);
+    __syncthreads();
+  }
+  auto make = [&](int i) {
     Item it;
-    it.b = lo;
-    it.hg = local / blocks;
-    const int t0 = (local % blocks) * p.tok_item;
+    int t0 = 0, q0, nq, base, len;
+    if (FEW) {
+      it.b = i / groups;
+      it.hg = i - it.b * groups;
+      sequence(p, it.b, &q0, &nq, &base, &len);
+    } else {
+      int lo = 0, hi = p.B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (item_base[mid] <= i) lo = mid;
+        else hi = mid - 1;
+      }
+      it.b = lo;
+      sequence(p, lo, &q0, &nq, &base, &len);
+      const int blocks = cdiv(nq, p.tok_item), local = i - item_base[lo];
+      it.hg = local / blocks;
+      t0 = (local - it.hg * blocks) * p.tok_item;
+    }
     it.tok0 = q0 + t0;
     it.ntok = min(p.tok_item, nq - t0);
     it.pos0 = base + t0;
     it.keys = min(max(it.pos0 + it.ntok, 0), len);
-    it.tiles = max(1, cdiv(it.keys, p.unit));
-    it.first = 0;
+    it.tiles = it.ntok > 0 ? max(1, cdiv(it.keys, p.unit)) : 0;
+    // Two query tiles share a unit's keys but need twice the softmax.
+    it.shift = !FEW && it.ntok * p.G > 128 ? 1 : 0;
+    it.index = i;
+    it.first = it.pad[0] = it.pad[1] = 0;
     return it;
   };
-  // One pass of the items for their total, a second for prefixes and shares;
-  // with at most a block of items the first pass's item is kept.
+  // A pass for the total weight, one for prefixes and shares; a single block
+  // of items keeps the first pass's results.
   Item mine{};
-  int total = 0;
+  int total = 0, pre = 0, sum;
   for (int i0 = 0; i0 < items; i0 += SCHED_THREADS) {
     const int i = i0 + tid;
-    int sum;
     if (i < items) mine = make(i);
-    block_scan(i < items ? mine.tiles : 0, warp_sums, &sum);
+    pre = block_scan(i < items ? mine.tiles << mine.shift : 0, warp_sums, &sum);
     total += sum;
   }
-  const int g = max(1, min(p.grid, total / p.min_units));
-  carry = 0;
+  Header h;
+  h.total = total;
+  h.shares = max(1, min(p.grid, total / p.min_share));
+  h.base = total / h.shares;
+  h.rest = total - h.base * h.shares;
+  if (tid == 0) *p.head = h;
+  int carry = 0;
   for (int i0 = 0; i0 < items; i0 += SCHED_THREADS) {
     const int i = i0 + tid;
-    int sum;
-    if (i < items && items > SCHED_THREADS) mine = make(i);
-    const int pre = block_scan(i < items ? mine.tiles : 0, warp_sums, &sum);
+    if (items > SCHED_THREADS) {
+      if (i < items) mine = make(i);
+      pre = block_scan(i < items ? mine.tiles << mine.shift : 0, warp_sums, &sum);
+    }
     if (i < items) {
       mine.first = carry + pre;
       p.items[i] = mine;
       p.tickets[i] = 0;
-      // Shares whose first unit lies in this item.
-      const int end = mine.first + mine.tiles;
-      int s = share_of(mine.first, total, g);
-      if (share_begin(s, total, g) < mine.first) ++s;
-      for (; s < g && share_begin(s, total, g) < end; ++s) p.starts[s] = i;
+      // Shares that begin in this item.
+      const int end = mine.first + (mine.tiles << mine.shift);
+      if (mine.tiles) {
+        int s = share_of(h, mine.first);
+        if (share_begin(h, s) < mine.first) ++s;
+        for (; s < h.shares && share_begin(h, s) < end; ++s) p.starts[s] = mine;
+      }
     }
     carry += sum;
   }
-  for (int i = tid; i < 2 * p.grid; i += SCHED_THREADS) p.tickets_g[i] = 0;
-  if (tid == 0) *p.head = Header{total, g, items, 0};
 }
 
 // ---------------------------------------------------------------------------
 // Joining the partials of a cut item. Segment (share c, which) owns a slot:
 // which = 0 where the share begins inside (or at) the item, 1 where the item
-// begins later in the share; only a share's first and last segment can be cut.
+// begins later in the share. Of a share's segments only the first and the last
+// can be cut, and of two of them only the first has which = 0.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ int slot_of(int c, int first_unit, int total, int g) {
-  return 2 * c + (share_begin(c, total, g) < first_unit ? 1 : 0);
-}
-
-// Joins `n` parts, part k in slot slot(k), for the float4 columns of `rows`
-// rows ([rows][D/4]) and hands each to emit(row, d4, m, l, o).
-template <int D, int NT, typename Slot, typename Emit>
-__device__ __forceinline__ void join(const Params& p, int n, int rows, int tid, Slot slot, Emit emit) {
-  for (int x = tid; x < rows * (D / 4); x += NT) {
-    const int row = x / (D / 4), d4 = x % (D / 4);
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < n; k += 8) {
-      float2 ml[8];
-      float4 ov[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        ml[u] = make_float2(-INFINITY, 0.f);
-        ov[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k + u < n) {
-          const long long at = (long long)slot(k + u) * p.part_rows + row;
-          ml[u] = __ldcg(p.part_ml + at);
-          ov[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + d4);
-        }
-      }
-      float mn = m;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) mn = fmaxf(mn, ml[u].x);
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      const float a = ex2(m - ref);
-      l *= a, acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float w = ex2(ml[u].x - ref);
-        l = fmaf(ml[u].y, w, l);
-        acc.x = fmaf(ov[u].x, w, acc.x);
-        acc.y = fmaf(ov[u].y, w, acc.y);
-        acc.z = fmaf(ov[u].z, w, acc.z);
-        acc.w = fmaf(ov[u].w, w, acc.w);
-      }
-      m = mn;
-    }
-    emit(row, d4, m, l, acc);
-  }
+__device__ __forceinline__ int slot_of(const Header& h, const Item& w, int c) {
+  return 2 * c + (share_begin(h, c) < w.first ? 1 : 0);
 }
 
 constexpr int JOIN = 16;  // shares joined per first-level group
@@ -269,39 +259,109 @@ __device__ __forceinline__ int group_slot(const Params& p, int c0, int k) {
   return 2 * p.grid + 2 * ((c0 + k * JOIN) / JOIN) + (k == 0 ? 1 : 0);
 }
 
+// Layouts of a slot's [rows][D] floats, in float4. ROWS32 interleaves blocks of
+// 32 rows, [row / 32][D / 4][row % 32]: a warp whose lanes own rows then writes
+// and reads whole lines. Otherwise rows are contiguous.
+template <int D, bool ROWS32>
+__device__ __forceinline__ long long part_at(const Params& p, int slot, int row, int d4) {
+  const long long r = (long long)slot * p.part_rows + row;
+  return ROWS32 ? ((r >> 5) * (D / 4) + d4) * 32 + (r & 31) : r * (D / 4) + d4;
+}
+
+// Joins part k = 0 .. n - 1 in slot(k) for `rows` rows by 256 threads; emit
+// gets (row, first d4, m, l, U float4). U columns x K parts are in flight per
+// thread and round: the loads' latency, not their bandwidth, is what a join
+// waits for.
+template <int D, bool ROWS32, int U, int K, typename Slot, typename Emit>
+__device__ __forceinline__ void join_parts(const Params& p, int n, int rows, int tid, Slot slot, Emit emit) {
+  constexpr int C = D / 4 / U;
+  const int span = ROWS32 ? (rows + 31) & ~31 : rows;
+  for (int x = tid; x < span * C; x += 256) {
+    const int row = ROWS32 ? (x / (32 * C)) * 32 + (x & 31) : x / C, d4 = (ROWS32 ? (x >> 5) % C : x % C) * U;
+    if (row >= rows) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 acc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < n; k0 += K) {
+      float2 ml[K];
+      float4 ov[K][U];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int u = 0; u < U; ++u) ov[k][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + k < n) {
+          const int sl = slot(k0 + k);
+          ml[k] = __ldcg(p.part_ml + (long long)sl * p.part_rows + row);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            ov[k][u] = __ldcg(reinterpret_cast<const float4*>(p.part_o) + part_at<D, ROWS32>(p, sl, row, d4 + u));
+        }
+      }
+      float mn = m;
+#pragma unroll
+      for (int k = 0; k < K; ++k) mn = fmaxf(mn, ml[k].x);
+      const float ref = mn == -INFINITY ? 0.f : mn, a = ex2(m - ref);
+      l *= a;
+#pragma unroll
+      for (int u = 0; u < U; ++u) acc[u].x *= a, acc[u].y *= a, acc[u].z *= a, acc[u].w *= a;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const float w = ex2(ml[k].x - ref);
+        l = fmaf(ml[k].y, w, l);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          acc[u].x = fmaf(ov[k][u].x, w, acc[u].x);
+          acc[u].y = fmaf(ov[k][u].y, w, acc[u].y);
+          acc[u].z = fmaf(ov[k][u].z, w, acc[u].z);
+          acc[u].w = fmaf(ov[k][u].w, w, acc[u].w);
+        }
+      }
+      m = mn;
+    }
+    emit(row, d4, m, l, acc);
+  }
+}
+
 // This share's segment of a cut item is in its slot (written by the 256
 // threads of named barrier 1, which all call). Two levels: the last of each
 // JOIN neighbouring shares joins them into a slot of its group, the last such
-// group joins the groups and finishes the rows.
-template <int D, typename Finish>
-__device__ __forceinline__ void join_cut(const Params& p, const Item& w, int item, int share, int total, int g,
-                                         int rows, int tid, int* s_flag, Finish finish) {
-  const int c0 = share_of(w.first, total, g), c1 = share_of(w.first + w.tiles - 1, total, g);
+// group joins the groups. finish(row, first d4, m, l, float4[U], U).
+template <int D, bool ROWS32, int U, int K, typename Finish>
+__device__ __forceinline__ void join_cut(const Params& p, const Header& h, const Item& w, int share, int rows, int tid,
+                                         int* s_flag, Finish finish) {
+  const int c0 = share_of(h, w.first), c1 = share_of(h, last_weight(w));
   const int k = (share - c0) / JOIN, grp0 = c0 + k * JOIN, gn = min(JOIN, c1 - grp0 + 1);
   const int ngrp = cdiv(c1 - c0 + 1, JOIN);
   auto meet = [] { asm volatile("bar.sync 1, 256;\n" ::: "memory"); };
   __threadfence();
   meet();
-  if (tid == 0) *s_flag = atomicAdd(p.tickets_g + slot_of(grp0, w.first, total, g), 1) == gn - 1;
+  if (tid == 0) *s_flag = atomicAdd(p.tickets_g + slot_of(h, w, grp0), 1) == gn - 1;
   meet();
   if (*s_flag) {
     __threadfence();
-    auto part = [&](int i) { return slot_of(grp0 + i, w.first, total, g); };
-    if (ngrp == 1) {
-      join<D, 256>(p, gn, rows, tid, part, finish);
-    } else {
-      const long long to = (long long)group_slot(p, c0, k) * p.part_rows;
-      join<D, 256>(p, gn, rows, tid, part, [&](int row, int d4, float m, float l, const float4& a) {
-        *reinterpret_cast<float4*>(p.part_o + (to + row) * D + d4 * 4) = a;
-        if (d4 == 0) p.part_ml[to + row] = make_float2(m, l);
-      });
+    auto part = [&](int i) { return slot_of(h, w, grp0 + i); };
+    const int to = ngrp == 1 ? -1 : group_slot(p, c0, k);
+    auto emit = [&](int row, int d4, float m, float l, const float4* a) {
+      if (to < 0) {
+        finish(row, d4, m, l, a);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          reinterpret_cast<float4*>(p.part_o)[part_at<D, ROWS32>(p, to, row, d4 + u)] = a[u];
+        if (d4 == 0) p.part_ml[(long long)to * p.part_rows + row] = make_float2(m, l);
+      }
+    };
+    join_parts<D, ROWS32, U, K>(p, gn, rows, tid, part, emit);
+    if (ngrp > 1) {
       __threadfence();
       meet();
-      if (tid == 0) *s_flag = atomicAdd(p.tickets + item, 1) == ngrp - 1;
+      if (tid == 0) *s_flag = atomicAdd(p.tickets + w.index, 1) == ngrp - 1;
       meet();
       if (*s_flag) {
         __threadfence();
-        join<D, 256>(p, ngrp, rows, tid, [&](int i) { return group_slot(p, c0, i); }, finish);
+        join_parts<D, ROWS32, U, K>(p, ngrp, rows, tid, [&](int i) { return group_slot(p, c0, i); }, finish);
       }
     }
   }
@@ -326,6 +386,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "[%6];\n" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
       : "memory");
+}
+
+// Steps to the next item of a share that ends at weight x1; false at its end.
+__device__ __forceinline__ bool advance(const Params& p, Item& w, int x1) {
+  if (w.first + (w.tiles << w.shift) >= x1) return false;
+  w = p.items[w.index + 1];
+  return true;
 }
 
 // ---------------------------------------------------------------------------
@@ -355,7 +422,7 @@ __host__ __device__ inline DLayout dlayout(int D, int stages, int rows, int hc) 
 }
 
 template <typename T, int D, bool R16>
-__global__ void __launch_bounds__(D_THREADS)
+__global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
     few_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, Params p,
                     int stages, int rows_max) {
   constexpr int DH = D / 64;
@@ -382,10 +449,10 @@ __global__ void __launch_bounds__(D_THREADS)
   wait_prerequisites();
   allow_dependents();
   const Header head = *p.head;
-  const int total = head.total, g = head.shares, share = blockIdx.x;
-  if (share >= g || total == 0) return;
-  const int x0 = share_begin(share, total, g), x1 = share_begin(share + 1, total, g);
-  const int item0 = p.starts[share];
+  const Item start = p.starts[blockIdx.x];
+  const int share = blockIdx.x;
+  if (share >= head.shares || head.total == 0) return;
+  const int x0 = share_begin(head, share), x1 = share_begin(head, share + 1);
   const int unit = p.unit, hc = p.hc;
   const int br = min(unit, 1 << p.page_shift), nb = unit / br;  // box rows, boxes per unit
 
@@ -393,11 +460,10 @@ __global__ void __launch_bounds__(D_THREADS)
     // Producer: lane i < nb looks up the page of box i one unit ahead; the
     // boxes of K and V (and of both halves of 128-wide heads) are issued by
     // the lanes in parallel, all counted on the stage's barrier.
-    int it = 0, item = item0;
+    int it = 0;
     bool ok = true;
-    for (int x = x0; ok && x < x1; ++item) {
-      const Item w = p.items[item];
-      const int u0 = x - w.first, u1 = min(w.tiles, x1 - w.first);
+    for (Item w = start; ok;) {
+      const int u0 = unit_at(w, x0), u1 = unit_at(w, x1);
       auto look = [&](int u) {
         const int key = u * unit + lane * br;
         return u < u1 && lane < nb && key < w.keys ? page_id(p, w.b, key) : 0;
@@ -423,7 +489,7 @@ __global__ void __launch_bounds__(D_THREADS)
         }
         id = next;
       }
-      x = w.first + u1;
+      if (!advance(p, w, x1)) break;
     }
     if (!ok)  // a wait gave up: let the copies in flight land before the CTA ends
       for (int f = max(0, it - stages); f < it; ++f) tc::mbar_wait_w(full_bar(f % stages), (f / stages) & 1, &g_status, 3);
@@ -441,11 +507,14 @@ __global__ void __launch_bounds__(D_THREADS)
   const int ki = (lane & 7) + ((lane >> 4) << 3), vi = (lane & 7) + ((lane >> 3) & 1) * 8;
   const uint32_t koff = row_off(ki), voff = row_off(vi);
   const int G = p.G;
-  int it = 0, item = item0;
+  int it = 0;
   bool ok = true;
-  for (int x = x0; x < x1; ++item) {
-    const Item w = p.items[item];
-    const int u0 = x - w.first, u1 = min(w.tiles, x1 - w.first);
+  for (Item w = start;;) {
+    const int u0 = unit_at(w, x0), u1 = unit_at(w, x1);
+    if (u0 >= u1) {
+      if (!advance(p, w, x1)) break;
+      continue;
+    }
     const int rows = w.ntok * G, hk = w.hg * hc + hl;
     uint32_t qa[D / 16][4];
     int lim[2];
@@ -535,15 +604,13 @@ __global__ void __launch_bounds__(D_THREADS)
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(empty_bar(st));
     }
-    x = w.first + u1;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
     }
-    const int c0 = share_of(w.first, total, g), c1 = share_of(w.first + w.tiles - 1, total, g);
-    const bool cut = c0 != c1;
-    const int slot = slot_of(share, w.first, total, g);
+    const bool cut = u0 > 0 || u1 < w.tiles;
+    const int slot = slot_of(head, w, share);
     auto finish = [&](int row, int h, int d4, float mm, float ll, const float4& a) {
       const float inv = ll > 0.f ? 1.f / ll : 0.f;
       const long long at = (long long)(w.tok0 + row / G) * p.H + (w.hg * hc + h) * G + row % G;
@@ -612,7 +679,10 @@ __global__ void __launch_bounds__(D_THREADS)
       }
       if (!cut) asm volatile("bar.sync 1, 256;\n" ::: "memory");  // before the area is written again
     }
-    if (cut) join_cut<D>(p, w, item, share, total, g, rows * hc, tid, &s_flag, finish_row);
+    if (cut)
+      join_cut<D, false, 1, 8>(p, head, w, share, rows * hc, tid, &s_flag,
+                            [&](int rh, int d4, float mm, float ll, const float4* a) { finish_row(rh, d4, mm, ll, *a); });
+    if (!advance(p, w, x1)) break;
   }
 }
 
@@ -631,10 +701,13 @@ __global__ void __launch_bounds__(D_THREADS)
 // place of S, O += P V (TMEM); the sum of P is kept in FP32 before rounding.
 // M moves only when a row's maximum has risen by more than 2^8, the row's O
 // and sum then being rescaled.
+// Each 128-key tile runs as two halves with barriers of their own: while the
+// softmax works on one half, the tensor core finishes P V of the other and
+// writes the next tile's scores over it, so a group never waits for the round
+// trip P -> P V -> S.
 // Items of more than 128 rows give each group one of the two query tiles;
 // smaller ones give both groups the same queries and alternate key tiles
-// between them, so that softmax and tensor core overlap either way; the two
-// accumulators are then joined in the epilogue.
+// between them; the two accumulators are then joined in the epilogue.
 // ---------------------------------------------------------------------------
 constexpr int T_THREADS = 320;
 
@@ -645,13 +718,41 @@ struct TShape {
   static constexpr int SLOTS = D == 64 ? 10 : 5;
   static constexpr uint32_t Q = 0, RING = 2 * SLOT, ML = RING + SLOTS * SLOT;  // ML: (max, sum) of group 1's rows
   static constexpr uint32_t BARS = ML + 1024;
-  static constexpr uint32_t TOTAL = 1024 + BARS + 8 * (2 * SLOTS + 13);
+  static constexpr int NBARS = 2 * SLOTS + 3 + 4 + 4 + 4 + 2;
+  static constexpr uint32_t TOTAL = 1024 + BARS + 8 * (NBARS + 1);
 };
 
 // Instruction descriptor of kind::f16 with FP32 accumulation; A and B bf16 or fp16.
 __host__ __device__ constexpr uint32_t idesc16(bool bf, int N, int b_mn) {
   return (1u << 4) | ((bf ? 1u : 0u) << 7) | ((bf ? 1u : 0u) << 10) | ((uint32_t)b_mn << 16) |
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// Two FP32 lanes per instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 template <typename T, int D>
@@ -667,11 +768,11 @@ __global__ void __launch_bounds__(T_THREADS, 1)
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (S::SLOTS + s); };
   const uint32_t q_full = bars + 8u * (2 * S::SLOTS), q_empty = q_full + 8, tail_bar = q_full + 16;
-  auto s_full = [&](int g) { return q_full + 24 + 8u * g; };
-  auto p_full = [&](int g) { return q_full + 40 + 8u * g; };
-  auto o_full = [&](int g) { return q_full + 56 + 8u * g; };
-  const uint32_t o_free = q_full + 72, done_bar = q_full + 80;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 8 * (2 * S::SLOTS + 11));
+  auto s_full = [&](int g, int h) { return q_full + 24 + 8u * (2 * g + h); };
+  auto p_full = [&](int g, int h) { return q_full + 56 + 8u * (2 * g + h); };
+  auto pv_done = [&](int g, int h) { return q_full + 88 + 8u * (2 * g + h); };
+  const uint32_t o_free = q_full + 120, done_bar = q_full + 128;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 8 * S::NBARS);
   __shared__ int s_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* status = &g_status;
@@ -685,9 +786,11 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     tc::mbar_init(q_empty, 1);
     tc::mbar_init(tail_bar, 1);
     for (int g = 0; g < 2; ++g) {
-      tc::mbar_init(s_full(g), 1);
-      tc::mbar_init(p_full(g), 128);
-      tc::mbar_init(o_full(g), 1);
+      for (int h = 0; h < 2; ++h) {
+        tc::mbar_init(s_full(g, h), 1);
+        tc::mbar_init(p_full(g, h), 128);
+        tc::mbar_init(pv_done(g, h), 1);
+      }
     }
     tc::mbar_init(o_free, 256);
     tc::mbar_init(done_bar, 1);
@@ -707,136 +810,148 @@ __global__ void __launch_bounds__(T_THREADS, 1)
   wait_prerequisites();
   allow_dependents();
   const Header head = *p.head;
-  const int total = head.total, g_n = head.shares, share = blockIdx.x;
-  const bool idle = share >= g_n || total == 0;
-  const int x0 = idle ? 0 : share_begin(share, total, g_n), x1 = idle ? 0 : share_begin(share + 1, total, g_n);
-  const int item0 = idle ? 0 : p.starts[share];
+  const Item start = p.starts[blockIdx.x];
+  const int share = blockIdx.x;
+  const bool idle = share >= head.shares || head.total == 0;
+  const int x0 = idle ? 0 : share_begin(head, share), x1 = idle ? 0 : share_begin(head, share + 1);
   const int G = p.G, tpt = 128 / G;  // tokens per query tile
   const int page = 1 << p.page_shift, br = min(128, page), nb = 128 / br;
 
-  if (warp == 0) {
-    int slot = 0, slot_ph = 0, fills = 0, seg = 0, tails = 0, item = item0;
+  if (idle) {
+    // nothing to do
+  } else if (warp == 0) {
+    int slot = 0, slot_ph = 0, fills = 0, seg = 0, tails = 0;
     bool ok = true;
-    for (int x = x0; ok && x < x1; ++item, ++seg) {
-      const Item w = p.items[item];
-      const int j0 = x - w.first, j1 = min(w.tiles, x1 - w.first), n = j1 - j0;
-      const bool dual = w.ntok > tpt;
-      const int delay = dual ? 1 : 2;
-      if (!(ok = tc::mbar_wait_w(q_empty, (seg & 1) ^ 1, status, 11))) break;
-      if (lane == 0) {
-        const int tiles = dual ? 2 : 1;
-        tc::mbar_expect_tx(q_full, (uint32_t)(tiles * DH * tpt * G * 128));
-        for (int t = 0; t < tiles; ++t)
-          for (int h = 0; h < DH; ++h)
-            tc::tma_load_3d(sb + S::Q + t * S::SLOT + h * 16384u, &tq, h * 64, w.hg * G, w.tok0 + t * tpt, q_full);
-      }
-      __syncwarp();
-      auto look = [&](int j) {
-        const int key = j * 128 + lane * br;
-        return j < j1 && lane < nb && key < w.keys ? page_id(p, w.b, key) : 0;
-      };
-      // Page ids of the next K tile and of the tiles whose V is still to come.
-      int id_next = look(j0), id_v0 = 0, id_v1 = 0;
-      auto load = [&](const CUtensorMap* map, int j, int id, bool is_v) {
-        if (!(ok = tc::mbar_wait_w(empty_bar(slot), slot_ph ^ 1, status, 12))) return;
-        const int valid = min(128, w.keys - j * 128), live = cdiv(max(valid, 0), br);
-        const bool tail = is_v && valid < 128;
-        const uint32_t bar = tail ? tail_bar : full_bar(slot), dst = sb + S::RING + slot * S::SLOT;
-        if (lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(live * br * 128 * DH));
-        __syncwarp();
-        const int bx = lane % max(live, 1), half = lane / max(live, 1);
-        const int pid = __shfl_sync(0xffffffffu, id, bx);
-        if (half < DH && lane < live * DH)
-          tma_load_4d(dst + half * 16384u + bx * br * 128, map, half * 64, (j * 128 + bx * br) & (page - 1), w.hg, pid, bar);
-        if (tail) {
-          // Rows past the sequence hold whatever the page (or the ring) held;
-          // zeros in their place, since 0 x NaN would not vanish in P V.
-          ok = tc::mbar_wait_w(tail_bar, tails & 1, status, 13);
-          ++tails;
-          for (int i = max(valid, 0) * 8 + lane; i < 128 * 8; i += 32)
+    for (Item w = start; ok;) {
+      const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
+      if (n > 0) {
+        const bool dual = w.ntok > tpt;
+        const int delay = dual ? 1 : 2;
+        if (!(ok = tc::mbar_wait_w(q_empty, (seg & 1) ^ 1, status, 11))) break;
+        ++seg;
+        if (lane == 0) {
+          const int tiles = dual ? 2 : 1;
+          tc::mbar_expect_tx(q_full, (uint32_t)(tiles * DH * tpt * G * 128));
+          for (int t = 0; t < tiles; ++t)
             for (int h = 0; h < DH; ++h)
-              *reinterpret_cast<uint4*>(smem + S::RING + slot * S::SLOT + h * 16384u + i * 16) = make_uint4(0, 0, 0, 0);
-          tc::fence_proxy_async_smem();
+              tc::tma_load_3d(sb + S::Q + t * S::SLOT + h * 16384u, &tq, h * 64, w.hg * G, w.tok0 + t * tpt, q_full);
+        }
+        __syncwarp();
+        auto look = [&](int j) {
+          const int key = j * 128 + lane * br;
+          return j < j1 && lane < nb && key < w.keys ? page_id(p, w.b, key) : 0;
+        };
+        // Page ids of the next K tile and of the tiles whose V is still to come.
+        int id_next = look(j0), id_v0 = 0, id_v1 = 0;
+        auto load = [&](const CUtensorMap* map, int j, int id, bool is_v) {
+          if (!(ok = tc::mbar_wait_w(empty_bar(slot), slot_ph ^ 1, status, 12))) return;
+          const int valid = min(128, w.keys - j * 128), live = cdiv(max(valid, 0), br);
+          const bool tail = is_v && valid < 128;
+          const uint32_t bar = tail ? tail_bar : full_bar(slot), dst = sb + S::RING + slot * S::SLOT;
+          if (lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(live * br * 128 * DH));
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(full_bar(slot));
+          const int bx = lane % max(live, 1), half = lane / max(live, 1);
+          const int pid = __shfl_sync(0xffffffffu, id, bx);
+          if (half < DH && lane < live * DH)
+            tma_load_4d(dst + half * 16384u + bx * br * 128, map, half * 64, (j * 128 + bx * br) & (page - 1), w.hg,
+                        pid, bar);
+          if (tail) {
+            // Rows past the sequence hold whatever the page (or the ring) held;
+            // zeros in their place, since 0 x NaN would not vanish in P V.
+            ok = tc::mbar_wait_w(tail_bar, tails & 1, status, 13);
+            ++tails;
+            for (int i = max(valid, 0) * 8 + lane; i < 128 * 8; i += 32)
+              for (int h = 0; h < DH; ++h)
+                *reinterpret_cast<uint4*>(smem + S::RING + slot * S::SLOT + h * 16384u + i * 16) = make_uint4(0, 0, 0, 0);
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(full_bar(slot));
+          }
+          ++fills;
+          if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+        };
+        for (int it = 0; ok && it < n + delay; ++it) {
+          const int id_k = id_next;
+          if (it + 1 < n) id_next = look(j0 + it + 1);
+          if (it >= delay) {
+            load(&tv, j0 + it - delay, dual ? id_v0 : id_v1, true);
+            if (!ok) break;
+          }
+          if (it < n) load(&tk, j0 + it, id_k, false);
+          id_v1 = id_v0;
+          id_v0 = id_k;
         }
-        ++fills;
-        if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
-      };
-      for (int it = 0; ok && it < n + delay; ++it) {
-        const int id_k = id_next;
-        if (it + 1 < n) id_next = look(j0 + it + 1);
-        if (it >= delay) {
-          load(&tv, j0 + it - delay, dual ? id_v0 : id_v1, true);
-          if (!ok) break;
-        }
-        if (it < n) load(&tk, j0 + it, id_k, false);
-        id_v1 = id_v0;
-        id_v0 = id_k;
       }
-      x = w.first + j1;
+      if (!advance(p, w, x1)) break;
     }
     if (!ok)  // a wait gave up: let the copies in flight land before the CTA ends
       for (int f = max(0, fills - S::SLOTS); f < fills; ++f)
         tc::mbar_wait_w(full_bar(f % S::SLOTS), (f / S::SLOTS) & 1, status, 14);
   } else if (warp == 1) {
-    const uint32_t idesc_s = idesc16(BF, 128, 0), idesc_o = idesc16(BF, D, 1);
-    int slot = 0, slot_ph = 0, seg = 0, item = item0;
+    const uint32_t idesc_s = idesc16(BF, 64, 0), idesc_o = idesc16(BF, D, 1);
+    int slot = 0, slot_ph = 0, seg = 0;
     int np[2] = {0, 0};  // P tiles consumed, per group
     bool ok = true;
-    for (int x = x0; ok && x < x1; ++item, ++seg) {
-      const Item w = p.items[item];
-      const int j0 = x - w.first, j1 = min(w.tiles, x1 - w.first), n = j1 - j0;
-      const bool dual = w.ntok > tpt;
-      const int delay = dual ? 1 : 2;
-      if (!(ok = tc::mbar_wait_w(q_full, seg & 1, status, 21))) break;
-      tc::tc_fence_after();
-      for (int it = 0; ok && it < n + delay; ++it) {
-        const bool do_pv = it >= delay, do_qk = it < n;
-        int vs = 0, ks = 0;
-        if (do_pv) {
-          vs = slot;
-          if (!(ok = tc::mbar_wait_w(full_bar(vs), slot_ph, status, 22))) break;
-          if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
-        }
-        if (do_qk) {
-          ks = slot;
-          if (!(ok = tc::mbar_wait_w(full_bar(ks), slot_ph, status, 23))) break;
-          if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
-        }
+    for (Item w = start; ok;) {
+      const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
+      if (n > 0) {
+        const bool dual = w.ntok > tpt;
+        const int delay = dual ? 1 : 2;
+        if (!(ok = tc::mbar_wait_w(q_full, seg & 1, status, 21))) break;
         tc::tc_fence_after();
-        // The output accumulators of the previous item are read out.
-        if (it == delay && !(ok = tc::mbar_wait_w(o_free, (seg & 1) ^ 1, status, 24))) break;
-        const int g_lo = dual ? 0 : (it & 1), g_hi = dual ? 1 : (it & 1);
-        for (int g = g_lo; ok && g <= g_hi; ++g) {
-          const uint32_t s_t = tmem + g * 128, o_t = tmem + 256 + g * D;
+        for (int it = 0; ok && it < n + delay; ++it) {
+          const bool do_pv = it >= delay, do_qk = it < n;
+          int vs = 0, ks = 0;
           if (do_pv) {
-            if (!(ok = tc::mbar_wait_w(p_full(g), np[g] & 1, status, 25))) break;
-            ++np[g];
-            tc::tc_fence_after();
-            const uint32_t vb = sb + S::RING + vs * S::SLOT;
-            const bool first = dual ? it == 1 : it < 4;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              tc::mma_bf16_ts_w(o_t, s_t + k * 8, tc::smem_desc_sw128(vb + k * 2048, 16384, 1024), idesc_o,
-                                (first && k == 0) ? 0u : 1u);
-            if (it >= n) tc::mma_commit_w(o_full(g));  // the group's last product of the item
+            vs = slot;
+            if (!(ok = tc::mbar_wait_w(full_bar(vs), slot_ph, status, 22))) break;
+            if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
           }
           if (do_qk) {
-            const uint32_t qb = sb + S::Q + (dual ? g : 0) * S::SLOT, kb = sb + S::RING + ks * S::SLOT;
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              tc::mma_bf16_w(s_t, tc::smem_desc_sw128(qb + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
-                             tc::smem_desc_sw128(kb + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
-            tc::mma_commit_w(s_full(g));
+            ks = slot;
+            if (!(ok = tc::mbar_wait_w(full_bar(ks), slot_ph, status, 23))) break;
+            if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
           }
+          tc::tc_fence_after();
+          // The output accumulators of the previous item are read out.
+          if (it == delay && !(ok = tc::mbar_wait_w(o_free, (seg & 1) ^ 1, status, 24))) break;
+          const int g_lo = dual ? 0 : (it & 1), g_hi = dual ? 1 : (it & 1);
+          for (int h = 0; ok && h < 2; ++h) {
+            for (int g = g_lo; ok && g <= g_hi; ++g) {
+              const uint32_t s_t = tmem + g * 128 + h * 64, o_t = tmem + 256 + g * D;
+              if (do_pv) {
+                if (!(ok = tc::mbar_wait_w(p_full(g, h), np[g] & 1, status, 25))) break;
+                tc::tc_fence_after();
+                const uint32_t vb = sb + S::RING + vs * S::SLOT + h * 8192;
+                const bool first = h == 0 && (dual ? it == 1 : it < 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  tc::mma_bf16_ts_w(o_t, s_t + k * 8, tc::smem_desc_sw128(vb + k * 2048, 16384, 1024), idesc_o,
+                                    (first && k == 0) ? 0u : 1u);
+                tc::mma_commit_w(pv_done(g, h));
+              }
+              if (do_qk) {
+                const uint32_t qb = sb + S::Q + (dual ? g : 0) * S::SLOT, kb = sb + S::RING + ks * S::SLOT + h * 8192;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                  tc::mma_bf16_w(s_t, tc::smem_desc_sw128(qb + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
+                                 tc::smem_desc_sw128(kb + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024), idesc_s,
+                                 k > 0 ? 1u : 0u);
+                tc::mma_commit_w(s_full(g, h));
+              }
+            }
+          }
+          if (!ok) break;
+          if (do_pv) {
+            tc::mma_commit_w(empty_bar(vs));
+            for (int g = g_lo; g <= g_hi; ++g) ++np[g];
+          }
+          if (do_qk) tc::mma_commit_w(empty_bar(ks));
+          if (it == n - 1) tc::mma_commit_w(q_empty);
         }
-        if (!ok) break;
-        if (do_pv) tc::mma_commit_w(empty_bar(vs));
-        if (do_qk) tc::mma_commit_w(empty_bar(ks));
-        if (it == n - 1) tc::mma_commit_w(q_empty);
+        ++seg;
       }
-      x = w.first + j1;
+      if (!advance(p, w, x1)) break;
     }
     tc::mma_commit_w(done_bar);
     tc::mbar_wait_w(done_bar, 0, status, 26);
@@ -846,84 +961,92 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     const uint32_t s_t = tmem + lane_off + grp * 128, o_t = tmem + lane_off + 256 + grp * D;
     float2* ml_s = reinterpret_cast<float2*>(smem + S::ML);
     const float sl2 = p.scale_log2;
-    int ns = 0, item = item0;
-    int no[2] = {0, 0};  // items whose output each group has had
+    int nt[2] = {0, 0};  // tiles each group has had
     bool ok = true;
-    for (int x = x0; x < x1; ++item) {
-      const Item w = p.items[item];
-      const int j0 = x - w.first, j1 = min(w.tiles, x1 - w.first), n = j1 - j0;
+    for (Item w = start;;) {
+      const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
+      if (n <= 0) {
+        if (!advance(p, w, x1)) break;
+        continue;
+      }
       const bool dual = w.ntok > tpt;
       const int t = (dual ? grp * tpt : 0) + r / G;
       const bool live = r < tpt * G && t < w.ntok;
       const bool warp_live = __any_sync(0xffffffffu, live);
       // Keys this row sees; rows that do not exist mask nothing and are never read.
       const int limit = live ? min(w.pos0 + t + 1, w.keys) : 0x7fffffff;
-      float M = -INFINITY, l = 0.f;
-      for (int it = dual ? 0 : grp; it < n; it += dual ? 1 : 2, ++ns) {
-        if (ok) ok = tc::mbar_wait_w(s_full(grp), ns & 1, status, 31);
-        if (!ok) break;
-        if (warp_live) {
-          tc::tc_fence_after();
-          uint32_t v[128];
+      float M = -INFINITY;
+      uint64_t l2 = pair(0.f, 0.f);
+      int mine = nt[grp];
+      for (int it = dual ? 0 : grp; it < n; it += dual ? 1 : 2, ++mine) {
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          if (ok) ok = tc::mbar_wait_w(s_full(grp, h), mine & 1, status, 31);
+          if (ok && warp_live) {
+            tc::tc_fence_after();
+            uint32_t v[64];
+            tc::tmem_ld_32x32b_x32(s_t + h * 64, v);
+            tc::tmem_ld_32x32b_x32(s_t + h * 64 + 32, v + 32);
+            tc::tmem_ld_wait();
+            const int lim = limit - ((j0 + it) * 128 + h * 64);
+            if (__any_sync(0xffffffffu, lim < 64)) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tc::tmem_ld_32x32b_x32(s_t + c * 32, v + c * 32);
-          tc::tmem_ld_wait();
-          const int lim = limit - (j0 + it) * 128;
-          if (__any_sync(0xffffffffu, lim < 128)) {
-#pragma unroll
-            for (int i = 0; i < 128; ++i) v[i] = i < lim ? v[i] : 0xFF800000u;
-          }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 128; i += 4) {
-            mx[0] = fmaxf(mx[0], __uint_as_float(v[i]));
-            mx[1] = fmaxf(mx[1], __uint_as_float(v[i + 1]));
-            mx[2] = fmaxf(mx[2], __uint_as_float(v[i + 2]));
-            mx[3] = fmaxf(mx[3], __uint_as_float(v[i + 3]));
-          }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-          // The group's previous product has landed: its commit precedes s_full's.
-          const bool up = top > M + 8.f;
-          if (__any_sync(0xffffffffu, up && M != -INFINITY)) {
-            const float a = (up && M != -INFINITY) ? ex2(M - top) : 1.f;
-            l *= a;
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t ov[16];
-              tc::tmem_ld_32x32b_x16(o_t + c * 16, ov);
-              tc::tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * a);
-              tc::tmem_st_32x32b_x16(o_t + c * 16, ov);
+              for (int i = 0; i < 64; ++i) v[i] = i < lim ? v[i] : 0xFF800000u;
             }
-          }
-          if (up) M = top;
-          const float neg = M == -INFINITY ? 0.f : -M;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            float mx[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
+            for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 4]));
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float e0 = ex2(fmaf(__uint_as_float(v[c * 32 + i]), sl2, neg));
-              const float e1 = ex2(fmaf(__uint_as_float(v[c * 32 + i + 1]), sl2, neg));
-              sum[i & 2] += e0;
-              sum[(i & 2) + 1] += e1;
+            for (int i = 8; i < 64; i += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                mx[e] = max3(mx[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + e + 4]));
+            const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sl2;
+            const bool up = top > M + 8.f, move = up && M != -INFINITY;
+            if (__any_sync(0xffffffffu, move)) {
+              // The product of the half before this one may still be adding to O.
+              ok = tc::mbar_wait_w(pv_done(grp, h ^ 1), (mine + h + 1) & 1, status, 34);
+              tc::tc_fence_after();
+              const float a = move ? ex2(M - top) : 1.f;
+              const float2 lv = unpair(l2);
+              l2 = pair(lv.x * a, lv.y * a);
+#pragma unroll
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t ov[16];
+                tc::tmem_ld_32x32b_x16(o_t + c * 16, ov);
+                tc::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * a);
+                tc::tmem_st_32x32b_x16(o_t + c * 16, ov);
+              }
+            }
+            if (up) M = top;
+            const float neg = M == -INFINITY ? 0.f : -M;
+            const uint64_t sl = pair(sl2, sl2), ng = pair(neg, neg);
+            uint32_t pk[32];
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) {
+              const float2 e = unpair(fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sl, ng));
+              const float e0 = ex2(e.x), e1 = ex2(e.y);
+              l2 = add2(l2, pair(e0, e1));
               pk[i >> 1] = Num16<T>::pack2(e0, e1);
             }
-            tc::tmem_st_32x32b_x16(s_t + c * 16, pk);
+            tc::tmem_st_32x32b_x16(s_t + h * 64, pk);
+            tc::tmem_st_32x32b_x16(s_t + h * 64 + 16, pk + 16);
+            tc::tmem_st_wait();
+            tc::tc_fence_before();
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tc::tmem_st_wait();
-          tc::tc_fence_before();
+          tc::mbar_arrive(p_full(grp, h));
         }
-        tc::mbar_arrive(p_full(grp));
       }
-      x = w.first + j1;
+      const float2 lv = unpair(l2);
+      float l = lv.x + lv.y;
 
       // Epilogue: this group's rows (dual), or both groups' accumulators of
       // the same rows joined by group 0.
       const bool has1 = dual || n > 1, cut = j0 > 0 || j1 < w.tiles;
+      nt[0] += dual ? n : (n + 1) / 2;
+      nt[1] += dual ? n : n / 2;
       float a0 = 1.f, a1 = 0.f;
       if (!dual) {
         if (grp == 1) ml_s[r] = make_float2(M, l);
@@ -940,14 +1063,14 @@ __global__ void __launch_bounds__(T_THREADS, 1)
       }
       const bool store = live && (dual || grp == 0);
       if ((dual || grp == 0) && ok) {
-        ok = tc::mbar_wait_w(o_full(grp), no[grp] & 1, status, 32);
-        if (ok && !dual && has1) ok = tc::mbar_wait_w(o_full(1), no[1] & 1, status, 33);
+        ok = tc::mbar_wait_w(pv_done(grp, 1), (nt[grp] - 1) & 1, status, 32);
+        if (ok && !dual && has1) ok = tc::mbar_wait_w(pv_done(1, 1), (nt[1] - 1) & 1, status, 33);
         if (ok && warp_live) {
           tc::tc_fence_after();
           const float inv = cut ? 1.f : (l > 0.f ? 1.f / l : 0.f);
           const float f0 = a0 * inv, f1 = a1 * inv;
           const long long at = (long long)(w.tok0 + t) * p.H + w.hg * G + r % G;
-          const long long pr = (long long)slot_of(share, w.first, total, g_n) * p.part_rows + t * G + r % G;
+          const int slot = slot_of(head, w, share), pr = t * G + r % G;
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t ov[32];
@@ -968,11 +1091,12 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             }
             if (!store) continue;
             if (cut) {
-              float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + c * 32);
+              float4* dst = reinterpret_cast<float4*>(p.part_o);
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                dst[e] = make_float4(__uint_as_float(ov[4 * e]), __uint_as_float(ov[4 * e + 1]),
-                                     __uint_as_float(ov[4 * e + 2]), __uint_as_float(ov[4 * e + 3]));
+                dst[part_at<D, true>(p, slot, pr, c * 8 + e)] =
+                    make_float4(__uint_as_float(ov[4 * e]), __uint_as_float(ov[4 * e + 1]),
+                                __uint_as_float(ov[4 * e + 2]), __uint_as_float(ov[4 * e + 3]));
             } else {
               uint4* dst = reinterpret_cast<uint4*>(p.o + at * D + c * 32);
 #pragma unroll
@@ -984,25 +1108,28 @@ __global__ void __launch_bounds__(T_THREADS, 1)
               }
             }
           }
-          if (store && cut) p.part_ml[pr] = make_float2(M, l);
+          if (store && cut) p.part_ml[(long long)slot * p.part_rows + pr] = make_float2(M, l);
           if (store && !cut && p.lse) p.lse[at] = lse_of(M, l);
           tc::tc_fence_before();
         }
       }
-      ++no[0];
-      if (has1) ++no[1];
       tc::mbar_arrive(o_free);
       if (cut)
-        join_cut<D>(p, w, item, share, total, g_n, w.ntok * G, stid, &s_flag,
-                    [&](int row, int d4, float mm, float ll, const float4& a) {
-                      const float inv = ll > 0.f ? 1.f / ll : 0.f;
-                      const long long at = (long long)(w.tok0 + row / G) * p.H + w.hg * G + row % G;
-                      uint2 out;
-                      out.x = Num16<T>::pack2(a.x * inv, a.y * inv);
-                      out.y = Num16<T>::pack2(a.z * inv, a.w * inv);
-                      *reinterpret_cast<uint2*>(p.o + at * D + d4 * 4) = out;
-                      if (p.lse && d4 == 0) p.lse[at] = lse_of(mm, ll);
-                    });
+        join_cut<D, true, 4, 4>(p, head, w, share, w.ntok * G, stid, &s_flag,
+                             [&](int row, int d4, float mm, float ll, const float4* a) {
+                               const float inv = ll > 0.f ? 1.f / ll : 0.f;
+                               const long long at = (long long)(w.tok0 + row / G) * p.H + w.hg * G + row % G;
+                               uint4* dst = reinterpret_cast<uint4*>(p.o + at * D + d4 * 4);
+#pragma unroll
+                               for (int u = 0; u < 2; ++u) {
+                                 const float f[8] = {a[2 * u].x * inv,     a[2 * u].y * inv,     a[2 * u].z * inv,
+                                                     a[2 * u].w * inv,     a[2 * u + 1].x * inv, a[2 * u + 1].y * inv,
+                                                     a[2 * u + 1].z * inv, a[2 * u + 1].w * inv};
+                                 dst[u] = pack16x8<T>(f);
+                               }
+                               if (p.lse && d4 == 0) p.lse[at] = lse_of(mm, ll);
+                             });
+      if (!advance(p, w, x1)) break;
     }
   }
   tc::tc_fence_before();
@@ -1048,7 +1175,7 @@ Plan plan(int N, int B, int max_q, int H, int Hk, int D) {
   }
   pl.slots = 2 * pl.grid_cap + 2 * (pl.grid_cap / JOIN + 1);
   pl.bytes = 256 + align256(sizeof(Item) * (size_t)pl.max_items) + align256(sizeof(int) * (size_t)pl.max_items) +
-             align256(sizeof(int) * 3 * (size_t)pl.grid_cap) +
+             align256(sizeof(Item) * (size_t)pl.grid_cap) + align256(sizeof(int) * 2 * (size_t)pl.grid_cap) +
              align256(sizeof(float) * (size_t)pl.slots * pl.part_rows * D) +
              align256(sizeof(float2) * (size_t)pl.slots * pl.part_rows);
   return pl;
@@ -1064,8 +1191,8 @@ void carve(Params& p, const Plan& pl, void* base, int D) {
   p.head = reinterpret_cast<Header*>(take(sizeof(Header)));
   p.items = reinterpret_cast<Item*>(take(sizeof(Item) * (size_t)pl.max_items));
   p.tickets = reinterpret_cast<int*>(take(sizeof(int) * (size_t)pl.max_items));
-  p.starts = reinterpret_cast<int*>(take(sizeof(int) * 3 * (size_t)pl.grid_cap));
-  p.tickets_g = p.starts + pl.grid_cap;
+  p.starts = reinterpret_cast<Item*>(take(sizeof(Item) * (size_t)pl.grid_cap));
+  p.tickets_g = reinterpret_cast<int*>(take(sizeof(int) * 2 * (size_t)pl.grid_cap));
   p.part_o = reinterpret_cast<float*>(take(sizeof(float) * (size_t)pl.slots * pl.part_rows * D));
   p.part_ml = reinterpret_cast<float2*>(take(sizeof(float2) * (size_t)pl.slots * pl.part_rows));
 }
@@ -1089,7 +1216,7 @@ int run_few(Params& p, const Plan& pl, const CUtensorMap& tk, const CUtensorMap&
   MFB_CUDA_TRY(cudaFuncSetAttribute(few_rows_kernel<T, D, R16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MAX_SMEM));
   const int per_sm = 2 * smem + 4096 <= 228 * 1024 ? 2 : 1;
   p.grid = std::min(per_sm * sms, pl.grid_cap);
-  schedule_kernel<<<1, SCHED_THREADS, sizeof(int) * (size_t)(p.B + 1), s>>>(p);
+  schedule_kernel<true><<<1, SCHED_THREADS, 0, s>>>(p);
   MFB_LAUNCH_CHECK("paged attention schedule");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.grid);
@@ -1118,10 +1245,10 @@ int run(Params& p, const Plan& pl, const void* q, const void* kp, const void* vp
   if ((st = make_tmap_pages(&tk, kp, bf, D, page_size, p.Hk, p.num_pages, head_major, br, pl.hc))) return st;
   if ((st = make_tmap_pages(&tv, vp, bf, D, page_size, p.Hk, p.num_pages, head_major, br, pl.hc))) return st;
   if (pl.few) {
-    p.min_units = 4;
+    p.min_share = 4;
     return p.max_q * p.G <= 8 ? run_few<T, D, false>(p, pl, tk, tv, sms, s) : run_few<T, D, true>(p, pl, tk, tv, sms, s);
   }
-  p.min_units = 2;
+  p.min_share = 4;
   const uint64_t dims[3] = {(uint64_t)D, (uint64_t)p.H, (uint64_t)p.N};
   const uint64_t strides[2] = {(uint64_t)D * 2, (uint64_t)p.H * D * 2};
   const uint32_t box[3] = {64, (uint32_t)p.G, (uint32_t)(128 / p.G)};
@@ -1130,7 +1257,7 @@ int run(Params& p, const Plan& pl, const void* q, const void* kp, const void* vp
   static_assert(smem <= MAX_SMEM, "chunk kernel shared memory");
   MFB_CUDA_TRY(cudaFuncSetAttribute(chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   p.grid = sms;
-  schedule_kernel<<<1, SCHED_THREADS, sizeof(int) * (size_t)(p.B + 1), s>>>(p);
+  schedule_kernel<false><<<1, SCHED_THREADS, sizeof(int) * (size_t)(p.B + 1), s>>>(p);
   MFB_LAUNCH_CHECK("paged attention schedule");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.grid);
