@@ -701,13 +701,18 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
 // place of S, O += P V (TMEM); the sum of P is kept in FP32 before rounding.
 // M moves only when a row's maximum has risen by more than 2^8, the row's O
 // and sum then being rescaled.
-// Each 128-key tile runs as two halves with barriers of their own: while the
-// softmax works on one half, the tensor core finishes P V of the other and
-// writes the next tile's scores over it, so a group never waits for the round
-// trip P -> P V -> S.
+// The scores rotate through NB TMEM buffers: three for 64-wide heads, so that a
+// group's next scores are there before its softmax ends; two for 128-wide ones
+// (the outputs take the rest of TMEM). Products of M = 128 with A in shared
+// memory take about 70 cycles per K = 16 step for N = 64 and N = 128 alike, and
+// 44 or 64 with A in TMEM, so whole 128-key tiles: halves of 64 keys, which
+// would double-buffer within the same columns, measured 2076 tensor cycles per
+// unit of two query tiles against 1244.
 // Items of more than 128 rows give each group one of the two query tiles;
 // smaller ones give both groups the same queries and alternate key tiles
-// between them; the two accumulators are then joined in the epilogue.
+// between them; the two accumulators are then joined in the epilogue. Either
+// way an item is a sequence of jobs (scores, softmax, product with V), job j
+// being group j & 1's: of a tile per job, or of a tile per pair of jobs.
 // ---------------------------------------------------------------------------
 constexpr int T_THREADS = 320;
 
@@ -718,7 +723,9 @@ struct TShape {
   static constexpr int SLOTS = D == 64 ? 10 : 5;
   static constexpr uint32_t Q = 0, RING = 2 * SLOT, ML = RING + SLOTS * SLOT;  // ML: (max, sum) of group 1's rows
   static constexpr uint32_t BARS = ML + 1024;
-  static constexpr int NBARS = 2 * SLOTS + 3 + 4 + 4 + 4 + 2;
+  static constexpr int NB = D == 64 ? 3 : 2;       // score buffers of 128 TMEM columns
+  static constexpr uint32_t O = NB * 128;          // first column of the outputs
+  static constexpr int NBARS = 2 * SLOTS + 3 + 2 * NB + 2 + 2;
   static constexpr uint32_t TOTAL = 1024 + BARS + 8 * (NBARS + 1);
 };
 
@@ -755,6 +762,33 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// Four K = 16 steps of one product, issued by one elected lane of a converged
+// warp: A in shared memory (descriptor steps of 32 bytes) or in tensor memory
+// (8 columns), B in shared memory (steps of 32 bytes K-major, 2048 MN-major).
+// One election and no arithmetic between the instructions: the issuing warp is
+// a serial stage of every tile.
+__device__ __forceinline__ void mma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred e, p, t;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %5, %8, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %6, %9, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %7, %10, %3, t;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b + 2), "l"(b + 4), "l"(b + 6)
+      : "memory");
+}
+__device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred e, p, t;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%5], %8, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%6], %9, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%7], %10, %3, t;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(a + 8), "r"(a + 16), "r"(a + 24), "l"(b + 128), "l"(b + 256),
+      "l"(b + 384)
+      : "memory");
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(T_THREADS, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -768,10 +802,10 @@ __global__ void __launch_bounds__(T_THREADS, 1)
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (S::SLOTS + s); };
   const uint32_t q_full = bars + 8u * (2 * S::SLOTS), q_empty = q_full + 8, tail_bar = q_full + 16;
-  auto s_full = [&](int g, int h) { return q_full + 24 + 8u * (2 * g + h); };
-  auto p_full = [&](int g, int h) { return q_full + 56 + 8u * (2 * g + h); };
-  auto pv_done = [&](int g, int h) { return q_full + 88 + 8u * (2 * g + h); };
-  const uint32_t o_free = q_full + 120, done_bar = q_full + 128;
+  auto s_full = [&](int b) { return q_full + 24 + 8u * b; };
+  auto p_full = [&](int b) { return q_full + 24 + 8u * (S::NB + b); };
+  auto pv_done = [&](int g) { return q_full + 24 + 8u * (2 * S::NB + g); };
+  const uint32_t o_free = pv_done(2), done_bar = o_free + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 8 * S::NBARS);
   __shared__ int s_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -785,13 +819,12 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     tc::mbar_init(q_full, 1);
     tc::mbar_init(q_empty, 1);
     tc::mbar_init(tail_bar, 1);
-    for (int g = 0; g < 2; ++g) {
-      for (int h = 0; h < 2; ++h) {
-        tc::mbar_init(s_full(g, h), 1);
-        tc::mbar_init(p_full(g, h), 128);
-        tc::mbar_init(pv_done(g, h), 1);
-      }
+    for (int i = 0; i < S::NB; ++i) {
+      tc::mbar_init(s_full(i), 1);
+      tc::mbar_init(p_full(i), 128);
     }
+    tc::mbar_init(pv_done(0), 1);
+    tc::mbar_init(pv_done(1), 1);
     tc::mbar_init(o_free, 256);
     tc::mbar_init(done_bar, 1);
     tc::mbar_fence_init();
@@ -826,7 +859,6 @@ __global__ void __launch_bounds__(T_THREADS, 1)
       const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
       if (n > 0) {
         const bool dual = w.ntok > tpt;
-        const int delay = dual ? 1 : 2;
         if (!(ok = tc::mbar_wait_w(q_empty, (seg & 1) ^ 1, status, 11))) break;
         ++seg;
         if (lane == 0) {
@@ -841,8 +873,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
           const int key = j * 128 + lane * br;
           return j < j1 && lane < nb && key < w.keys ? page_id(p, w.b, key) : 0;
         };
-        // Page ids of the next K tile and of the tiles whose V is still to come.
-        int id_next = look(j0), id_v0 = 0, id_v1 = 0;
+        // Page ids of the next K and of the next V tile.
+        int id_k = look(j0), id_v = id_k, kj = j0, vj = j0;
         auto load = [&](const CUtensorMap* map, int j, int id, bool is_v) {
           if (!(ok = tc::mbar_wait_w(empty_bar(slot), slot_ph ^ 1, status, 12))) return;
           const int valid = min(128, w.keys - j * 128), live = cdiv(max(valid, 0), br);
@@ -870,16 +902,20 @@ __global__ void __launch_bounds__(T_THREADS, 1)
           ++fills;
           if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
         };
-        for (int it = 0; ok && it < n + delay; ++it) {
-          const int id_k = id_next;
-          if (it + 1 < n) id_next = look(j0 + it + 1);
-          if (it >= delay) {
-            load(&tv, j0 + it - delay, dual ? id_v0 : id_v1, true);
+        // Jobs' order of need: step s runs the product of job s - NB, then the
+        // scores of job s.
+        const int jobs = dual ? 2 * n : n;
+        for (int st = 0; ok && st < jobs + S::NB; ++st) {
+          const int pj = st - S::NB;
+          if (pj >= 0 && (!dual || !(pj & 1))) {
+            load(&tv, vj, id_v, true);
+            id_v = look(++vj);
             if (!ok) break;
           }
-          if (it < n) load(&tk, j0 + it, id_k, false);
-          id_v1 = id_v0;
-          id_v0 = id_k;
+          if (st < jobs && (!dual || !(st & 1))) {
+            load(&tk, kj, id_k, false);
+            id_k = look(++kj);
+          }
         }
       }
       if (!advance(p, w, x1)) break;
@@ -888,66 +924,61 @@ __global__ void __launch_bounds__(T_THREADS, 1)
       for (int f = max(0, fills - S::SLOTS); f < fills; ++f)
         tc::mbar_wait_w(full_bar(f % S::SLOTS), (f / S::SLOTS) & 1, status, 14);
   } else if (warp == 1) {
-    const uint32_t idesc_s = idesc16(BF, 64, 0), idesc_o = idesc16(BF, D, 1);
+    // Item fields are broadcast from lane 0, so that the compiler knows the
+    // loop to be uniform and keeps the operands in the uniform datapath.
+    // Item fields are broadcast from lane 0, so that the compiler knows the
+    // loop to be uniform and keeps the operands in the uniform datapath.
+    const uint32_t idesc_s = idesc16(BF, 128, 0), idesc_o = idesc16(BF, D, 1);
+    const uint64_t q_desc = tc::smem_desc_sw128(sb + S::Q, 16, 1024);
+    const uint64_t k_desc = tc::smem_desc_sw128(sb + S::RING, 16, 1024);
+    const uint64_t v_desc = tc::smem_desc_sw128(sb + S::RING, 16384, 1024);
     int slot = 0, slot_ph = 0, seg = 0;
-    int np[2] = {0, 0};  // P tiles consumed, per group
+    int sbuf = 0, pbuf = 0, pph = 0;  // buffer of the next scores, of the next product, and its phase
     bool ok = true;
     for (Item w = start; ok;) {
-      const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
+      const int n = __shfl_sync(0xffffffffu, unit_at(w, x1) - unit_at(w, x0), 0);
       if (n > 0) {
-        const bool dual = w.ntok > tpt;
-        const int delay = dual ? 1 : 2;
+        const bool dual = __shfl_sync(0xffffffffu, w.ntok, 0) > tpt;
+        const int jobs = dual ? 2 * n : n;
+        int ks = 0, vs = 0;
         if (!(ok = tc::mbar_wait_w(q_full, seg & 1, status, 21))) break;
-        tc::tc_fence_after();
-        for (int it = 0; ok && it < n + delay; ++it) {
-          const bool do_pv = it >= delay, do_qk = it < n;
-          int vs = 0, ks = 0;
-          if (do_pv) {
-            vs = slot;
-            if (!(ok = tc::mbar_wait_w(full_bar(vs), slot_ph, status, 22))) break;
-            if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
-          }
-          if (do_qk) {
-            ks = slot;
-            if (!(ok = tc::mbar_wait_w(full_bar(ks), slot_ph, status, 23))) break;
-            if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
-          }
-          tc::tc_fence_after();
-          // The output accumulators of the previous item are read out.
-          if (it == delay && !(ok = tc::mbar_wait_w(o_free, (seg & 1) ^ 1, status, 24))) break;
-          const int g_lo = dual ? 0 : (it & 1), g_hi = dual ? 1 : (it & 1);
-          for (int h = 0; ok && h < 2; ++h) {
-            for (int g = g_lo; ok && g <= g_hi; ++g) {
-              const uint32_t s_t = tmem + g * 128 + h * 64, o_t = tmem + 256 + g * D;
-              if (do_pv) {
-                if (!(ok = tc::mbar_wait_w(p_full(g, h), np[g] & 1, status, 25))) break;
-                tc::tc_fence_after();
-                const uint32_t vb = sb + S::RING + vs * S::SLOT + h * 8192;
-                const bool first = h == 0 && (dual ? it == 1 : it < 4);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  tc::mma_bf16_ts_w(o_t, s_t + k * 8, tc::smem_desc_sw128(vb + k * 2048, 16384, 1024), idesc_o,
-                                    (first && k == 0) ? 0u : 1u);
-                tc::mma_commit_w(pv_done(g, h));
-              }
-              if (do_qk) {
-                const uint32_t qb = sb + S::Q + (dual ? g : 0) * S::SLOT, kb = sb + S::RING + ks * S::SLOT + h * 8192;
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                  tc::mma_bf16_w(s_t, tc::smem_desc_sw128(qb + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
-                                 tc::smem_desc_sw128(kb + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024), idesc_s,
-                                 k > 0 ? 1u : 0u);
-                tc::mma_commit_w(s_full(g, h));
-              }
+        for (int st = 0; ok && st < jobs + S::NB; ++st) {
+          const int pj = st - S::NB;
+          if (pj >= 0) {
+            if (!dual || !(pj & 1)) {
+              vs = slot;
+              if (!(ok = tc::mbar_wait_w(full_bar(vs), slot_ph, status, 22))) break;
+              if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
             }
+            // The output accumulators of the previous item are read out.
+            if (pj == 0 && !(ok = tc::mbar_wait_w(o_free, (seg & 1) ^ 1, status, 24))) break;
+            if (!(ok = tc::mbar_wait_w(p_full(pbuf), pph, status, 25))) break;
+            tc::tc_fence_after();
+            const uint32_t o_t = tmem + S::O + (pj & 1) * D, p_t = tmem + pbuf * 128;
+            const uint64_t vd = v_desc + (uint64_t)(vs * (S::SLOT >> 4));
+            mma4_ts(o_t, p_t, vd, idesc_o, pj > 1 ? 1u : 0u);
+            mma4_ts(o_t, p_t + 32, vd + 512, idesc_o, 1u);
+            tc::mma_commit_w(pv_done(pj & 1));
+            if (!dual || (pj & 1)) tc::mma_commit_w(empty_bar(vs));
+            if (++pbuf == S::NB) pbuf = 0, pph ^= 1;
           }
-          if (!ok) break;
-          if (do_pv) {
-            tc::mma_commit_w(empty_bar(vs));
-            for (int g = g_lo; g <= g_hi; ++g) ++np[g];
+          if (st < jobs) {
+            if (!dual || !(st & 1)) {
+              ks = slot;
+              if (!(ok = tc::mbar_wait_w(full_bar(ks), slot_ph, status, 23))) break;
+              if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+            }
+            tc::tc_fence_after();
+            const uint32_t s_t = tmem + sbuf * 128;
+            const uint64_t qd = q_desc + (uint64_t)(dual && (st & 1) ? S::SLOT >> 4 : 0);
+            const uint64_t kd = k_desc + (uint64_t)(ks * (S::SLOT >> 4));
+            mma4_ss(s_t, qd, kd, idesc_s, 0u);
+            if (D == 128) mma4_ss(s_t, qd + 1024, kd + 1024, idesc_s, 1u);
+            tc::mma_commit_w(s_full(sbuf));
+            if (!dual || (st & 1)) tc::mma_commit_w(empty_bar(ks));
+            if (st == jobs - 1) tc::mma_commit_w(q_empty);
+            if (++sbuf == S::NB) sbuf = 0;
           }
-          if (do_qk) tc::mma_commit_w(empty_bar(ks));
-          if (it == n - 1) tc::mma_commit_w(q_empty);
         }
         ++seg;
       }
@@ -958,10 +989,11 @@ __global__ void __launch_bounds__(T_THREADS, 1)
   } else {
     const int grp = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane, stid = tid - 64;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_t = tmem + lane_off + grp * 128, o_t = tmem + lane_off + 256 + grp * D;
+    const uint32_t o_t = tmem + lane_off + S::O + grp * D;
     float2* ml_s = reinterpret_cast<float2*>(smem + S::ML);
     const float sl2 = p.scale_log2;
-    int nt[2] = {0, 0};  // tiles each group has had
+    int nj0 = 0, nj1 = 0;  // jobs each group has had
+    int buf = 0, ph = 0;   // buffer and phase of the item's job 0
     bool ok = true;
     for (Item w = start;;) {
       const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
@@ -977,76 +1009,104 @@ __global__ void __launch_bounds__(T_THREADS, 1)
       const int limit = live ? min(w.pos0 + t + 1, w.keys) : 0x7fffffff;
       float M = -INFINITY;
       uint64_t l2 = pair(0.f, 0.f);
-      int mine = nt[grp];
-      for (int it = dual ? 0 : grp; it < n; it += dual ? 1 : 2, ++mine) {
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          if (ok) ok = tc::mbar_wait_w(s_full(grp, h), mine & 1, status, 31);
-          if (ok && warp_live) {
-            tc::tc_fence_after();
-            uint32_t v[64];
-            tc::tmem_ld_32x32b_x32(s_t + h * 64, v);
-            tc::tmem_ld_32x32b_x32(s_t + h * 64 + 32, v + 32);
+      const int jobs = dual ? 2 * n : n;
+      int mine = grp ? nj1 : nj0;
+      int bj = buf + grp, pj = ph;  // buffer and phase of this group's next job
+      if (bj >= S::NB) bj -= S::NB, pj ^= 1;
+      for (int j = grp; j < jobs; j += 2, ++mine) {
+        if (ok) ok = tc::mbar_wait_w(s_full(bj), pj, status, 31);
+        if (ok && warp_live) {
+          const uint32_t s_t = tmem + lane_off + bj * 128;
+          const int lim = limit - (j0 + (dual ? j >> 1 : j)) * 128;
+          const bool masked = __any_sync(0xffffffffu, lim < 128);
+          tc::tc_fence_after();
+          // Maximum of the row's 128 scores; the second 64 stay in registers,
+          // the first are read again when their turn comes.
+          uint32_t v[64];
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            tc::tmem_ld_32x32b_x32(s_t + half * 64, v);
+            tc::tmem_ld_32x32b_x32(s_t + half * 64 + 32, v + 32);
             tc::tmem_ld_wait();
-            const int lim = limit - ((j0 + it) * 128 + h * 64);
-            if (__any_sync(0xffffffffu, lim < 64)) {
+            if (masked) {
 #pragma unroll
-              for (int i = 0; i < 64; ++i) v[i] = i < lim ? v[i] : 0xFF800000u;
+              for (int i = 0; i < 64; ++i) v[i] = half * 64 + i < lim ? v[i] : 0xFF800000u;
             }
-            float mx[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 4]));
-#pragma unroll
-            for (int i = 8; i < 64; i += 8)
+            for (int i = 0; i < 64; i += 8)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 mx[e] = max3(mx[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + e + 4]));
-            const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sl2;
-            const bool up = top > M + 8.f, move = up && M != -INFINITY;
-            if (__any_sync(0xffffffffu, move)) {
-              // The product of the half before this one may still be adding to O.
-              ok = tc::mbar_wait_w(pv_done(grp, h ^ 1), (mine + h + 1) & 1, status, 34);
-              tc::tc_fence_after();
-              const float a = move ? ex2(M - top) : 1.f;
-              const float2 lv = unpair(l2);
-              l2 = pair(lv.x * a, lv.y * a);
+          }
+          const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sl2;
+          const bool up = top > M + 8.f, move = up && M != -INFINITY;
+          if (__any_sync(0xffffffffu, move)) {
+            // This group's previous product may still be adding to O.
+            ok = tc::mbar_wait_w(pv_done(grp), (mine - 1) & 1, status, 34);
+            tc::tc_fence_after();
+            const float a = move ? ex2(M - top) : 1.f;
+            const float2 lv = unpair(l2);
+            l2 = pair(lv.x * a, lv.y * a);
 #pragma unroll
-              for (int c = 0; c < D / 16; ++c) {
-                uint32_t ov[16];
-                tc::tmem_ld_32x32b_x16(o_t + c * 16, ov);
-                tc::tmem_ld_wait();
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t ov[16];
+              tc::tmem_ld_32x32b_x16(o_t + c * 16, ov);
+              tc::tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * a);
-                tc::tmem_st_32x32b_x16(o_t + c * 16, ov);
-              }
+              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * a);
+              tc::tmem_st_32x32b_x16(o_t + c * 16, ov);
             }
-            if (up) M = top;
-            const float neg = M == -INFINITY ? 0.f : -M;
-            const uint64_t sl = pair(sl2, sl2), ng = pair(neg, neg);
-            uint32_t pk[32];
+          }
+          if (up) M = top;
+          const float neg = M == -INFINITY ? 0.f : -M;
+          const uint64_t sl = pair(sl2, sl2), ng = pair(neg, neg);
+          // P over the scores: 16-bit pairs in the first 64 columns. Scores
+          // 0-63 are read before their columns are written.
+          auto weigh = [&](const uint32_t* x, uint32_t* pk) {
 #pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-              const float2 e = unpair(fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sl, ng));
+            for (int i = 0; i < 32; i += 2) {
+              const float2 e = unpair(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sl, ng));
               const float e0 = ex2(e.x), e1 = ex2(e.y);
               l2 = add2(l2, pair(e0, e1));
               pk[i >> 1] = Num16<T>::pack2(e0, e1);
             }
-            tc::tmem_st_32x32b_x16(s_t + h * 64, pk);
-            tc::tmem_st_32x32b_x16(s_t + h * 64 + 16, pk + 16);
-            tc::tmem_st_wait();
-            tc::tc_fence_before();
+          };
+          uint32_t y[64], pk[32];
+          weigh(v, pk);
+          tc::tmem_ld_32x32b_x32(s_t, y);
+          weigh(v + 32, pk + 16);
+          tc::tmem_ld_32x32b_x32(s_t + 32, y + 32);
+          tc::tmem_ld_wait();
+          tc::tmem_st_32x32b_x16(s_t + 32, pk);
+          tc::tmem_st_32x32b_x16(s_t + 48, pk + 16);
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) y[i] = i < lim ? y[i] : 0xFF800000u;
           }
-          tc::mbar_arrive(p_full(grp, h));
+          weigh(y, pk);
+          tc::tmem_st_32x32b_x16(s_t, pk);
+          weigh(y + 32, pk + 16);
+          tc::tmem_st_32x32b_x16(s_t + 16, pk + 16);
+          tc::tmem_st_wait();
+          tc::tc_fence_before();
         }
+        tc::mbar_arrive(p_full(bj));
+        bj += 2;
+        if (bj >= S::NB) bj -= S::NB, pj ^= 1;
       }
+      // The next item's job 0: `jobs` buffers on.
+      buf += jobs % S::NB;
+      ph ^= (jobs / S::NB) & 1;
+      if (buf >= S::NB) buf -= S::NB, ph ^= 1;
       const float2 lv = unpair(l2);
       float l = lv.x + lv.y;
 
       // Epilogue: this group's rows (dual), or both groups' accumulators of
       // the same rows joined by group 0.
       const bool has1 = dual || n > 1, cut = j0 > 0 || j1 < w.tiles;
-      nt[0] += dual ? n : (n + 1) / 2;
-      nt[1] += dual ? n : n / 2;
+      nj0 += (jobs + 1) / 2;
+      nj1 += jobs / 2;
       float a0 = 1.f, a1 = 0.f;
       if (!dual) {
         if (grp == 1) ml_s[r] = make_float2(M, l);
@@ -1063,8 +1123,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
       }
       const bool store = live && (dual || grp == 0);
       if ((dual || grp == 0) && ok) {
-        ok = tc::mbar_wait_w(pv_done(grp, 1), (nt[grp] - 1) & 1, status, 32);
-        if (ok && !dual && has1) ok = tc::mbar_wait_w(pv_done(1, 1), (nt[1] - 1) & 1, status, 33);
+        ok = tc::mbar_wait_w(pv_done(grp), ((grp ? nj1 : nj0) - 1) & 1, status, 32);
+        if (ok && !dual && has1) ok = tc::mbar_wait_w(pv_done(1), (nj1 - 1) & 1, status, 33);
         if (ok && warp_live) {
           tc::tc_fence_after();
           const float inv = cut ? 1.f : (l > 0.f ? 1.f / l : 0.f);
