@@ -378,6 +378,33 @@ __device__ __forceinline__ int page_id(const Params& p, int b, int key) {
   return p.num_pages;  // outside the tensor: the load fills zeros
 }
 
+// Page ids of a stream of tiles, 32 boxes ahead: lane l holds the id of box
+// 32 window + l (a box is `br` keys of one page, a tile `nb` boxes, a power of
+// two up to 32). The next window's ids are read while this one is used, so
+// the loads never wait for a table lookup.
+struct PageIds {
+  int b, br, nb, end;  // sequence, keys per box, boxes per tile, keys that are needed
+  int window, cur, next;
+  __device__ __forceinline__ int fetch(const Params& p, int w) const {
+    const int key = (w * 32 + (int)(threadIdx.x & 31)) * br;
+    return key < end ? page_id(p, b, key) : 0;
+  }
+  __device__ __forceinline__ PageIds(const Params& p, int seq, int rows, int boxes, int tile, int keys)
+      : b(seq), br(rows), nb(boxes), end(keys), window(tile * boxes >> 5) {
+    cur = fetch(p, window);
+    next = fetch(p, window + 1);
+  }
+  // The id of box `lane % nb` (or any of the caller's choice) of a tile; tiles in order.
+  __device__ __forceinline__ int get(const Params& p, int tile, int box) {
+    if (tile * nb >> 5 != window) {
+      ++window;
+      cur = next;
+      next = fetch(p, window + 1);
+    }
+    return __shfl_sync(0xffffffffu, cur, (tile * nb & 31) + box);
+  }
+};
+
 // 4-D tiled load, no multicast.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
                                             uint32_t bar) {
@@ -457,21 +484,15 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
   const int br = min(unit, 1 << p.page_shift), nb = unit / br;  // box rows, boxes per unit
 
   if (warp == DW) {
-    // Producer: lane i < nb looks up the page of box i one unit ahead; the
-    // boxes of K and V (and of both halves of 128-wide heads) are issued by
-    // the lanes in parallel, all counted on the stage's barrier.
+    // Producer: the boxes of K and V (and of both halves of 128-wide heads) are
+    // issued by the lanes in parallel, all counted on the stage's barrier.
     int it = 0;
     bool ok = true;
     for (Item w = start; ok;) {
       const int u0 = unit_at(w, x0), u1 = unit_at(w, x1);
-      auto look = [&](int u) {
-        const int key = u * unit + lane * br;
-        return u < u1 && lane < nb && key < w.keys ? page_id(p, w.b, key) : 0;
-      };
-      int id = look(u0);
+      PageIds ids(p, w.b, br, nb, u0, min(w.keys, u1 * unit));
       for (int u = u0; u < u1; ++u, ++it) {
         const int st = it % stages;
-        const int next = look(u + 1);
         if (!(ok = tc::mbar_wait_w(empty_bar(st), ((it / stages) & 1) ^ 1, &g_status, 1))) break;
         const int live = min(nb, cdiv(max(w.keys - u * unit, 0), br));  // boxes that hold keys
         const uint32_t box = (uint32_t)br * hc * 128u;
@@ -479,7 +500,7 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
         __syncwarp();
         for (int j = lane; j - lane < live * 2 * DH; j += 32) {
           const int bx = j % max(live, 1), rest = j / max(live, 1);  // rest: half, then K or V
-          const int pid = __shfl_sync(0xffffffffu, id, bx);
+          const int pid = ids.get(p, u, bx);
           if (j < live * 2 * DH) {
             const int half = rest % DH, kv = rest / DH;
             const uint32_t dst = sb + st * kStage + kv * (kStage / 2) + half * 16384u + bx * box;
@@ -487,7 +508,6 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
                         pid, full_bar(st));
           }
         }
-        id = next;
       }
       if (!advance(p, w, x1)) break;
     }
@@ -692,11 +712,12 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
 // An item is one KV head and up to 2 x 128 query rows, row r of a tile being
 // (token r / G, head r % G of the group): every query head of the group and
 // every token share the K/V tiles. Units are 128 keys.
-//   warp 0      producer: Q tiles per item, K and V tiles (one TMA box per
+//   warps 0-7   softmax: two groups of four, one query row (TMEM lane) per thread
+//   warp 8      producer: Q tiles per item, K and V tiles (one TMA box per
 //               page touched) through one ring, in the order they are used
-//   warp 1      TMEM owner and MMA issuer (whole warp, one elected lane)
-//   warps 2-9   softmax: two groups of four, a group per S accumulator, one
-//               query row (TMEM lane) per thread
+//   warp 9      TMEM owner and MMA issuer (whole warp, one elected lane)
+//   warps 10-11 idle: they complete the third warpgroup, whose registers go to
+//               the softmax (a row's 128 scores stay in registers)
 // S = Q K^T (TMEM), P = 2^(scale S - M) rounded to the cache's 16-bit type in
 // place of S, O += P V (TMEM); the sum of P is kept in FP32 before rounding.
 // M moves only when a row's maximum has risen by more than 2^8, the row's O
@@ -714,7 +735,9 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
 // way an item is a sequence of jobs (scores, softmax, product with V), job j
 // being group j & 1's: of a tile per job, or of a tile per pair of jobs.
 // ---------------------------------------------------------------------------
-constexpr int T_THREADS = 320;
+constexpr int T_THREADS = 384;
+// 384 threads x 168 registers at launch = 64512 >= 256 x 208 + 128 x 80 = 63488.
+constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 80;
 
 template <int D>
 struct TShape {
@@ -756,11 +779,45 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+
+// 2^x for two x < 128 on the FMA and integer pipes, for part of a tile: the
+// special-function unit alone would bound the softmax. x = n + f with n the
+// nearest integer (read off the low bits of x + 1.5 * 2^23 + 127, so that the
+// shifted bits are the FP32 exponent of 2^n) and |f| <= 1/2; 2^f by the degree-4
+// polynomial of least relative error on that interval (Remez exchange on
+// p(f) 2^-f - 1), off by at most 2.7e-6 in FP32. From -126.5 down the result is
+// exactly 0, as it has to be for masked keys; NaN stays NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
+  const float2 f = unpair(x);
+  x = pair(max_nan(f.x, -127.f), max_nan(f.y, -127.f));
+  const uint64_t t = add2(x, pair(12583039.f, 12583039.f));
+  const uint64_t r = fma2(add2(t, pair(-12583039.f, -12583039.f)), pair(-1.f, -1.f), x);
+  uint64_t q = fma2(pair(9.570101911150505e-3f, 9.570101911150505e-3f), r, pair(5.5917860319385004e-2f, 5.5917860319385004e-2f));
+  q = fma2(q, r, pair(0.24024744827864145f, 0.24024744827864145f));
+  q = fma2(q, r, pair(0.6931218147366899f, 0.6931218147366899f));
+  q = fma2(q, r, pair(0.999999261445712f, 0.999999261445712f));
+  const float2 n = unpair(t);
+  return mul2(q, pair(__int_as_float(__float_as_int(n.x) << 23), __int_as_float(__float_as_int(n.y) << 23)));
+}
+// One pair of keys in POLY_OF goes through the polynomial. Measured on a
+// 2 x 2048-token prefill over 8192 keys: none 168, 1/8 157, 1/4 157, 3/8 166,
+// 1/2 185 us.
+constexpr int POLY_OF = 8;
 
 // Four K = 16 steps of one product, issued by one elected lane of a converged
 // warp: A in shared memory (descriptor steps of 32 bytes) or in tensor memory
@@ -789,6 +846,31 @@ __device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint
       : "memory");
 }
 
+// A value every lane of the warp holds, in a form the compiler knows to be
+// uniform: what is computed from it stays in the uniform datapath, where the
+// tensor instructions take their operands from.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// Whole-warp bounded wait that suspends in the barrier instead of polling: the
+// producer and the issuer share their schedulers with two softmax warps each,
+// and every issue slot they spin in is taken from those.
+__device__ __forceinline__ bool wait_quiet(uint32_t bar, uint32_t parity, int* status, int code) {
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, done)) return true;
+    if (__any_sync(0xffffffffu, clock64() - t0 > (1LL << 32))) {
+      atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(T_THREADS, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -808,7 +890,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
   const uint32_t o_free = pv_done(2), done_bar = o_free + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 8 * S::NBARS);
   __shared__ int s_flag;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   int* status = &g_status;
 
   if (tid == 0) {
@@ -821,7 +903,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     tc::mbar_init(tail_bar, 1);
     for (int i = 0; i < S::NB; ++i) {
       tc::mbar_init(s_full(i), 1);
-      tc::mbar_init(p_full(i), 128);
+      tc::mbar_init(p_full(i), 4);  // one arrival per warp
     }
     tc::mbar_init(pv_done(0), 1);
     tc::mbar_init(pv_done(1), 1);
@@ -832,162 +914,155 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     tc::tma_prefetch_desc(&tk);
     tc::tma_prefetch_desc(&tv);
   }
-  if (warp == 1) {
+  if (warp == 9) {
     tc::tmem_alloc(smem_u32(tmem_slot), 512);
     tc::tmem_relinquish();
   }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   wait_prerequisites();
   allow_dependents();
   const Header head = *p.head;
   const Item start = p.starts[blockIdx.x];
   const int share = blockIdx.x;
-  const bool idle = share >= head.shares || head.total == 0;
+  const bool idle = uniform(share >= head.shares || head.total == 0);
   const int x0 = idle ? 0 : share_begin(head, share), x1 = idle ? 0 : share_begin(head, share + 1);
   const int G = p.G, tpt = 128 / G;  // tokens per query tile
   const int page = 1 << p.page_shift, br = min(128, page), nb = 128 / br;
 
-  if (idle) {
-    // nothing to do
-  } else if (warp == 0) {
-    int slot = 0, slot_ph = 0, fills = 0, seg = 0, tails = 0;
-    bool ok = true;
-    for (Item w = start; ok;) {
-      const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
-      if (n > 0) {
-        const bool dual = w.ntok > tpt;
-        if (!(ok = tc::mbar_wait_w(q_empty, (seg & 1) ^ 1, status, 11))) break;
-        ++seg;
-        if (lane == 0) {
-          const int tiles = dual ? 2 : 1;
-          tc::mbar_expect_tx(q_full, (uint32_t)(tiles * DH * tpt * G * 128));
-          for (int t = 0; t < tiles; ++t)
-            for (int h = 0; h < DH; ++h)
-              tc::tma_load_3d(sb + S::Q + t * S::SLOT + h * 16384u, &tq, h * 64, w.hg * G, w.tok0 + t * tpt, q_full);
-        }
-        __syncwarp();
-        auto look = [&](int j) {
-          const int key = j * 128 + lane * br;
-          return j < j1 && lane < nb && key < w.keys ? page_id(p, w.b, key) : 0;
-        };
-        // Page ids of the next K and of the next V tile.
-        int id_k = look(j0), id_v = id_k, kj = j0, vj = j0;
-        auto load = [&](const CUtensorMap* map, int j, int id, bool is_v) {
-          if (!(ok = tc::mbar_wait_w(empty_bar(slot), slot_ph ^ 1, status, 12))) return;
-          const int valid = min(128, w.keys - j * 128), live = cdiv(max(valid, 0), br);
-          const bool tail = is_v && valid < 128;
-          const uint32_t bar = tail ? tail_bar : full_bar(slot), dst = sb + S::RING + slot * S::SLOT;
-          if (lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(live * br * 128 * DH));
-          __syncwarp();
-          const int bx = lane % max(live, 1), half = lane / max(live, 1);
-          const int pid = __shfl_sync(0xffffffffu, id, bx);
-          if (half < DH && lane < live * DH)
-            tma_load_4d(dst + half * 16384u + bx * br * 128, map, half * 64, (j * 128 + bx * br) & (page - 1), w.hg,
-                        pid, bar);
-          if (tail) {
-            // Rows past the sequence hold whatever the page (or the ring) held;
-            // zeros in their place, since 0 x NaN would not vanish in P V.
-            ok = tc::mbar_wait_w(tail_bar, tails & 1, status, 13);
-            ++tails;
-            for (int i = max(valid, 0) * 8 + lane; i < 128 * 8; i += 32)
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(OTHER_REGS));
+    if (!idle && warp == 8) {
+      int slot = 0, slot_ph = 0, fills = 0, seg = 0, tails = 0;
+      bool ok = true;
+      for (Item w = start; ok;) {
+        const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
+        if (n > 0) {
+          const bool dual = w.ntok > tpt;
+          if (!(ok = wait_quiet(q_empty, (seg & 1) ^ 1, status, 11))) break;
+          ++seg;
+          if (lane == 0) {
+            const int tiles = dual ? 2 : 1;
+            tc::mbar_expect_tx(q_full, (uint32_t)(tiles * DH * tpt * G * 128));
+            for (int t = 0; t < tiles; ++t)
               for (int h = 0; h < DH; ++h)
-                *reinterpret_cast<uint4*>(smem + S::RING + slot * S::SLOT + h * 16384u + i * 16) = make_uint4(0, 0, 0, 0);
-            tc::fence_proxy_async_smem();
+                tc::tma_load_3d(sb + S::Q + t * S::SLOT + h * 16384u, &tq, h * 64, w.hg * G, w.tok0 + t * tpt, q_full);
+          }
+          __syncwarp();
+          const int end = min(w.keys, j1 * 128);
+          PageIds k_ids(p, w.b, br, nb, j0, end), v_ids = k_ids;
+          int kj = j0, vj = j0;
+          auto load = [&](const CUtensorMap* map, int j, PageIds& ids, bool is_v) {
+            if (!(ok = wait_quiet(empty_bar(slot), slot_ph ^ 1, status, 12))) return;
+            const int valid = min(128, w.keys - j * 128), live = cdiv(max(valid, 0), br);
+            const bool tail = is_v && valid < 128;
+            const uint32_t bar = tail ? tail_bar : full_bar(slot), dst = sb + S::RING + slot * S::SLOT;
+            if (lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(live * br * 128 * DH));
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(full_bar(slot));
-          }
-          ++fills;
-          if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
-        };
-        // Jobs' order of need: step s runs the product of job s - NB, then the
-        // scores of job s.
-        const int jobs = dual ? 2 * n : n;
-        for (int st = 0; ok && st < jobs + S::NB; ++st) {
-          const int pj = st - S::NB;
-          if (pj >= 0 && (!dual || !(pj & 1))) {
-            load(&tv, vj, id_v, true);
-            id_v = look(++vj);
-            if (!ok) break;
-          }
-          if (st < jobs && (!dual || !(st & 1))) {
-            load(&tk, kj, id_k, false);
-            id_k = look(++kj);
+            const int bx = lane % max(live, 1), half = lane / max(live, 1);
+            const int pid = ids.get(p, j, bx);
+            if (half < DH && lane < live * DH)
+              tma_load_4d(dst + half * 16384u + bx * br * 128, map, half * 64, (j * 128 + bx * br) & (page - 1), w.hg,
+                          pid, bar);
+            if (tail) {
+              // Rows past the sequence hold whatever the page (or the ring) held;
+              // zeros in their place, since 0 x NaN would not vanish in P V.
+              ok = wait_quiet(tail_bar, tails & 1, status, 13);
+              ++tails;
+              for (int i = max(valid, 0) * 8 + lane; i < 128 * 8; i += 32)
+                for (int h = 0; h < DH; ++h)
+                  *reinterpret_cast<uint4*>(smem + S::RING + slot * S::SLOT + h * 16384u + i * 16) = make_uint4(0, 0, 0, 0);
+              tc::fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) tc::mbar_arrive(full_bar(slot));
+            }
+            ++fills;
+            if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+          };
+          // Jobs' order of need: step s runs the product of job s - NB, then the
+          // scores of job s.
+          const int jobs = dual ? 2 * n : n;
+          for (int st = 0; ok && st < jobs + S::NB; ++st) {
+            const int pj = st - S::NB;
+            if (pj >= 0 && (!dual || !(pj & 1))) {
+              load(&tv, vj++, v_ids, true);
+              if (!ok) break;
+            }
+            if (st < jobs && (!dual || !(st & 1))) {
+              load(&tk, kj++, k_ids, false);
+            }
           }
         }
+        if (!advance(p, w, x1)) break;
       }
-      if (!advance(p, w, x1)) break;
-    }
-    if (!ok)  // a wait gave up: let the copies in flight land before the CTA ends
-      for (int f = max(0, fills - S::SLOTS); f < fills; ++f)
-        tc::mbar_wait_w(full_bar(f % S::SLOTS), (f / S::SLOTS) & 1, status, 14);
-  } else if (warp == 1) {
-    // Item fields are broadcast from lane 0, so that the compiler knows the
-    // loop to be uniform and keeps the operands in the uniform datapath.
-    // Item fields are broadcast from lane 0, so that the compiler knows the
-    // loop to be uniform and keeps the operands in the uniform datapath.
-    const uint32_t idesc_s = idesc16(BF, 128, 0), idesc_o = idesc16(BF, D, 1);
-    const uint64_t q_desc = tc::smem_desc_sw128(sb + S::Q, 16, 1024);
-    const uint64_t k_desc = tc::smem_desc_sw128(sb + S::RING, 16, 1024);
-    const uint64_t v_desc = tc::smem_desc_sw128(sb + S::RING, 16384, 1024);
-    int slot = 0, slot_ph = 0, seg = 0;
-    int sbuf = 0, pbuf = 0, pph = 0;  // buffer of the next scores, of the next product, and its phase
-    bool ok = true;
-    for (Item w = start; ok;) {
-      const int n = __shfl_sync(0xffffffffu, unit_at(w, x1) - unit_at(w, x0), 0);
-      if (n > 0) {
-        const bool dual = __shfl_sync(0xffffffffu, w.ntok, 0) > tpt;
-        const int jobs = dual ? 2 * n : n;
-        int ks = 0, vs = 0;
-        if (!(ok = tc::mbar_wait_w(q_full, seg & 1, status, 21))) break;
-        for (int st = 0; ok && st < jobs + S::NB; ++st) {
-          const int pj = st - S::NB;
-          if (pj >= 0) {
-            if (!dual || !(pj & 1)) {
-              vs = slot;
-              if (!(ok = tc::mbar_wait_w(full_bar(vs), slot_ph, status, 22))) break;
-              if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+      if (!ok)  // a wait gave up: let the copies in flight land before the CTA ends
+        for (int f = max(0, fills - S::SLOTS); f < fills; ++f)
+          wait_quiet(full_bar(f % S::SLOTS), (f / S::SLOTS) & 1, status, 14);
+    } else if (!idle && warp == 9) {
+      const uint32_t idesc_s = idesc16(BF, 128, 0), idesc_o = idesc16(BF, D, 1);
+      const uint64_t q_desc = tc::smem_desc_sw128(sb + S::Q, 16, 1024);
+      const uint64_t k_desc = tc::smem_desc_sw128(sb + S::RING, 16, 1024);
+      const uint64_t v_desc = tc::smem_desc_sw128(sb + S::RING, 16384, 1024);
+      int slot = 0, slot_ph = 0, seg = 0;
+      int sbuf = 0, pbuf = 0, pph = 0;  // buffer of the next scores, of the next product, and its phase
+      bool ok = true;
+      for (Item w = start; ok;) {
+        const int n = uniform(unit_at(w, x1) - unit_at(w, x0));
+        if (n > 0) {
+          const bool dual = uniform(w.ntok) > tpt;
+          const int jobs = dual ? 2 * n : n;
+          int ks = 0, vs = 0;
+          if (!(ok = wait_quiet(q_full, seg & 1, status, 21))) break;
+          for (int st = 0; ok && st < jobs + S::NB; ++st) {
+            const int pj = st - S::NB;
+            if (pj >= 0) {
+              if (!dual || !(pj & 1)) {
+                vs = slot;
+                if (!(ok = wait_quiet(full_bar(vs), slot_ph, status, 22))) break;
+                if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+              }
+              // The output accumulators of the previous item are read out.
+              if (pj == 0 && !(ok = wait_quiet(o_free, (seg & 1) ^ 1, status, 24))) break;
+              if (!(ok = wait_quiet(p_full(pbuf), pph, status, 25))) break;
+              tc::tc_fence_after();
+              const uint32_t o_t = tmem + S::O + (pj & 1) * D, p_t = tmem + pbuf * 128;
+              const uint64_t vd = v_desc + (uint64_t)(vs * (S::SLOT >> 4));
+              mma4_ts(o_t, p_t, vd, idesc_o, pj > 1 ? 1u : 0u);
+              mma4_ts(o_t, p_t + 32, vd + 512, idesc_o, 1u);
+              tc::mma_commit_w(pv_done(pj & 1));
+              if (!dual || (pj & 1)) tc::mma_commit_w(empty_bar(vs));
+              if (++pbuf == S::NB) pbuf = 0, pph ^= 1;
             }
-            // The output accumulators of the previous item are read out.
-            if (pj == 0 && !(ok = tc::mbar_wait_w(o_free, (seg & 1) ^ 1, status, 24))) break;
-            if (!(ok = tc::mbar_wait_w(p_full(pbuf), pph, status, 25))) break;
-            tc::tc_fence_after();
-            const uint32_t o_t = tmem + S::O + (pj & 1) * D, p_t = tmem + pbuf * 128;
-            const uint64_t vd = v_desc + (uint64_t)(vs * (S::SLOT >> 4));
-            mma4_ts(o_t, p_t, vd, idesc_o, pj > 1 ? 1u : 0u);
-            mma4_ts(o_t, p_t + 32, vd + 512, idesc_o, 1u);
-            tc::mma_commit_w(pv_done(pj & 1));
-            if (!dual || (pj & 1)) tc::mma_commit_w(empty_bar(vs));
-            if (++pbuf == S::NB) pbuf = 0, pph ^= 1;
-          }
-          if (st < jobs) {
-            if (!dual || !(st & 1)) {
-              ks = slot;
-              if (!(ok = tc::mbar_wait_w(full_bar(ks), slot_ph, status, 23))) break;
-              if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+            if (st < jobs) {
+              if (!dual || !(st & 1)) {
+                ks = slot;
+                if (!(ok = wait_quiet(full_bar(ks), slot_ph, status, 23))) break;
+                if (++slot == S::SLOTS) slot = 0, slot_ph ^= 1;
+              }
+              tc::tc_fence_after();
+              const uint32_t s_t = tmem + sbuf * 128;
+              const uint64_t qd = q_desc + (uint64_t)(dual && (st & 1) ? S::SLOT >> 4 : 0);
+              const uint64_t kd = k_desc + (uint64_t)(ks * (S::SLOT >> 4));
+              mma4_ss(s_t, qd, kd, idesc_s, 0u);
+              if (D == 128) mma4_ss(s_t, qd + 1024, kd + 1024, idesc_s, 1u);
+              tc::mma_commit_w(s_full(sbuf));
+              if (!dual || (st & 1)) tc::mma_commit_w(empty_bar(ks));
+              if (st == jobs - 1) tc::mma_commit_w(q_empty);
+              if (++sbuf == S::NB) sbuf = 0;
             }
-            tc::tc_fence_after();
-            const uint32_t s_t = tmem + sbuf * 128;
-            const uint64_t qd = q_desc + (uint64_t)(dual && (st & 1) ? S::SLOT >> 4 : 0);
-            const uint64_t kd = k_desc + (uint64_t)(ks * (S::SLOT >> 4));
-            mma4_ss(s_t, qd, kd, idesc_s, 0u);
-            if (D == 128) mma4_ss(s_t, qd + 1024, kd + 1024, idesc_s, 1u);
-            tc::mma_commit_w(s_full(sbuf));
-            if (!dual || (st & 1)) tc::mma_commit_w(empty_bar(ks));
-            if (st == jobs - 1) tc::mma_commit_w(q_empty);
-            if (++sbuf == S::NB) sbuf = 0;
           }
+          ++seg;
         }
-        ++seg;
+        if (!uniform(advance(p, w, x1))) break;
       }
-      if (!advance(p, w, x1)) break;
+      tc::mma_commit_w(done_bar);
+      wait_quiet(done_bar, 0, status, 26);
     }
-    tc::mma_commit_w(done_bar);
-    tc::mbar_wait_w(done_bar, 0, status, 26);
   } else {
-    const int grp = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane, stid = tid - 64;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(SOFTMAX_REGS));
+    const int grp = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t o_t = tmem + lane_off + S::O + grp * D;
     float2* ml_s = reinterpret_cast<float2*>(smem + S::ML);
@@ -995,7 +1070,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     int nj0 = 0, nj1 = 0;  // jobs each group has had
     int buf = 0, ph = 0;   // buffer and phase of the item's job 0
     bool ok = true;
-    for (Item w = start;;) {
+    for (Item w = start; !idle;) {
       const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
       if (n <= 0) {
         if (!advance(p, w, x1)) break;
@@ -1020,25 +1095,22 @@ __global__ void __launch_bounds__(T_THREADS, 1)
           const int lim = limit - (j0 + (dual ? j >> 1 : j)) * 128;
           const bool masked = __any_sync(0xffffffffu, lim < 128);
           tc::tc_fence_after();
-          // Maximum of the row's 128 scores; the second 64 stay in registers,
-          // the first are read again when their turn comes.
-          uint32_t v[64];
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          uint32_t v[128];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            tc::tmem_ld_32x32b_x32(s_t + half * 64, v);
-            tc::tmem_ld_32x32b_x32(s_t + half * 64 + 32, v + 32);
-            tc::tmem_ld_wait();
-            if (masked) {
+          for (int c = 0; c < 4; ++c) tc::tmem_ld_32x32b_x32(s_t + c * 32, v + c * 32);
+          tc::tmem_ld_wait();
+          if (masked) {
 #pragma unroll
-              for (int i = 0; i < 64; ++i) v[i] = half * 64 + i < lim ? v[i] : 0xFF800000u;
-            }
-#pragma unroll
-            for (int i = 0; i < 64; i += 8)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                mx[e] = max3(mx[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + e + 4]));
+            for (int i = 0; i < 128; ++i) v[i] = i < lim ? v[i] : 0xFF800000u;
           }
+          float mx[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 4]));
+#pragma unroll
+          for (int i = 8; i < 128; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              mx[e] = max3(mx[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + e + 4]));
           const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sl2;
           const bool up = top > M + 8.f, move = up && M != -INFINITY;
           if (__any_sync(0xffffffffu, move)) {
@@ -1061,37 +1133,46 @@ __global__ void __launch_bounds__(T_THREADS, 1)
           if (up) M = top;
           const float neg = M == -INFINITY ? 0.f : -M;
           const uint64_t sl = pair(sl2, sl2), ng = pair(neg, neg);
-          // P over the scores: 16-bit pairs in the first 64 columns. Scores
-          // 0-63 are read before their columns are written.
-          auto weigh = [&](const uint32_t* x, uint32_t* pk) {
+          // P over the scores: 16-bit pairs in the first 64 columns. Blocks of
+          // 32 keys, the sums and conversions of one behind the exponentials
+          // of the next, so that the special-function unit is rarely waited for.
+          uint64_t e[2][16], sum[4] = {l2, pair(0.f, 0.f), pair(0.f, 0.f), pair(0.f, 0.f)};
+          auto weigh = [&](int c, uint64_t* out) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float2 e = unpair(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sl, ng));
-              const float e0 = ex2(e.x), e1 = ex2(e.y);
-              l2 = add2(l2, pair(e0, e1));
-              pk[i >> 1] = Num16<T>::pack2(e0, e1);
+            for (int i = 0; i < 16; ++i) {
+              const int k = c * 32 + 2 * i;
+              const uint64_t x = fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), sl, ng);
+              if (i % POLY_OF == 0) {
+                out[i] = ex2_poly2(x);
+              } else {
+                const float2 f = unpair(x);
+                out[i] = pair(ex2(f.x), ex2(f.y));
+              }
             }
           };
-          uint32_t y[64], pk[32];
-          weigh(v, pk);
-          tc::tmem_ld_32x32b_x32(s_t, y);
-          weigh(v + 32, pk + 16);
-          tc::tmem_ld_32x32b_x32(s_t + 32, y + 32);
-          tc::tmem_ld_wait();
-          tc::tmem_st_32x32b_x16(s_t + 32, pk);
-          tc::tmem_st_32x32b_x16(s_t + 48, pk + 16);
-          if (masked) {
+          auto store = [&](int c, const uint64_t* in) {
+            uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) y[i] = i < lim ? y[i] : 0xFF800000u;
+            for (int i = 0; i < 16; ++i) {
+              sum[i & 3] = add2(sum[i & 3], in[i]);
+              const float2 f = unpair(in[i]);
+              pk[i] = Num16<T>::pack2(f.x, f.y);
+            }
+            tc::tmem_st_32x32b_x16(s_t + c * 16, pk);
+          };
+          weigh(0, e[0]);
+#pragma unroll
+          for (int c = 1; c < 4; ++c) {
+            weigh(c, e[c & 1]);
+            store(c - 1, e[(c - 1) & 1]);
           }
-          weigh(y, pk);
-          tc::tmem_st_32x32b_x16(s_t, pk);
-          weigh(y + 32, pk + 16);
-          tc::tmem_st_32x32b_x16(s_t + 16, pk + 16);
+          store(3, e[1]);
+          l2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
           tc::tmem_st_wait();
           tc::tc_fence_before();
         }
-        tc::mbar_arrive(p_full(bj));
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_full(bj));
         bj += 2;
         if (bj >= S::NB) bj -= S::NB, pj ^= 1;
       }
@@ -1175,7 +1256,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
       }
       tc::mbar_arrive(o_free);
       if (cut)
-        join_cut<D, true, 4, 4>(p, head, w, share, w.ntok * G, stid, &s_flag,
+        join_cut<D, true, 4, 4>(p, head, w, share, w.ntok * G, tid, &s_flag,
                              [&](int row, int d4, float mm, float ll, const float4* a) {
                                const float inv = ll > 0.f ? 1.f / ll : 0.f;
                                const long long at = (long long)(w.tok0 + row / G) * p.H + w.hg * G + row % G;
@@ -1194,7 +1275,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 9) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
