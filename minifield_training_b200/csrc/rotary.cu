@@ -18,9 +18,13 @@
 // Layout: a warp owns a token (or one of `slices` interleaved shares of its
 // heads, for calls with few tokens) and D/8 lanes own a head, 8 values (16
 // bytes) each, so every load and store is a full 128-byte line or more. The
-// warp computes each of the token's rotary_dim/2 angles once, keeps them in
-// shared memory and reads back the lane's own; a half-layout partner is
-// rotary_dim/16 lanes away (shuffle), an interleaved one in the same lane.
+// warp computes each of the token's rotary_dim/2 angles once and passes them
+// through shared memory. With cw = cos * w and sw = -+sin * w_partner per lane,
+//   y = r (x cw + x_partner sw),
+// and the partners are exchanged as the raw 16-bit words: rotary_dim/16 lanes
+// away in the half layout, in the same lane in the interleaved one. The pass is
+// bandwidth-bound; registers are held down so that enough warps have loads in
+// flight (q, k and v heads run in loops of their own, one set of gains live).
 #include <algorithm>
 
 #include "types16.cuh"
@@ -30,7 +34,7 @@ namespace rot {
 
 constexpr int WARPS = 8;
 constexpr int MAX_D = 128;
-constexpr int BWD_GRID_MAX = 4 * 160;  // bounds the gain-gradient partials
+constexpr int BWD_GRID_MAX = 3 * 160;  // bounds the gain-gradient partials
 constexpr double kInvTwoPi = 0.15915494309189533577;
 
 struct Params {
@@ -59,64 +63,59 @@ struct Params {
   float amplitude, eps;
 };
 
-// cos and sin of a position's angles: lane-parallel, one per pair, into the
-// warp's table; then this lane's own into c / s (1 and 0 where not rotated).
-// Half layout: values sub*8 + e use pair (sub*8 + e) mod (rotary_dim / 2).
-// Interleaved: values 2j and 2j + 1 use pair sub*4 + j.
-template <bool IL>
-__device__ __forceinline__ void angles(const Params& p, int pos, float2* table, int lane, int sub, float* c, float* s) {
-  const int half = p.rotary_dim >> 1;
+// The angles of a position into the warp's table: (cos, sin) times amplitude.
+__device__ __forceinline__ void angles(const Params& p, int pos, float2* table, int lane) {
   __syncwarp();
-  for (int i = lane; i < half; i += 32) {
+  for (int i = lane; i < p.rotary_dim >> 1; i += 32) {
     const double t = (double)pos * (double)p.freqs[i] * kInvTwoPi;
     float sn, cs;
     sincospif(2.f * (float)(t - rint(t)), &sn, &cs);
     table[i] = make_float2(cs * p.amplitude, sn * p.amplitude);
   }
   __syncwarp();
-  if (sub * 8 < p.rotary_dim) {
-    if (IL) {
+}
+
+// This lane's coefficients: value e becomes x cw + partner sw. Half layout:
+// values sub*8 + e use pair (sub*8 + e) mod (rotary_dim / 2); interleaved:
+// values 2j and 2j + 1 use pair sub*4 + j. INV rotates back (R^T); w (and the
+// partner's wp) multiply the inputs.
+template <bool IL, bool INV>
+__device__ __forceinline__ void coefficients(const Params& p, const float2* table, int sub, bool turned, bool low,
+                                             const float* gains, float* cw, float* sw) {
+  const int half = p.rotary_dim >> 1;
+  float w[8], wp[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = table[sub * 4 + j];
-        c[2 * j] = c[2 * j + 1] = f.x;
-        s[2 * j] = s[2 * j + 1] = f.y;
-      }
-    } else {
-      const int base = sub * 8 < half ? sub * 8 : sub * 8 - half;
+  for (int e = 0; e < 8; ++e) w[e] = wp[e] = 1.f;
+  if (gains) {
+    const int mine = sub * 8, other = !turned || IL ? mine : (low ? mine + half : mine - half);
+    const float4 a = reinterpret_cast<const float4*>(gains + mine)[0], b = reinterpret_cast<const float4*>(gains + mine)[1];
+    const float4 c = reinterpret_cast<const float4*>(gains + other)[0], d = reinterpret_cast<const float4*>(gains + other)[1];
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    wp[0] = c.x, wp[1] = c.y, wp[2] = c.z, wp[3] = c.w, wp[4] = d.x, wp[5] = d.y, wp[6] = d.z, wp[7] = d.w;
+  }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 f = table[base + e];
-        c[e] = f.x;
-        s[e] = f.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = 1.f, s[e] = 0.f;
+  for (int e = 0; e < 8; ++e) {
+    float2 f = make_float2(1.f, 0.f);
+    if (turned) f = table[IL ? sub * 4 + e / 2 : (low ? sub * 8 + e : sub * 8 + e - half)];
+    const bool minus = (IL ? (e & 1) == 0 : low) != INV;  // y_first = x_first c - x_second s
+    cw[e] = f.x * w[e];
+    sw[e] = (minus ? -f.y : f.y) * (IL ? wp[e ^ 1] : wp[e]);
   }
 }
 
-// x <- R x, or R^T x for INV (the angles negated). `from` is the lane holding
-// the half-layout partners (this lane itself where nothing is rotated), `low`
-// whether this lane holds the first of each pair.
-template <bool IL, bool INV>
-__device__ __forceinline__ void rotate(float* x, const float* c, const float* s, int from, bool low) {
+// The partners' raw words (zeros where nothing is rotated).
+template <bool IL>
+__device__ __forceinline__ uint4 partners(const uint4& v, int from, bool turned) {
   if (IL) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float a = x[2 * j], b = x[2 * j + 1], sn = INV ? -s[2 * j] : s[2 * j];
-      x[2 * j] = a * c[2 * j] - b * sn;
-      x[2 * j + 1] = b * c[2 * j] + a * sn;
-    }
-  } else {
-    const bool minus = low != INV;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float o = __shfl_sync(0xffffffffu, x[e], from);
-      x[e] = fmaf(minus ? -o : o, s[e], x[e] * c[e]);
-    }
+    return make_uint4(__byte_perm(v.x, 0, 0x1032), __byte_perm(v.y, 0, 0x1032), __byte_perm(v.z, 0, 0x1032),
+                      __byte_perm(v.w, 0, 0x1032));
   }
+  uint4 o;
+  o.x = __shfl_sync(0xffffffffu, v.x, from);
+  o.y = __shfl_sync(0xffffffffu, v.y, from);
+  o.z = __shfl_sync(0xffffffffu, v.z, from);
+  o.w = __shfl_sync(0xffffffffu, v.w, from);
+  return turned ? o : make_uint4(0, 0, 0, 0);
 }
 
 template <int L>
@@ -137,8 +136,29 @@ __device__ __forceinline__ int sequence_of(const int* cu_q, int B, int t) {
   return lo;
 }
 
+__device__ __forceinline__ uint4 ld16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ void st16(uint16_t* p, const uint4& v) { *reinterpret_cast<uint4*>(p) = v; }
+
+// Runs body(i, h, live) over this warp's heads [0, n) in steps of `step`, four
+// steps' loads ahead of their use: load(h) -> uint4. All lanes take part in
+// every step (shuffles); heads past the end are not live.
+template <int AHEAD, typename Load, typename Body>
+__device__ __forceinline__ void over_heads(int first, int grp, int step, int n, Load load, Body body) {
+  for (int h0 = first; h0 < n; h0 += AHEAD * step) {
+    uint4 v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int h = h0 + i * step + grp;
+      v[i] = h < n ? load(h) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (h0 + i * step < n) body(h0 + i * step + grp, h0 + i * step + grp < n, v[i]);
+  }
+}
+
 template <typename T, int D, bool IL, bool PAGED>
-__global__ void __launch_bounds__(32 * WARPS) rotary_fwd_kernel(Params p) {
+__global__ void __launch_bounds__(32 * WARPS, 4) rotary_fwd_kernel(Params p) {
   constexpr int L = D / 8, HPW = 32 / L;  // lanes per head, heads per warp
   __shared__ float2 tables[WARPS][MAX_D / 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L, grp = lane / L;
@@ -146,24 +166,10 @@ __global__ void __launch_bounds__(32 * WARPS) rotary_fwd_kernel(Params p) {
   const bool turned = sub * 8 < p.rotary_dim, low = sub < half8;
   const int from = turned ? (low ? lane + half8 : lane - half8) : lane;
   const bool norm = p.wq != nullptr;
-  float wq[8], wk[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    wq[e] = norm ? p.wq[sub * 8 + e] : 1.f;
-    wk[e] = norm ? p.wk[sub * 8 + e] : 1.f;
-  }
-  const int heads = p.H + (p.v ? 2 : 1) * p.Hk;
   const long long units = (long long)p.M * p.slices, step = (long long)gridDim.x * WARPS;
   for (long long u = (long long)blockIdx.x * WARPS + warp; u < units; u += step) {
-    const int row = (int)(u / p.slices), slice = (int)(u % p.slices);
+    const int row = (int)(u / p.slices), first = (int)(u % p.slices) * HPW, hstep = p.slices * HPW;
     const uint16_t* src = p.qkv + (long long)row * p.ld + sub * 8;
-    // Four heads' loads in flight before the first is used.
-    int h = slice * HPW + grp;
-    const int hstep = p.slices * HPW;
-    uint4 buf[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (h + i * hstep < heads) buf[i] = *reinterpret_cast<const uint4*>(src + (long long)(h + i * hstep) * D);
     int pos;
     long long slot = -1;  // element offset of the token's first head in the pages; -1: not stored
     if (PAGED) {
@@ -178,48 +184,44 @@ __global__ void __launch_bounds__(32 * WARPS) rotary_fwd_kernel(Params p) {
       }
     } else {
       pos = p.positions[row];
+      slot = (long long)row * p.Hk * D;
     }
-    float c[8], s[8];
-    angles<IL>(p, pos, tables[warp], lane, sub, c, s);
-    // The warp's heads in steps; a step past the end runs on for its shuffles.
-    for (int h0 = slice * HPW; h0 < heads; h0 += 4 * hstep) {
+    // Values: copied. Their loads are under way while the angles are computed.
+    if (p.v && slot >= 0)
+      over_heads<4>(first, grp, hstep, p.Hk, [&](int h) { return ld16(src + (long long)(p.H + p.Hk + h) * D); },
+                    [&](int h, bool live, const uint4& v) {
+                      if (live) st16(p.v + slot + (long long)h * p.head_stride + sub * 8, v);
+                    });
+    angles(p, pos, tables[warp], lane);
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+      float cw[8], sw[8];
+      coefficients<IL, false>(p, tables[warp], sub, turned, low, which ? p.wk : p.wq, cw, sw);
+      const uint16_t* in = src + (which ? (long long)p.H * D : 0);
+      uint16_t* out = which ? p.k + slot : p.q + (long long)row * p.H * D;
+      const long long hs = which ? p.head_stride : D;
+      const bool stored = !which || slot >= 0;
+      over_heads<4>(first, grp, hstep, which ? p.Hk : p.H, [&](int h) { return ld16(in + (long long)h * D); },
+                    [&](int h, bool live, const uint4& v) {
+                      float x[8], y[8], r = 1.f;
+                      unpack16x8<T>(v, x);
+                      unpack16x8<T>(partners<IL>(v, from, turned), y);
+                      if (norm) {
+                        float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (h0 + i * hstep >= heads) break;
-        const int hh = h0 + i * hstep + grp;
-        const bool live = hh < heads;
-        const uint4 raw = live ? buf[i] : make_uint4(0, 0, 0, 0);
-        const int next = hh + 4 * hstep;
-        if (next < heads) buf[i] = *reinterpret_cast<const uint4*>(src + (long long)next * D);
-        const bool is_q = hh < p.H, is_k = !is_q && hh < p.H + p.Hk;
-        float x[8];
-        unpack16x8<T>(raw, x);
-        if (norm) {
-          float ss = 0.f;
+                        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+                        r = rsqrtf(head_sum<L>(ss) * (1.f / D) + p.eps);
+                      }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-          const float r = rsqrtf(head_sum<L>(ss) * (1.f / D) + p.eps);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= r * (is_q ? wq[e] : wk[e]);
-        }
-        rotate<IL, false>(x, c, s, from, low);
-        if (!live) continue;
-        if (is_q) {
-          *reinterpret_cast<uint4*>(p.q + ((long long)row * p.H + hh) * D + sub * 8) = pack16x8<T>(x);
-        } else {
-          const int kh = is_k ? hh - p.H : hh - p.H - p.Hk;
-          uint16_t* dst = is_k ? p.k : p.v;
-          const uint4 out = is_k ? pack16x8<T>(x) : raw;
-          if (!PAGED) *reinterpret_cast<uint4*>(dst + ((long long)row * p.Hk + kh) * D + sub * 8) = out;
-          else if (slot >= 0) *reinterpret_cast<uint4*>(dst + slot + (long long)kh * p.head_stride + sub * 8) = out;
-        }
-      }
+                      for (int e = 0; e < 8; ++e) x[e] = fmaf(y[e], sw[e], x[e] * cw[e]) * r;
+                      if (live && stored) st16(out + h * hs + sub * 8, pack16x8<T>(x));
+                    });
     }
   }
 }
 
 template <typename T, int D, bool IL>
-__global__ void __launch_bounds__(32 * WARPS) rotary_bwd_kernel(Params p) {
+__global__ void __launch_bounds__(32 * WARPS, 3) rotary_bwd_kernel(Params p) {
   constexpr int L = D / 8, HPW = 32 / L;
   __shared__ float2 tables[WARPS][MAX_D / 2];
   __shared__ float sums[WARPS][2 * D];
@@ -228,86 +230,83 @@ __global__ void __launch_bounds__(32 * WARPS) rotary_bwd_kernel(Params p) {
   const bool turned = sub * 8 < p.rotary_dim, low = sub < half8;
   const int from = turned ? (low ? lane + half8 : lane - half8) : lane;
   const bool norm = p.wq != nullptr;
-  float wq[8], wk[8], accq[8], acck[8];
+  float acc[2][8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    wq[e] = norm ? p.wq[sub * 8 + e] : 1.f;
-    wk[e] = norm ? p.wk[sub * 8 + e] : 1.f;
-    accq[e] = acck[e] = 0.f;
-  }
-  const int heads = p.H + 2 * p.Hk;
+  for (int e = 0; e < 8; ++e) acc[0][e] = acc[1][e] = 0.f;
   const long long units = (long long)p.M * p.slices, step = (long long)gridDim.x * WARPS;
   for (long long u = (long long)blockIdx.x * WARPS + warp; u < units; u += step) {
-    const int row = (int)(u / p.slices), slice = (int)(u % p.slices);
+    const int row = (int)(u / p.slices), first = (int)(u % p.slices) * HPW, hstep = p.slices * HPW;
     const long long base = (long long)row * p.ld + sub * 8;
-    const int hstep = p.slices * HPW;
-    auto upstream = [&](int hh) {
-      const uint16_t* g = hh < p.H ? p.dq + ((long long)row * p.H + hh) * D
-                                   : (hh < p.H + p.Hk ? p.dk + ((long long)row * p.Hk + hh - p.H) * D
-                                                      : p.dv + ((long long)row * p.Hk + hh - p.H - p.Hk) * D);
-      return *reinterpret_cast<const uint4*>(g + sub * 8);
-    };
-    uint4 bg[2], bx[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int hh = slice * HPW + grp + i * hstep;
-      bg[i] = bx[i] = make_uint4(0, 0, 0, 0);
-      if (hh < heads) bg[i] = upstream(hh);
-      if (norm && hh < p.H + p.Hk) bx[i] = *reinterpret_cast<const uint4*>(p.qkv + base + (long long)hh * D);
-    }
+    over_heads<4>(first, grp, hstep, p.Hk, [&](int h) { return ld16(p.dv + ((long long)row * p.Hk + h) * D + sub * 8); },
+                  [&](int h, bool live, const uint4& v) {
+                    if (live) st16(p.dqkv + base + (long long)(p.H + p.Hk + h) * D, v);
+                  });
+    angles(p, p.positions[row], tables[warp], lane);
     float c[8], s[8];
-    angles<IL>(p, p.positions[row], tables[warp], lane, sub, c, s);
-    for (int h0 = slice * HPW; h0 < heads; h0 += 2 * hstep) {
+    coefficients<IL, true>(p, tables[warp], sub, turned, low, nullptr, c, s);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (h0 + i * hstep >= heads) break;
-        const int hh = h0 + i * hstep + grp;
-        const bool live = hh < heads;
-        const uint4 graw = bg[i], xraw = bx[i];
-        const int next = hh + 2 * hstep;
-        if (next < heads) bg[i] = upstream(next);
-        if (norm && next < p.H + p.Hk) bx[i] = *reinterpret_cast<const uint4*>(p.qkv + base + (long long)next * D);
-        const bool is_q = hh < p.H, is_v = hh >= p.H + p.Hk;
-        float g[8];
-        unpack16x8<T>(graw, g);
-        rotate<IL, true>(g, c, s, from, low);
-        if (norm) {
-          float x[8], ss = 0.f, dot = 0.f;
-          unpack16x8<T>(xraw, x);
+    for (int which = 0; which < 2; ++which) {
+      const int heads = which ? p.Hk : p.H;
+      const long long in = base + (which ? (long long)p.H * D : 0);
+      const uint16_t* up = (which ? p.dk : p.dq) + (long long)row * heads * D + sub * 8;
+      float w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-          const float r = rsqrtf(head_sum<L>(ss) * (1.f / D) + p.eps);
-          const bool add_q = live && is_q, add_k = live && !is_q && !is_v;
+      for (int e = 0; e < 8; ++e) w[e] = norm ? (which ? p.wk : p.wq)[sub * 8 + e] : 1.f;
+      for (int h0 = first; h0 < heads; h0 += 2 * hstep) {
+        uint4 bg[2], bx[2];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] *= r;
-            const float gn = g[e] * x[e];
-            accq[e] += add_q ? gn : 0.f;
-            acck[e] += add_k ? gn : 0.f;
-            g[e] *= is_q ? wq[e] : wk[e];
-            dot = fmaf(g[e], x[e], dot);
+        for (int i = 0; i < 2; ++i) {
+          const int h = h0 + i * hstep + grp;
+          bg[i] = bx[i] = make_uint4(0, 0, 0, 0);
+          if (h < heads) {
+            bg[i] = ld16(up + (long long)h * D);
+            if (norm) bx[i] = ld16(p.qkv + in + (long long)h * D);
           }
-          const float mean = head_sum<L>(dot) * (1.f / D);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[e] = r * fmaf(-x[e], mean, g[e]);
         }
-        if (live) *reinterpret_cast<uint4*>(p.dqkv + base + (long long)hh * D) = is_v ? graw : pack16x8<T>(g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (h0 + i * hstep >= heads) break;
+          const int h = h0 + i * hstep + grp;
+          float g[8], y[8];
+          unpack16x8<T>(bg[i], g);
+          unpack16x8<T>(partners<IL>(bg[i], from, turned), y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] = fmaf(y[e], s[e], g[e] * c[e]);
+          if (norm) {
+            float x[8], ss = 0.f, dot = 0.f;
+            unpack16x8<T>(bx[i], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+            const float r = rsqrtf(head_sum<L>(ss) * (1.f / D) + p.eps);
+            // Heads past the end are zeros and add nothing.
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              x[e] *= r;
+              acc[which][e] = fmaf(g[e], x[e], acc[which][e]);
+              g[e] *= w[e];
+              dot = fmaf(g[e], x[e], dot);
+            }
+            const float mean = head_sum<L>(dot) * (1.f / D);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[e] = r * fmaf(-x[e], mean, g[e]);
+          }
+          if (h < heads) st16(p.dqkv + in + (long long)h * D, pack16x8<T>(g));
+        }
       }
     }
   }
   if (p.partial == nullptr) return;
+  allow_dependents();
   // Gain gradients: heads of the warp, warps of the block, then one row of
   // partials per block for the column sum below -- all in a fixed order.
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int which = 0; which < 2; ++which) {
 #pragma unroll
-    for (int o = L; o < 32; o <<= 1) {
-      accq[e] += __shfl_xor_sync(0xffffffffu, accq[e], o);
-      acck[e] += __shfl_xor_sync(0xffffffffu, acck[e], o);
-    }
-    if (grp == 0) {
-      sums[warp][sub * 8 + e] = accq[e];
-      sums[warp][D + sub * 8 + e] = acck[e];
+    for (int e = 0; e < 8; ++e) {
+      float t = acc[which][e];
+#pragma unroll
+      for (int o = L; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      if (grp == 0) sums[warp][which * D + sub * 8 + e] = t;
     }
   }
   __syncthreads();
@@ -319,22 +318,28 @@ __global__ void __launch_bounds__(32 * WARPS) rotary_bwd_kernel(Params p) {
   }
 }
 
-// dw[col] (+)= sum over `rows` partial rows; 32 columns per block, 32 row
-// lanes, combined in a fixed tree. Columns [0, D) are wq's, [D, 2D) wk's.
+// dw[col] (+)= sum over `rows` partial rows; 8 columns per block (a 32-byte
+// sector of each row), 128 row lanes, combined in a fixed tree. Columns [0, D)
+// are wq's, [D, 2D) wk's.
 __global__ void __launch_bounds__(1024) gain_sum_kernel(const float* __restrict__ partial, int rows, int D,
                                                         float* __restrict__ dwq, float* __restrict__ dwk,
                                                         int accumulate) {
-  __shared__ float part[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  __shared__ float part[8][128];
+  const int x = threadIdx.x & 7, y = threadIdx.x >> 3, col = blockIdx.x * 8 + x;
+  wait_prerequisites();
   float t = 0.f;
-  for (int r = y; r < rows; r += 32) t += partial[(long long)r * 2 * D + col];
-  part[y][lane] = t;
+#pragma unroll 5
+  for (int r = y; r < rows; r += 128) t += partial[(long long)r * 2 * D + col];
+  part[x][y] = t;
   __syncthreads();
-  t = warp_sum(part[lane][y]);  // row lane `lane` of column blockIdx.x * 32 + y
-  if (lane == 0) {
-    const int c = blockIdx.x * 32 + y;
-    float* dst = c < D ? dwq + c : dwk + (c - D);
-    *dst = accumulate ? *dst + t : t;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < 8) {  // warp w sums column blockIdx.x * 8 + w
+    t = warp_sum((part[warp][lane] + part[warp][lane + 32]) + (part[warp][lane + 64] + part[warp][lane + 96]));
+    if (lane == 0) {
+      const int c = blockIdx.x * 8 + warp;
+      float* dst = c < D ? dwq + c : dwk + (c - D);
+      *dst = accumulate ? *dst + t : t;
+    }
   }
 }
 
@@ -365,13 +370,14 @@ int check_common(const void* qkv, const float* wq, const float* wk, const float*
   MFB_CHECK_ARG(dtype == MFB_DTYPE_BF16 || dtype == MFB_DTYPE_F16, "rotary dtype must be bf16 or fp16");
   MFB_CHECK_ARG(qkv && (freqs || rotary_dim == 0), "NULL rotary argument");
   MFB_CHECK_ARG((wq == nullptr) == (wk == nullptr), "q and k gains must both be given or both be NULL");
+  MFB_CHECK_ARG((((uintptr_t)wq | (uintptr_t)wk) & 15) == 0, "gains must be 16-byte aligned");
   return MFB_OK;
 }
 
 template <typename T, int D, bool PAGED>
 int launch_fwd(const Params& p, bool interleaved, int sms, cudaStream_t s) {
   const long long units = (long long)p.M * p.slices;
-  const int grid = (int)std::min<long long>((units + WARPS - 1) / WARPS, 8LL * sms);
+  const int grid = (int)std::min<long long>((units + WARPS - 1) / WARPS, 4LL * sms);
   if (interleaved) rotary_fwd_kernel<T, D, true, PAGED><<<grid, 32 * WARPS, 0, s>>>(p);
   else rotary_fwd_kernel<T, D, false, PAGED><<<grid, 32 * WARPS, 0, s>>>(p);
   MFB_LAUNCH_CHECK(PAGED ? "paged append" : "rotary fwd");
@@ -422,6 +428,7 @@ extern "C" int mfb_qk_rotary_fwd(const void* qkv, int ld_qkv, const float* wq, c
   p.q = (uint16_t*)q;
   p.k = (uint16_t*)k;
   p.v = (uint16_t*)v;
+  p.head_stride = D;
   p.ld = ld_qkv;
   p.M = M;
   p.H = H;
@@ -470,7 +477,7 @@ extern "C" int mfb_qk_rotary_bwd(const void* qkv, int ld_qkv, const float* wq, c
   p.slices = rot::slices_for(M, cdiv(H + 2 * Hk, 256 / D), sms);
   const long long units = (long long)M * p.slices;
   const int grid = (int)std::min<long long>((units + rot::WARPS - 1) / rot::WARPS,
-                                            std::min<long long>(4LL * sms, rot::BWD_GRID_MAX));
+                                            std::min<long long>(3LL * sms, rot::BWD_GRID_MAX));
   cudaStream_t s = (cudaStream_t)stream;
   const bool il = interleaved != 0;
   if (dtype == MFB_DTYPE_BF16) {
@@ -482,8 +489,16 @@ extern "C" int mfb_qk_rotary_bwd(const void* qkv, int ld_qkv, const float* wq, c
   }
   MFB_LAUNCH_CHECK("rotary bwd");
   if (dwq) {
-    rot::gain_sum_kernel<<<2 * D / 32, 1024, 0, s>>>(p.partial, grid, D, dwq, dwk, accumulate);
-    MFB_LAUNCH_CHECK("rotary gain gradients");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2 * D / 8);
+    cfg.blockDim = dim3(1024);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MFB_CUDA_TRY(cudaLaunchKernelEx(&cfg, rot::gain_sum_kernel, (const float*)p.partial, grid, D, dwq, dwk, accumulate));
   }
   return MFB_OK;
 }
