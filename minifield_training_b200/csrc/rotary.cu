@@ -15,16 +15,18 @@
 // 2^20 an FP32 product is off by up to 2^-4 rad, the FP64 one by less than
 // 2^-20 for any int32 position.
 //
-// Layout: a warp owns a token (or one of `slices` interleaved shares of its
-// heads, for calls with few tokens) and D/8 lanes own a head, 8 values (16
-// bytes) each, so every load and store is a full 128-byte line or more. The
-// warp computes each of the token's rotary_dim/2 angles once and passes them
-// through shared memory. With cw = cos * w and sw = -+sin * w_partner per lane,
-//   y = r (x cw + x_partner sw),
-// and the partners are exchanged as the raw 16-bit words: rotary_dim/16 lanes
-// away in the half layout, in the same lane in the interleaved one. The pass is
-// bandwidth-bound; registers are held down so that enough warps have loads in
-// flight (q, k and v heads run in loops of their own, one set of gains live).
+// Layout: a thread keeps its place in the heads -- one head, two chunks of four
+// values that are each other's partners (4s.. and rotary_dim/2 + 4s.. in the
+// half layout; the 8 values from 8s in the interleaved one and in the part
+// that is not rotated) -- and walks a run of tokens, so that gains, addresses
+// and the kind of head are settled once and the rotation needs no exchange
+// between lanes. Every 32-byte sector is still read and written whole. A block
+// takes a few tokens at a time: their heads' loads are under way while the
+// block computes the tokens' rotary_dim/2 angles each into shared memory. The
+// floor is the bytes; what keeps a kernel of this kind above it is the
+// instructions per byte: with a warp per token that loops over the heads, the
+// same arithmetic took three times the instructions and 84 to 111 us where
+// this takes 76 us (16384 tokens of 32 heads, forward and backward).
 #include <algorithm>
 
 #include "types16.cuh"
@@ -32,9 +34,14 @@
 namespace mfb {
 namespace rot {
 
-constexpr int WARPS = 8;
+constexpr int THREADS = 256;
 constexpr int MAX_D = 128;
-constexpr int BWD_GRID_MAX = 3 * 160;  // bounds the gain-gradient partials
+// Tokens of a block's pass, and blocks per SM. Measured together on 16384 tokens
+// forward and backward: 8 tokens / 3 blocks forward with 4 / 3 backward 78.7,
+// 4 / 4 with 2 / 4 75.7, 4 / 5 with 2 / 5 83.3, 2 / 6 with 1 / 5 87.2 us.
+constexpr int FWD_TOKENS = 4, BWD_TOKENS = 2, BLOCKS_PER_SM = 4;
+constexpr int MAX_SMS = 160;
+constexpr int BWD_GRID_MAX = BLOCKS_PER_SM * MAX_SMS;  // blocks of a backward pass: rows of gain-gradient partials
 constexpr double kInvTwoPi = 0.15915494309189533577;
 
 struct Params {
@@ -59,70 +66,112 @@ struct Params {
   const uint16_t* dv;
   uint16_t* dqkv;
   float* partial;  // [grid][2][D]
-  int ld, M, H, Hk, rotary_dim, slices;
+  int ld, M, H, Hk, rotary_dim, heads;  // heads: q, k and (when written) v
   float amplitude, eps;
 };
 
-// The angles of a position into the warp's table: (cos, sin) times amplitude.
-__device__ __forceinline__ void angles(const Params& p, int pos, float2* table, int lane) {
-  __syncwarp();
-  for (int i = lane; i < p.rotary_dim >> 1; i += 32) {
-    const double t = (double)pos * (double)p.freqs[i] * kInvTwoPi;
-    float sn, cs;
-    sincospif(2.f * (float)(t - rint(t)), &sn, &cs);
-    table[i] = make_float2(cs * p.amplitude, sn * p.amplitude);
+// cos and sin (times amplitude) of a block's tokens, position of token t in
+// pos[t]; a warp per token. The turn is reduced in FP64, so the hardware's
+// sine and cosine see at most half a turn, where they are off by 2^-20.5 at most.
+template <int TOKENS>
+struct Angles {
+  float c[TOKENS][MAX_D / 2], s[TOKENS][MAX_D / 2];
+  __device__ __forceinline__ void fill(const Params& p, const int* pos, int tokens) {
+    const int half = p.rotary_dim >> 1;
+    for (int t = threadIdx.x >> 5; t < tokens; t += THREADS / 32) {
+      const double at = (double)pos[t] * kInvTwoPi;
+      for (int k = threadIdx.x & 31; k < half; k += 32) {
+        const double turns = at * (double)p.freqs[k];
+        const float x = 6.283185307f * (float)(turns - rint(turns));
+        c[t][k] = __cosf(x) * p.amplitude;
+        s[t][k] = __sinf(x) * p.amplitude;
+      }
+    }
   }
-  __syncwarp();
-}
+};
 
-// This lane's coefficients: value e becomes x cw + partner sw. Half layout:
-// values sub*8 + e use pair (sub*8 + e) mod (rotary_dim / 2); interleaved:
-// values 2j and 2j + 1 use pair sub*4 + j. INV rotates back (R^T); w (and the
-// partner's wp) multiply the inputs.
-template <bool IL, bool INV>
-__device__ __forceinline__ void coefficients(const Params& p, const float2* table, int sub, bool turned, bool low,
-                                             const float* gains, float* cw, float* sw) {
-  const int half = p.rotary_dim >> 1;
-  float w[8], wp[8];
+// Runs body(t) for t < tokens: unrolled without tests where the pass is full.
+template <int TOKENS, typename Body>
+__device__ __forceinline__ void over_tokens(int tokens, Body body) {
+  if (tokens == TOKENS) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = wp[e] = 1.f;
-  if (gains) {
-    const int mine = sub * 8, other = !turned || IL ? mine : (low ? mine + half : mine - half);
-    const float4 a = reinterpret_cast<const float4*>(gains + mine)[0], b = reinterpret_cast<const float4*>(gains + mine)[1];
-    const float4 c = reinterpret_cast<const float4*>(gains + other)[0], d = reinterpret_cast<const float4*>(gains + other)[1];
-    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-    wp[0] = c.x, wp[1] = c.y, wp[2] = c.z, wp[3] = c.w, wp[4] = d.x, wp[5] = d.y, wp[6] = d.z, wp[7] = d.w;
-  }
+    for (int t = 0; t < TOKENS; ++t) body(t);
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float2 f = make_float2(1.f, 0.f);
-    if (turned) f = table[IL ? sub * 4 + e / 2 : (low ? sub * 8 + e : sub * 8 + e - half)];
-    const bool minus = (IL ? (e & 1) == 0 : low) != INV;  // y_first = x_first c - x_second s
-    cw[e] = f.x * w[e];
-    sw[e] = (minus ? -f.y : f.y) * (IL ? wp[e ^ 1] : wp[e]);
+    for (int t = 0; t < TOKENS; ++t)
+      if (t < tokens) body(t);
   }
 }
 
-// The partners' raw words (zeros where nothing is rotated).
-template <bool IL>
-__device__ __forceinline__ uint4 partners(const uint4& v, int from, bool turned) {
-  if (IL) {
-    return make_uint4(__byte_perm(v.x, 0, 0x1032), __byte_perm(v.y, 0, 0x1032), __byte_perm(v.z, 0, 0x1032),
-                      __byte_perm(v.w, 0, 0x1032));
+// A thread's place: head `head` of the row (kind 0 q, 1 k, 2 v; head `in_kind`
+// of its kind), values oa.. and ob... Threads past the last head take the last
+// head's place (shuffles need them) and store nothing.
+template <int D, bool IL>
+struct Place {
+  static constexpr int L = D / 8;  // lanes per head
+  int head, kind, in_kind, sub, oa, ob;
+  bool live, turned, copies;  // copies: all of this warp's heads are v's
+  __device__ __forceinline__ explicit Place(const Params& p) {
+    const int h = blockIdx.y * (THREADS / L) + threadIdx.x / L;
+    sub = threadIdx.x % L;
+    live = h < p.heads;
+    head = min(h, p.heads - 1);
+    kind = head < p.H ? 0 : head < p.H + p.Hk ? 1 : 2;
+    in_kind = head - (kind == 0 ? 0 : kind == 1 ? p.H : p.H + p.Hk);
+    turned = sub * 8 < p.rotary_dim;
+    copies = __all_sync(0xffffffffu, kind == 2);
+    oa = turned && !IL ? sub * 4 : sub * 8;
+    ob = turned && !IL ? sub * 4 + (p.rotary_dim >> 1) : sub * 8 + 4;
   }
-  uint4 o;
-  o.x = __shfl_sync(0xffffffffu, v.x, from);
-  o.y = __shfl_sync(0xffffffffu, v.y, from);
-  o.z = __shfl_sync(0xffffffffu, v.z, from);
-  o.w = __shfl_sync(0xffffffffu, v.w, from);
-  return turned ? o : make_uint4(0, 0, 0, 0);
-}
+  __device__ __forceinline__ void gains(const Params& p, uint64_t* w) const {
+    const float* g = kind == 0 ? p.wq : kind == 1 ? p.wk : nullptr;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 a = g ? reinterpret_cast<const float2*>(g + oa)[i] : make_float2(1.f, 1.f);
+      const float2 b = g ? reinterpret_cast<const float2*>(g + ob)[i] : make_float2(1.f, 1.f);
+      w[i] = pair(a.x, a.y);
+      w[2 + i] = pair(b.x, b.y);
+    }
+  }
+  // Rotates x (chunk a in x[0..1], b in x[2..3]) by one token's angles; INV back.
+  template <bool INV>
+  __device__ __forceinline__ void rotate(const float* cs, const float* sn, uint64_t* x) const {
+    if (!turned) return;
+    const float4 c = *reinterpret_cast<const float4*>(cs + sub * 4), s = *reinterpret_cast<const float4*>(sn + sub * 4);
+    if (IL) {
+      const float ca[4] = {c.x, c.y, c.z, c.w}, sa[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpair(x[i]);
+        const float sg = INV ? -sa[i] : sa[i];
+        x[i] = pair(f.x * ca[i] - f.y * sg, f.y * ca[i] + f.x * sg);
+      }
+    } else {
+      const uint64_t ca[2] = {pair(c.x, c.y), pair(c.z, c.w)}, sa[2] = {pair(s.x, s.y), pair(s.z, s.w)};
+      const uint64_t na[2] = {pair(-s.x, -s.y), pair(-s.z, -s.w)};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint64_t a = x[i], b = x[2 + i];
+        x[i] = fma2(b, INV ? sa[i] : na[i], mul2(a, ca[i]));
+        x[2 + i] = fma2(a, INV ? na[i] : sa[i], mul2(b, ca[i]));
+      }
+    }
+  }
+};
 
 template <int L>
 __device__ __forceinline__ float head_sum(float v) {
 #pragma unroll
   for (int o = 1; o < L; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+template <int D>
+__device__ __forceinline__ float head_rnorm(const uint64_t* x, float eps) {
+  uint64_t ss = mul2(x[0], x[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) ss = fma2(x[i], x[i], ss);
+  const float2 f = unpair(ss);
+  return rsqrtf(head_sum<D / 8>(f.x + f.y) * (1.f / D) + eps);
 }
 
 // Sequence of token t: the last b with cu_q[b] <= t.
@@ -136,185 +185,184 @@ __device__ __forceinline__ int sequence_of(const int* cu_q, int B, int t) {
   return lo;
 }
 
-__device__ __forceinline__ uint4 ld16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
-__device__ __forceinline__ void st16(uint16_t* p, const uint4& v) { *reinterpret_cast<uint4*>(p) = v; }
+__device__ __forceinline__ uint2 ld8(const uint16_t* p) { return *reinterpret_cast<const uint2*>(p); }
+__device__ __forceinline__ void st8(uint16_t* p, const uint2& v) { *reinterpret_cast<uint2*>(p) = v; }
 
-// Runs body(i, h, live) over this warp's heads [0, n) in steps of `step`, four
-// steps' loads ahead of their use: load(h) -> uint4. All lanes take part in
-// every step (shuffles); heads past the end are not live.
-template <int AHEAD, typename Load, typename Body>
-__device__ __forceinline__ void over_heads(int first, int grp, int step, int n, Load load, Body body) {
-  for (int h0 = first; h0 < n; h0 += AHEAD * step) {
-    uint4 v[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int h = h0 + i * step + grp;
-      v[i] = h < n ? load(h) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      if (h0 + i * step < n) body(h0 + i * step + grp, h0 + i * step + grp < n, v[i]);
-  }
-}
+// A block's run of tokens.
+__device__ __forceinline__ int run_begin(const Params& p, int i) { return (int)((long long)p.M * i / gridDim.x); }
 
 template <typename T, int D, bool IL, bool PAGED>
-__global__ void __launch_bounds__(32 * WARPS, 4) rotary_fwd_kernel(Params p) {
-  constexpr int L = D / 8, HPW = 32 / L;  // lanes per head, heads per warp
-  __shared__ float2 tables[WARPS][MAX_D / 2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L, grp = lane / L;
-  const int half8 = p.rotary_dim >> 4;  // lanes of half a rotated part
-  const bool turned = sub * 8 < p.rotary_dim, low = sub < half8;
-  const int from = turned ? (low ? lane + half8 : lane - half8) : lane;
-  const bool norm = p.wq != nullptr;
-  const long long units = (long long)p.M * p.slices, step = (long long)gridDim.x * WARPS;
-  for (long long u = (long long)blockIdx.x * WARPS + warp; u < units; u += step) {
-    const int row = (int)(u / p.slices), first = (int)(u % p.slices) * HPW, hstep = p.slices * HPW;
-    const uint16_t* src = p.qkv + (long long)row * p.ld + sub * 8;
-    int pos;
-    long long slot = -1;  // element offset of the token's first head in the pages; -1: not stored
-    if (PAGED) {
-      if (row < p.cu_q[0] || row >= p.cu_q[p.B]) continue;  // padding: left as it was
-      const int b = sequence_of(p.cu_q, p.B, row);
-      pos = p.seq_lens[b] - (p.cu_q[b + 1] - row);
-      const int pg = pos >> p.page_shift;
-      if (pos >= 0 && pg < p.max_pages) {
-        const int id = p.page_table[(long long)b * p.max_pages + pg];
-        if ((unsigned)id < (unsigned)p.num_pages)
-          slot = (long long)id * p.page_stride + (long long)(pos - (pg << p.page_shift)) * p.token_stride;
+__global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_fwd_kernel(Params p) {
+  __shared__ __align__(16) Angles<FWD_TOKENS> angles;
+  __shared__ int s_pos[FWD_TOKENS];
+  __shared__ long long s_place[FWD_TOKENS];  // element offset of a token's first head in k and v; -1: not stored
+  const Place<D, IL> w(p);
+  uint64_t gain[4];
+  w.gains(p, gain);
+  const uint16_t* in = p.qkv + w.head * D;
+  uint16_t* out = w.kind == 0 ? p.q + w.in_kind * D : (w.kind == 1 ? p.k : p.v) + (long long)w.in_kind * p.head_stride;
+  const int begin = run_begin(p, blockIdx.x), end = run_begin(p, blockIdx.x + 1);
+  for (int row0 = begin; row0 < end; row0 += FWD_TOKENS) {
+    const int tokens = min(FWD_TOKENS, end - row0);
+    uint2 va[FWD_TOKENS], vb[FWD_TOKENS];
+    const uint16_t* src = in + (long long)row0 * p.ld;
+    over_tokens<FWD_TOKENS>(tokens, [&](int t) {
+      va[t] = ld8(src + w.oa);
+      vb[t] = ld8(src + w.ob);
+      src += p.ld;
+    });
+    __syncthreads();  // the last pass is done with the shared tables
+    if (threadIdx.x < tokens) {
+      const int row = row0 + threadIdx.x;
+      int pos = 0;
+      long long place = -1;
+      if (PAGED) {
+        if (row < p.cu_q[0] || row >= p.cu_q[p.B]) {
+          place = -2;  // padding: nothing is stored
+        } else {
+          const int b = sequence_of(p.cu_q, p.B, row);
+          pos = p.seq_lens[b] - (p.cu_q[b + 1] - row);
+          const int pg = pos >> p.page_shift;
+          if (pos >= 0 && pg < p.max_pages) {
+            const int id = p.page_table[(long long)b * p.max_pages + pg];
+            if ((unsigned)id < (unsigned)p.num_pages)
+              place = (long long)id * p.page_stride + (long long)(pos - (pg << p.page_shift)) * p.token_stride;
+          }
+        }
+      } else {
+        pos = p.positions[row];
+        place = (long long)row * p.Hk * D;
       }
-    } else {
-      pos = p.positions[row];
-      slot = (long long)row * p.Hk * D;
+      s_pos[threadIdx.x] = pos;
+      s_place[threadIdx.x] = place;
     }
-    // Values: copied. Their loads are under way while the angles are computed.
-    if (p.v && slot >= 0)
-      over_heads<4>(first, grp, hstep, p.Hk, [&](int h) { return ld16(src + (long long)(p.H + p.Hk + h) * D); },
-                    [&](int h, bool live, const uint4& v) {
-                      if (live) st16(p.v + slot + (long long)h * p.head_stride + sub * 8, v);
-                    });
-    angles(p, pos, tables[warp], lane);
-#pragma unroll 1
-    for (int which = 0; which < 2; ++which) {
-      float cw[8], sw[8];
-      coefficients<IL, false>(p, tables[warp], sub, turned, low, which ? p.wk : p.wq, cw, sw);
-      const uint16_t* in = src + (which ? (long long)p.H * D : 0);
-      uint16_t* out = which ? p.k + slot : p.q + (long long)row * p.H * D;
-      const long long hs = which ? p.head_stride : D;
-      const bool stored = !which || slot >= 0;
-      over_heads<4>(first, grp, hstep, which ? p.Hk : p.H, [&](int h) { return ld16(in + (long long)h * D); },
-                    [&](int h, bool live, const uint4& v) {
-                      float x[8], y[8], r = 1.f;
-                      unpack16x8<T>(v, x);
-                      unpack16x8<T>(partners<IL>(v, from, turned), y);
-                      if (norm) {
-                        float ss = 0.f;
+    __syncthreads();
+    angles.fill(p, s_pos, tokens);
+    __syncthreads();
+    long long q_to = (long long)row0 * p.H * D;
+    over_tokens<FWD_TOKENS>(tokens, [&](int t) {
+      uint2 a = va[t], b = vb[t];
+      if (!w.copies) {
+        uint64_t x[4];
+        unpack16x4<T>(a, x);
+        unpack16x4<T>(b, x + 2);
+        if (p.wq) {
+          const float r = head_rnorm<D>(x, p.eps);
+          const uint64_t r2 = pair(r, r);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-                        r = rsqrtf(head_sum<L>(ss) * (1.f / D) + p.eps);
-                      }
-#pragma unroll
-                      for (int e = 0; e < 8; ++e) x[e] = fmaf(y[e], sw[e], x[e] * cw[e]) * r;
-                      if (live && stored) st16(out + h * hs + sub * 8, pack16x8<T>(x));
-                    });
-    }
+          for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], mul2(r2, gain[i]));
+        }
+        w.template rotate<false>(angles.c[t], angles.s[t], x);
+        if (w.kind < 2) {
+          a = pack16x4<T>(x);
+          b = pack16x4<T>(x + 2);
+        }
+      }
+      long long to = s_place[t];
+      const bool stored = w.live && to >= (w.kind ? 0 : -1);
+      if (w.kind == 0) to = q_to;
+      q_to += p.H * D;
+      if (stored) {
+        st8(out + to + w.oa, a);
+        st8(out + to + w.ob, b);
+      }
+    });
   }
 }
 
 template <typename T, int D, bool IL>
-__global__ void __launch_bounds__(32 * WARPS, 3) rotary_bwd_kernel(Params p) {
-  constexpr int L = D / 8, HPW = 32 / L;
-  __shared__ float2 tables[WARPS][MAX_D / 2];
-  __shared__ float sums[WARPS][2 * D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L, grp = lane / L;
-  const int half8 = p.rotary_dim >> 4;
-  const bool turned = sub * 8 < p.rotary_dim, low = sub < half8;
-  const int from = turned ? (low ? lane + half8 : lane - half8) : lane;
-  const bool norm = p.wq != nullptr;
-  float acc[2][8];
+__global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_bwd_kernel(Params p) {
+  using W = Place<D, IL>;
+  __shared__ __align__(16) Angles<BWD_TOKENS> angles;
+  __shared__ int s_pos[BWD_TOKENS];
+  __shared__ float sums[THREADS / W::L][D];
+  const W w(p);
+  uint64_t gain[4], acc[4];
+  w.gains(p, gain);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[0][e] = acc[1][e] = 0.f;
-  const long long units = (long long)p.M * p.slices, step = (long long)gridDim.x * WARPS;
-  for (long long u = (long long)blockIdx.x * WARPS + warp; u < units; u += step) {
-    const int row = (int)(u / p.slices), first = (int)(u % p.slices) * HPW, hstep = p.slices * HPW;
-    const long long base = (long long)row * p.ld + sub * 8;
-    over_heads<4>(first, grp, hstep, p.Hk, [&](int h) { return ld16(p.dv + ((long long)row * p.Hk + h) * D + sub * 8); },
-                  [&](int h, bool live, const uint4& v) {
-                    if (live) st16(p.dqkv + base + (long long)(p.H + p.Hk + h) * D, v);
-                  });
-    angles(p, p.positions[row], tables[warp], lane);
-    float c[8], s[8];
-    coefficients<IL, true>(p, tables[warp], sub, turned, low, nullptr, c, s);
+  for (int i = 0; i < 4; ++i) acc[i] = pair(0.f, 0.f);
+  const int kind_heads = w.kind ? p.Hk : p.H;
+  const uint16_t* up = (w.kind == 0 ? p.dq : w.kind == 1 ? p.dk : p.dv) + w.in_kind * D;
+  const long long up_row = (long long)kind_heads * D;
+  const int begin = run_begin(p, blockIdx.x), end = run_begin(p, blockIdx.x + 1);
+  for (int row0 = begin; row0 < end; row0 += BWD_TOKENS) {
+    const int tokens = min(BWD_TOKENS, end - row0);
+    uint2 ga[BWD_TOKENS], gb[BWD_TOKENS], xa[BWD_TOKENS], xb[BWD_TOKENS];
+    const uint16_t* src = up + row0 * up_row;
+    const uint16_t* row = p.qkv + (long long)row0 * p.ld + w.head * D;
+    over_tokens<BWD_TOKENS>(tokens, [&](int t) {
+      ga[t] = ld8(src + w.oa);
+      gb[t] = ld8(src + w.ob);
+      src += up_row;
+      if (p.wq && !w.copies) {
+        xa[t] = ld8(row + w.oa);
+        xb[t] = ld8(row + w.ob);
+      }
+      row += p.ld;
+    });
+    __syncthreads();
+    if (threadIdx.x < tokens) s_pos[threadIdx.x] = p.positions[row0 + threadIdx.x];
+    __syncthreads();
+    angles.fill(p, s_pos, tokens);
+    __syncthreads();
+    uint16_t* out = p.dqkv + (long long)row0 * p.ld + w.head * D;
+    over_tokens<BWD_TOKENS>(tokens, [&](int t) {
+      uint2 a = ga[t], b = gb[t];
+      if (!w.copies) {
+        uint64_t g[4];
+        unpack16x4<T>(a, g);
+        unpack16x4<T>(b, g + 2);
+        w.template rotate<true>(angles.c[t], angles.s[t], g);
+        if (p.wq) {
+          uint64_t x[4], dot = pair(0.f, 0.f);
+          unpack16x4<T>(xa[t], x);
+          unpack16x4<T>(xb[t], x + 2);
+          const float r = head_rnorm<D>(x, p.eps);
+          const uint64_t r2 = pair(r, r);
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const int heads = which ? p.Hk : p.H;
-      const long long in = base + (which ? (long long)p.H * D : 0);
-      const uint16_t* up = (which ? p.dk : p.dq) + (long long)row * heads * D + sub * 8;
-      float w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = norm ? (which ? p.wk : p.wq)[sub * 8 + e] : 1.f;
-      for (int h0 = first; h0 < heads; h0 += 2 * hstep) {
-        uint4 bg[2], bx[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int h = h0 + i * hstep + grp;
-          bg[i] = bx[i] = make_uint4(0, 0, 0, 0);
-          if (h < heads) {
-            bg[i] = ld16(up + (long long)h * D);
-            if (norm) bx[i] = ld16(p.qkv + in + (long long)h * D);
+          for (int i = 0; i < 4; ++i) {
+            x[i] = mul2(x[i], r2);
+            acc[i] = fma2(g[i], x[i], acc[i]);
+            g[i] = mul2(g[i], gain[i]);
+            dot = fma2(g[i], x[i], dot);
           }
+          const float2 d2 = unpair(dot);
+          const float mean = head_sum<W::L>(d2.x + d2.y) * (-1.f / D);
+          const uint64_t m2 = pair(mean, mean);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) g[i] = mul2(r2, fma2(x[i], m2, g[i]));
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (h0 + i * hstep >= heads) break;
-          const int h = h0 + i * hstep + grp;
-          float g[8], y[8];
-          unpack16x8<T>(bg[i], g);
-          unpack16x8<T>(partners<IL>(bg[i], from, turned), y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[e] = fmaf(y[e], s[e], g[e] * c[e]);
-          if (norm) {
-            float x[8], ss = 0.f, dot = 0.f;
-            unpack16x8<T>(bx[i], x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-            const float r = rsqrtf(head_sum<L>(ss) * (1.f / D) + p.eps);
-            // Heads past the end are zeros and add nothing.
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              x[e] *= r;
-              acc[which][e] = fmaf(g[e], x[e], acc[which][e]);
-              g[e] *= w[e];
-              dot = fmaf(g[e], x[e], dot);
-            }
-            const float mean = head_sum<L>(dot) * (1.f / D);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] = r * fmaf(-x[e], mean, g[e]);
-          }
-          if (h < heads) st16(p.dqkv + in + (long long)h * D, pack16x8<T>(g));
+        if (w.kind < 2) {
+          a = pack16x4<T>(g);
+          b = pack16x4<T>(g + 2);
         }
       }
-    }
+      if (w.live) {
+        st8(out + w.oa, a);
+        st8(out + w.ob, b);
+      }
+      out += p.ld;
+    });
   }
   if (p.partial == nullptr) return;
   allow_dependents();
-  // Gain gradients: heads of the warp, warps of the block, then one row of
-  // partials per block for the column sum below -- all in a fixed order.
+  // Gain gradients: the block's q heads and its k heads, each in head order,
+  // then one row of partials per block for the column sum below.
+  float* mine = sums[threadIdx.x / W::L];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float t = acc[which][e];
-#pragma unroll
-      for (int o = L; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if (grp == 0) sums[warp][which * D + sub * 8 + e] = t;
-    }
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpair(acc[i]);
+    float* at = mine + (i < 2 ? w.oa + 2 * i : w.ob + 2 * (i - 2));
+    at[0] = w.live ? f.x : 0.f;
+    at[1] = w.live ? f.y : 0.f;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * D; i += 32 * WARPS) {
+  const int h0 = blockIdx.y * (THREADS / W::L);
+  for (int i = threadIdx.x; i < 2 * D; i += THREADS) {
+    const int lo = i < D ? 0 : p.H, hi = i < D ? p.H : p.H + p.Hk;
     float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) t += sums[w][i];
-    p.partial[(long long)blockIdx.x * 2 * D + i] = t;
+    for (int k = max(lo - h0, 0); k < min(hi - h0, THREADS / W::L); ++k) t += sums[k][i % D];
+    p.partial[(long long)(blockIdx.y * gridDim.x + blockIdx.x) * 2 * D + i] = t;
   }
 }
 
@@ -347,22 +395,21 @@ int sm_count() {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
+  return std::min(sms, MAX_SMS);
 }
 
-// Shares of a token's heads: more than one where whole tokens would leave the
-// GPU short of warps (each share computes the token's angles again).
-int slices_for(int M, int groups, int sms) {
-  int s = 1;
-  while (s < 8 && s * 2 <= groups && (long long)M * s * 2 <= (long long)sms * 16) s *= 2;
-  return s;
+// Blocks: `chunks` in y cover a row's heads, x cuts the tokens into runs, as
+// many as are resident, one token each at least.
+dim3 grid_for(const Params& p, int D, int sms) {
+  const int chunks = cdiv(p.heads, THREADS / (D / 8));
+  return dim3((unsigned)std::max(1, std::min(p.M, BLOCKS_PER_SM * sms / chunks)), (unsigned)chunks);
 }
 
 int check_common(const void* qkv, const float* wq, const float* wk, const float* freqs, int ld, int M, int H, int Hk,
                  int D, int rotary_dim, int dtype) {
   MFB_CHECK_ARG(M > 0 && H > 0 && Hk > 0, "rotary needs tokens and heads (M=%d H=%d Hk=%d)", M, H, Hk);
   MFB_CHECK_ARG(D == 64 || D == 128, "rotary head_dim %d unsupported (64 or 128)", D);
-  MFB_CHECK_ARG((long long)(H + 2LL * Hk) * D <= 1 << 24, "too many heads (H=%d Hk=%d)", H, Hk);
+  MFB_CHECK_ARG(H + 2LL * Hk <= 1024, "rotary supports up to 1024 heads in a row (H=%d Hk=%d)", H, Hk);
   MFB_CHECK_ARG(ld >= (H + 2 * Hk) * D && ld % 8 == 0, "qkv rows need a stride of at least %d, a multiple of 8 (ld=%d)",
                 (H + 2 * Hk) * D, ld);
   MFB_CHECK_ARG(rotary_dim >= 0 && rotary_dim <= D && rotary_dim % 16 == 0,
@@ -376,10 +423,9 @@ int check_common(const void* qkv, const float* wq, const float* wk, const float*
 
 template <typename T, int D, bool PAGED>
 int launch_fwd(const Params& p, bool interleaved, int sms, cudaStream_t s) {
-  const long long units = (long long)p.M * p.slices;
-  const int grid = (int)std::min<long long>((units + WARPS - 1) / WARPS, 4LL * sms);
-  if (interleaved) rotary_fwd_kernel<T, D, true, PAGED><<<grid, 32 * WARPS, 0, s>>>(p);
-  else rotary_fwd_kernel<T, D, false, PAGED><<<grid, 32 * WARPS, 0, s>>>(p);
+  const dim3 grid = grid_for(p, D, sms);
+  if (interleaved) rotary_fwd_kernel<T, D, true, PAGED><<<grid, THREADS, 0, s>>>(p);
+  else rotary_fwd_kernel<T, D, false, PAGED><<<grid, THREADS, 0, s>>>(p);
   MFB_LAUNCH_CHECK(PAGED ? "paged append" : "rotary fwd");
   return MFB_OK;
 }
@@ -394,9 +440,9 @@ int dispatch_fwd(const Params& p, int D, bool interleaved, int dtype, int sms, c
 }
 
 template <typename T, int D>
-void launch_bwd(const Params& p, bool interleaved, int grid, cudaStream_t s) {
-  if (interleaved) rotary_bwd_kernel<T, D, true><<<grid, 32 * WARPS, 0, s>>>(p);
-  else rotary_bwd_kernel<T, D, false><<<grid, 32 * WARPS, 0, s>>>(p);
+void launch_bwd(const Params& p, bool interleaved, dim3 grid, cudaStream_t s) {
+  if (interleaved) rotary_bwd_kernel<T, D, true><<<grid, THREADS, 0, s>>>(p);
+  else rotary_bwd_kernel<T, D, false><<<grid, THREADS, 0, s>>>(p);
 }
 
 bool aligned16(std::initializer_list<const void*> ptrs) {
@@ -433,10 +479,11 @@ extern "C" int mfb_qk_rotary_fwd(const void* qkv, int ld_qkv, const float* wq, c
   p.M = M;
   p.H = H;
   p.Hk = Hk;
+  p.heads = H + 2 * Hk;
   p.rotary_dim = rotary_dim;
   p.amplitude = amplitude;
   p.eps = eps;
-  p.slices = rot::slices_for(M, cdiv(H + 2 * Hk, 256 / D), sms);
+  if (!v) p.heads = H + Hk;
   return rot::dispatch_fwd<false>(p, D, interleaved != 0, dtype, sms, (cudaStream_t)stream);
 }
 
@@ -471,13 +518,11 @@ extern "C" int mfb_qk_rotary_bwd(const void* qkv, int ld_qkv, const float* wq, c
   p.M = M;
   p.H = H;
   p.Hk = Hk;
+  p.heads = H + 2 * Hk;
   p.rotary_dim = rotary_dim;
   p.amplitude = amplitude;
   p.eps = eps;
-  p.slices = rot::slices_for(M, cdiv(H + 2 * Hk, 256 / D), sms);
-  const long long units = (long long)M * p.slices;
-  const int grid = (int)std::min<long long>((units + rot::WARPS - 1) / rot::WARPS,
-                                            std::min<long long>(3LL * sms, rot::BWD_GRID_MAX));
+  const dim3 grid = rot::grid_for(p, D, sms);
   cudaStream_t s = (cudaStream_t)stream;
   const bool il = interleaved != 0;
   if (dtype == MFB_DTYPE_BF16) {
@@ -498,7 +543,7 @@ extern "C" int mfb_qk_rotary_bwd(const void* qkv, int ld_qkv, const float* wq, c
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    MFB_CUDA_TRY(cudaLaunchKernelEx(&cfg, rot::gain_sum_kernel, (const float*)p.partial, grid, D, dwq, dwk, accumulate));
+    MFB_CUDA_TRY(cudaLaunchKernelEx(&cfg, rot::gain_sum_kernel, (const float*)p.partial, (int)(grid.x * grid.y), D, dwq, dwk, accumulate));
   }
   return MFB_OK;
 }
@@ -540,9 +585,9 @@ extern "C" int mfb_paged_append(const void* qkv, int ld_qkv, const float* wq, co
   p.M = N;
   p.H = H;
   p.Hk = Hk;
+  p.heads = H + 2 * Hk;
   p.rotary_dim = rotary_dim;
   p.amplitude = amplitude;
   p.eps = eps;
-  p.slices = rot::slices_for(N, cdiv(H + 2 * Hk, 256 / D), sms);
   return rot::dispatch_fwd<true>(p, D, interleaved != 0, dtype, sms, (cudaStream_t)stream);
 }

@@ -55,4 +55,44 @@ __device__ __forceinline__ uint4 pack16x8(const float* x) {
                     Num16<T>::pack2(x[6], x[7]));
 }
 
+// Two FP32 lanes per instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Four 16-bit values as two FP32 pairs, and back.
+template <typename T>
+__device__ __forceinline__ void unpack16x4(const uint2& v, uint64_t* x) {
+  const float2 a = Num16<T>::unpack2(v.x), b = Num16<T>::unpack2(v.y);
+  x[0] = pair(a.x, a.y);
+  x[1] = pair(b.x, b.y);
+}
+template <typename T>
+__device__ __forceinline__ uint2 pack16x4(const uint64_t* x) {
+  const float2 a = unpair(x[0]), b = unpair(x[1]);
+  return make_uint2(Num16<T>::pack2(a.x, a.y), Num16<T>::pack2(b.x, b.y));
+}
+
 }  // namespace mfb
