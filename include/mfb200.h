@@ -466,7 +466,7 @@ int mfb_paged_attn_status(int* code);
  *   x = -inf where bit t % 32 of mask word t / 32 is 0
  * mask [mask_count, ceil(V/32)]: row mask_rows[b], or b when mask_rows is NULL;
  * an index outside [0, mask_count) leaves the row unmasked. history_capacity <
- * 2^20, bias_count <= 2047, V <= 393216. */
+ * 2^20, bias_count <= 2047, V <= 2^24. */
 int mfb_logits_process(const void* logits, int dtype, const int32_t* history, int history_capacity,
                        const int32_t* prompt_len, const int32_t* history_len, const float* repetition,
                        const float* frequency, const float* presence, const int32_t* bias_ids,

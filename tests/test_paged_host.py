@@ -191,7 +191,7 @@ def test_empty_calls_launch_nothing():
     (dict(mask_rows=fake((2,), "int32")), "needs a mask"),
     (dict(logits=fake((2, 100), "int32")), "logits must be"),
     (dict(logits=fake((2, 100), "bfloat16", ptr=(1 << 20) + 2)), "16-byte aligned"),
-    (dict(logits=fake((1, 393217), "bfloat16"), out=fake((1, 393217), "float32")), "vocabulary"),
+    (dict(logits=fake((1, (1 << 24) + 1), "bfloat16"), out=fake((1, (1 << 24) + 1), "float32")), "vocabulary"),
 ])
 def test_logits_refuse(kw, match):
     a = dict(logits=fake((2, 100), "bfloat16"), out=fake((2, 100), "float32"))
