@@ -12,13 +12,16 @@
 // Floor: every live K/V row is read from HBM once per KV head; 4 D operations
 // per (query head, key) pair on the tensor cores and one exponential.
 //
-// Both kernels are persistent: a small schedule kernel lists the work items --
-// (sequence, KV heads, query rows) with their number of key tiles -- and cuts
-// the tiles of all items, in order, into equal contiguous shares, one per CTA.
+// Both kernels are persistent: the work items -- (sequence, KV heads, query
+// rows) with their number of key tiles -- are listed, and the tiles of all
+// items, in order, cut into equal contiguous shares, one per CTA: by every CTA
+// for itself where a sequence is one item per head group (few query rows), by
+// a small schedule kernel otherwise.
 // A long context with few queries is thereby spread over the whole GPU and a
 // ragged batch stays balanced without the host knowing any length. Items cut
-// between CTAs leave FP32 partials (max, sum, output) in the workspace; the
-// last CTA to finish one (ticket, no waiting) joins them in CTA order.
+// between CTAs leave FP32 partials (max, sum, output) in the workspace, which a
+// third kernel joins in CTA order with the whole GPU. (Joined by the last CTA
+// of an item, they took up to 24 us: 590 KB through one SM.)
 #include <math.h>
 
 #include <algorithm>
@@ -64,8 +67,6 @@ struct Params {
   Header* head;
   Item* items;
   Item* starts;    // [grid] each share's first item
-  int* tickets;    // [items]
-  int* tickets_g;  // [2 * grid] first-level tickets of items cut into many parts
   float* part_o;   // [slots][part_rows] x D
   float2* part_ml; // [slots][part_rows]
   int N, B, H, Hk, G, max_q, max_pages, num_pages, page_shift;
@@ -120,6 +121,14 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* sum) {
   return incl - v + (warp ? warp_sums[warp - 1] : 0);
 }
 
+__device__ __forceinline__ Header cut(const Params& p, int total) {
+  Header h;
+  h.total = total;
+  h.shares = max(1, min(p.grid, total / p.min_share));
+  h.base = total / h.shares;
+  h.rest = total - h.base * h.shares;
+  return h;
+}
 __device__ __forceinline__ int share_begin(const Header& h, int i) { return i * h.base + min(i, h.rest); }
 __device__ __forceinline__ int share_of(const Header& h, int x) {
   const int split = h.rest * (h.base + 1);
@@ -146,56 +155,43 @@ __device__ __forceinline__ void sequence(const Params& p, int b, int* q0, int* n
   if (c0 != lo || c1 != hi || *nq != hi - lo || *len != s) atomicCAS(&g_status, 0, kBadLength);
 }
 
-// FEW: one item per sequence and head group (its new tokens fit one item);
-// otherwise a sequence has cdiv(new tokens, tok_item) blocks per head.
-template <bool FEW>
+// Sequence b has cdiv(new tokens, tok_item) items per head.
 __global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
   allow_dependents();
-  extern __shared__ int item_base[];  // [B + 1] items before each sequence (not FEW)
+  extern __shared__ int item_base[];  // [B] items before each sequence
   __shared__ int warp_sums[32];
-  const int tid = threadIdx.x, groups = p.Hk / p.hc;
-  for (int i = tid; i < 2 * p.grid; i += SCHED_THREADS) p.tickets_g[i] = 0;
-  int items = p.B * groups;
-  if (!FEW) {
-    int carry = 0;
-    for (int b0 = 0; b0 < p.B; b0 += SCHED_THREADS) {
-      const int b = b0 + tid;
-      int q0, nq = 0, base, len, sum;
-      if (b < p.B) sequence(p, b, &q0, &nq, &base, &len);
-      const int pre = block_scan(cdiv(nq, p.tok_item) * groups, warp_sums, &sum);
-      if (b < p.B) item_base[b] = carry + pre;
-      carry += sum;
-    }
-    items = min(carry, p.max_items);
-    __syncthreads();
+  const int tid = threadIdx.x;
+  int carry = 0;
+  for (int b0 = 0; b0 < p.B; b0 += SCHED_THREADS) {
+    const int b = b0 + tid;
+    int q0, nq = 0, base, len, sum;
+    if (b < p.B) sequence(p, b, &q0, &nq, &base, &len);
+    const int pre = block_scan(cdiv(nq, p.tok_item) * p.Hk, warp_sums, &sum);
+    if (b < p.B) item_base[b] = carry + pre;
+    carry += sum;
   }
+  const int items = min(carry, p.max_items);
+  __syncthreads();
   auto make = [&](int i) {
     Item it;
-    int t0 = 0, q0, nq, base, len;
-    if (FEW) {
-      it.b = i / groups;
-      it.hg = i - it.b * groups;
-      sequence(p, it.b, &q0, &nq, &base, &len);
-    } else {
-      int lo = 0, hi = p.B - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (item_base[mid] <= i) lo = mid;
-        else hi = mid - 1;
-      }
-      it.b = lo;
-      sequence(p, lo, &q0, &nq, &base, &len);
-      const int blocks = cdiv(nq, p.tok_item), local = i - item_base[lo];
-      it.hg = local / blocks;
-      t0 = (local - it.hg * blocks) * p.tok_item;
+    int q0, nq, base, len, lo = 0, hi = p.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (item_base[mid] <= i) lo = mid;
+      else hi = mid - 1;
     }
+    it.b = lo;
+    sequence(p, lo, &q0, &nq, &base, &len);
+    const int blocks = cdiv(nq, p.tok_item), local = i - item_base[lo];
+    it.hg = local / blocks;
+    const int t0 = (local - it.hg * blocks) * p.tok_item;
     it.tok0 = q0 + t0;
     it.ntok = min(p.tok_item, nq - t0);
     it.pos0 = base + t0;
     it.keys = min(max(it.pos0 + it.ntok, 0), len);
     it.tiles = it.ntok > 0 ? max(1, cdiv(it.keys, p.unit)) : 0;
     // Two query tiles share a unit's keys but need twice the softmax.
-    it.shift = !FEW && it.ntok * p.G > 128 ? 1 : 0;
+    it.shift = it.ntok * p.G > 128 ? 1 : 0;
     it.index = i;
     it.first = it.pad[0] = it.pad[1] = 0;
     return it;
@@ -210,13 +206,9 @@ __global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
     pre = block_scan(i < items ? mine.tiles << mine.shift : 0, warp_sums, &sum);
     total += sum;
   }
-  Header h;
-  h.total = total;
-  h.shares = max(1, min(p.grid, total / p.min_share));
-  h.base = total / h.shares;
-  h.rest = total - h.base * h.shares;
+  const Header h = cut(p, total);
   if (tid == 0) *p.head = h;
-  int carry = 0;
+  carry = 0;
   for (int i0 = 0; i0 < items; i0 += SCHED_THREADS) {
     const int i = i0 + tid;
     if (items > SCHED_THREADS) {
@@ -226,7 +218,6 @@ __global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
     if (i < items) {
       mine.first = carry + pre;
       p.items[i] = mine;
-      p.tickets[i] = 0;
       // Shares that begin in this item.
       const int end = mine.first + (mine.tiles << mine.shift);
       if (mine.tiles) {
@@ -249,16 +240,6 @@ __device__ __forceinline__ int slot_of(const Header& h, const Item& w, int c) {
   return 2 * c + (share_begin(h, c) < w.first ? 1 : 0);
 }
 
-constexpr int JOIN = 16;  // shares joined per first-level group
-
-// Slot of group k of the item whose first share is c0, behind the segments'
-// slots. Items of several groups have more than JOIN shares each, so within
-// JOIN neighbouring shares at most one item has its first group and at most
-// one a later group.
-__device__ __forceinline__ int group_slot(const Params& p, int c0, int k) {
-  return 2 * p.grid + 2 * ((c0 + k * JOIN) / JOIN) + (k == 0 ? 1 : 0);
-}
-
 // Layouts of a slot's [rows][D] floats, in float4. ROWS32 interleaves blocks of
 // 32 rows, [row / 32][D / 4][row % 32]: a warp whose lanes own rows then writes
 // and reads whole lines. Otherwise rows are contiguous.
@@ -268,107 +249,101 @@ __device__ __forceinline__ long long part_at(const Params& p, int slot, int row,
   return ROWS32 ? ((r >> 5) * (D / 4) + d4) * 32 + (r & 31) : r * (D / 4) + d4;
 }
 
-// Joins part k = 0 .. n - 1 in slot(k) for `rows` rows by 256 threads; emit
-// gets (row, first d4, m, l, U float4). U columns x K parts are in flight per
-// thread and round: the loads' latency, not their bandwidth, is what a join
-// waits for.
-template <int D, bool ROWS32, int U, int K, typename Slot, typename Emit>
-__device__ __forceinline__ void join_parts(const Params& p, int n, int rows, int tid, Slot slot, Emit emit) {
-  constexpr int C = D / 4 / U;
-  const int span = ROWS32 ? (rows + 31) & ~31 : rows;
-  for (int x = tid; x < span * C; x += 256) {
-    const int row = ROWS32 ? (x / (32 * C)) * 32 + (x & 31) : x / C, d4 = (ROWS32 ? (x >> 5) % C : x % C) * U;
-    if (row >= rows) continue;
-    float m = -INFINITY, l = 0.f;
-    float4 acc[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 < n; k0 += K) {
-      float2 ml[K];
-      float4 ov[K][U];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        ml[k] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int u = 0; u < U; ++u) ov[k][u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k0 + k < n) {
-          const int sl = slot(k0 + k);
-          ml[k] = __ldcg(p.part_ml + (long long)sl * p.part_rows + row);
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-            ov[k][u] = __ldcg(reinterpret_cast<const float4*>(p.part_o) + part_at<D, ROWS32>(p, sl, row, d4 + u));
-        }
-      }
-      float mn = m;
-#pragma unroll
-      for (int k = 0; k < K; ++k) mn = fmaxf(mn, ml[k].x);
-      const float ref = mn == -INFINITY ? 0.f : mn, a = ex2(m - ref);
-      l *= a;
-#pragma unroll
-      for (int u = 0; u < U; ++u) acc[u].x *= a, acc[u].y *= a, acc[u].z *= a, acc[u].w *= a;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const float w = ex2(ml[k].x - ref);
-        l = fmaf(ml[k].y, w, l);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          acc[u].x = fmaf(ov[k][u].x, w, acc[u].x);
-          acc[u].y = fmaf(ov[k][u].y, w, acc[u].y);
-          acc[u].z = fmaf(ov[k][u].z, w, acc[u].z);
-          acc[u].w = fmaf(ov[k][u].w, w, acc[u].w);
-        }
-      }
-      m = mn;
-    }
-    emit(row, d4, m, l, acc);
-  }
-}
-
-// This share's segment of a cut item is in its slot (written by the 256
-// threads of named barrier 1, which all call). Two levels: the last of each
-// JOIN neighbouring shares joins them into a slot of its group, the last such
-// group joins the groups. finish(row, first d4, m, l, float4[U], U).
-template <int D, bool ROWS32, int U, int K, typename Finish>
-__device__ __forceinline__ void join_cut(const Params& p, const Header& h, const Item& w, int share, int rows, int tid,
-                                         int* s_flag, Finish finish) {
-  const int c0 = share_of(h, w.first), c1 = share_of(h, last_weight(w));
-  const int k = (share - c0) / JOIN, grp0 = c0 + k * JOIN, gn = min(JOIN, c1 - grp0 + 1);
-  const int ngrp = cdiv(c1 - c0 + 1, JOIN);
-  auto meet = [] { asm volatile("bar.sync 1, 256;\n" ::: "memory"); };
-  __threadfence();
-  meet();
-  if (tid == 0) *s_flag = atomicAdd(p.tickets_g + slot_of(h, w, grp0), 1) == gn - 1;
-  meet();
-  if (*s_flag) {
-    __threadfence();
-    auto part = [&](int i) { return slot_of(h, w, grp0 + i); };
-    const int to = ngrp == 1 ? -1 : group_slot(p, c0, k);
-    auto emit = [&](int row, int d4, float m, float l, const float4* a) {
-      if (to < 0) {
-        finish(row, d4, m, l, a);
-      } else {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          reinterpret_cast<float4*>(p.part_o)[part_at<D, ROWS32>(p, to, row, d4 + u)] = a[u];
-        if (d4 == 0) p.part_ml[(long long)to * p.part_rows + row] = make_float2(m, l);
-      }
-    };
-    join_parts<D, ROWS32, U, K>(p, gn, rows, tid, part, emit);
-    if (ngrp > 1) {
-      __threadfence();
-      meet();
-      if (tid == 0) *s_flag = atomicAdd(p.tickets + w.index, 1) == ngrp - 1;
-      meet();
-      if (*s_flag) {
-        __threadfence();
-        join_parts<D, ROWS32, U, K>(p, ngrp, rows, tid, [&](int i) { return group_slot(p, c0, i); }, finish);
-      }
-    }
-  }
-  meet();  // s_flag may be written again
-}
-
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY; }
+
+// Joins the cut items. A work unit is one of `chunks` runs of rows of the item
+// that share s is the second of; its threads are float4 columns x lanes, a lane
+// taking every lanes-th part, K of them in flight: the loads' latency is what a
+// join waits for. The lanes meet in shared memory, in lane order.
+constexpr int JOIN_THREADS = 256;
+
+template <typename T, int D, bool ROWS32, int K>
+__global__ void __launch_bounds__(JOIN_THREADS, 4) join_kernel(Params p, int chunks) {
+  __shared__ float4 s_o[JOIN_THREADS];
+  __shared__ float2 s_ml[JOIN_THREADS];
+  allow_dependents();
+  wait_prerequisites();
+  const Header h = *p.head;
+  if (h.total == 0) return;
+  const int tid = threadIdx.x;
+  for (int u = blockIdx.x; u < h.shares * chunks; u += gridDim.x) {
+    const int s = u / chunks, chunk = u - s * chunks;
+    if (s == 0) continue;
+    const Item w = p.starts[s];
+    const int c0 = share_of(h, w.first), c1 = share_of(h, last_weight(w));
+    if (c0 != s - 1 || c1 < s) continue;
+    const int n = c1 - c0 + 1, rows = w.ntok * p.G * p.hc, per = cdiv(rows, chunks);
+    const int r0 = chunk * per, r1 = min(rows, r0 + per), cols = (r1 - r0) * (D / 4);
+    // Lanes: the power of two that fits the threads, no more than the parts.
+    int lanes = 1;
+    while (lanes * 2 * cols <= JOIN_THREADS && lanes < n) lanes *= 2;
+    for (int x0 = 0; x0 < cols; x0 += JOIN_THREADS / lanes) {
+      const int x = x0 + tid % (JOIN_THREADS / lanes), lane = tid / (JOIN_THREADS / lanes);
+      const bool live = x < cols;
+      // Rows run fastest where they do in the slot.
+      const int row = r0 + (ROWS32 ? x % (r1 - r0) : x / (D / 4)), d4 = ROWS32 ? x / (r1 - r0) : x % (D / 4);
+      float m = -INFINITY, l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k0 = lane; live && k0 < n; k0 += K * lanes) {
+        float2 ml[K];
+        float4 ov[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int part = k0 + k * lanes;
+          ml[k] = make_float2(-INFINITY, 0.f);
+          ov[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (part < n) {
+            const int slot = slot_of(h, w, c0 + part);
+            ml[k] = p.part_ml[(long long)slot * p.part_rows + row];
+            ov[k] = reinterpret_cast<const float4*>(p.part_o)[part_at<D, ROWS32>(p, slot, row, d4)];
+          }
+        }
+        float mn = m;
+#pragma unroll
+        for (int k = 0; k < K; ++k) mn = fmaxf(mn, ml[k].x);
+        const float ref = mn == -INFINITY ? 0.f : mn, a = ex2(m - ref);
+        l *= a, acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const float g = ex2(ml[k].x - ref);
+          l = fmaf(ml[k].y, g, l);
+          acc.x = fmaf(ov[k].x, g, acc.x);
+          acc.y = fmaf(ov[k].y, g, acc.y);
+          acc.z = fmaf(ov[k].z, g, acc.z);
+          acc.w = fmaf(ov[k].w, g, acc.w);
+        }
+        m = mn;
+      }
+      if (lanes > 1) {
+        __syncthreads();
+        s_o[tid] = acc;
+        s_ml[tid] = make_float2(m, l);
+        __syncthreads();
+        if (lane == 0) {
+          for (int k = 1; k < lanes; ++k) {
+            const float2 o = s_ml[tid + k * (JOIN_THREADS / lanes)];
+            const float4 v = s_o[tid + k * (JOIN_THREADS / lanes)];
+            const float mn = fmaxf(m, o.x), ref = mn == -INFINITY ? 0.f : mn, a = ex2(m - ref), g = ex2(o.x - ref);
+            l = l * a + o.y * g;
+            acc = make_float4(acc.x * a + v.x * g, acc.y * a + v.y * g, acc.z * a + v.z * g, acc.w * a + v.w * g);
+            m = mn;
+          }
+        }
+      }
+      if (live && lane == 0) {
+        // Row of the slot: (token, head of the item) or (token x group, KV head).
+        const int rt = row / p.hc, hh = row - rt * p.hc, t = rt / p.G;
+        const long long at = (long long)(w.tok0 + t) * p.H + (w.hg * p.hc + hh) * p.G + (rt - t * p.G);
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        uint2 out;
+        out.x = Num16<T>::pack2(acc.x * inv, acc.y * inv);
+        out.y = Num16<T>::pack2(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2*>(p.o + at * D + d4 * 4) = out;
+        if (p.lse && d4 == 0) p.lse[at] = lse_of(m, l);
+      }
+    }
+  }
+}
 
 // Key tile boxes of one unit: rows of a page, at most the unit's.
 __device__ __forceinline__ int page_id(const Params& p, int b, int key) {
@@ -436,14 +411,50 @@ __device__ __forceinline__ bool advance(const Params& p, Item& w, int x1) {
 constexpr int DW = 8;                    // compute warps
 constexpr int D_THREADS = 32 * (DW + 1);
 
+// Whether every warp of the 256 compute threads says yes.
+__device__ __forceinline__ bool all_came(bool mine) {
+  int all;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n barrier.red.and.pred q, 1, 256, p;\n selp.s32 %0, 1, 0, q;\n}\n"
+      : "=r"(all)
+      : "r"((int)mine)
+      : "memory");
+  return all != 0;
+}
+
+// Item i (sequence i / groups, head group i % groups); its weight is its tiles.
+__device__ __forceinline__ Item few_item(const Params& p, int i, int first) {
+  Item w;
+  int q0, nq, base, len;
+  const int groups = p.Hk / p.hc;
+  w.b = i / groups;
+  w.hg = i - w.b * groups;
+  sequence(p, w.b, &q0, &nq, &base, &len);
+  w.tok0 = q0;
+  w.ntok = nq;
+  w.pos0 = base;
+  w.keys = min(max(base + nq, 0), len);
+  w.tiles = nq > 0 ? max(1, cdiv(w.keys, p.unit)) : 0;
+  w.first = first;
+  w.shift = 0;
+  w.index = i;
+  return w;
+}
+__device__ __forceinline__ bool few_advance(const Params& p, Item& w, int x1) {
+  if (w.first + w.tiles >= x1) return false;
+  w = few_item(p, w.index + 1, w.first + w.tiles);
+  return true;
+}
+
 struct DLayout {
-  uint32_t merge, bars, total;
+  uint32_t merge, q, bars, total;
 };
 __host__ __device__ inline DLayout dlayout(int D, int stages, int rows, int hc) {
   DLayout L;
   L.merge = (uint32_t)stages * 2u * 16384u * (uint32_t)(D / 64);
   const uint32_t m = hc < 8 ? 8u * (uint32_t)rows * (uint32_t)(D + 4) * 4u : 0u;  // [warp][row]{o[D], m, l}
-  L.bars = L.merge + m;
+  L.q = L.merge + m;  // an item's query rows, [token][head of the item][D]
+  L.bars = L.q + (uint32_t)(rows * hc * D) * 2u;
   L.total = 1024 + L.bars + 16u * (uint32_t)stages + 16u;
   return L;
 }
@@ -459,38 +470,92 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
   const uint32_t sb = smem_u32(smem);
   const DLayout lay = dlayout(D, stages, rows_max, p.hc);
   float* merge = reinterpret_cast<float*>(smem + lay.merge);
-  __shared__ int s_flag;
+  __shared__ int s_sums[DW + 1];
+  __shared__ Item s_start, s_item;  // the share's first item, and the one whose queries lie in shared memory
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto full_bar = [&](int s) { return sb + lay.bars + 8u * s; };
   auto empty_bar = [&](int s) { return sb + lay.bars + 8u * (stages + s); };
+  const uint32_t q_full = empty_bar(stages), q_empty = q_full + 8;
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
       tc::mbar_init(full_bar(s), 1);
       tc::mbar_init(empty_bar(s), DW);
     }
+    tc::mbar_init(q_full, 1);
+    tc::mbar_init(q_empty, DW);
     tc::mbar_fence_init();
     tc::tma_prefetch_desc(&tk);
     tc::tma_prefetch_desc(&tv);
   }
-  __syncthreads();
-  wait_prerequisites();
   allow_dependents();
-  const Header head = *p.head;
-  const Item start = p.starts[blockIdx.x];
+  // The schedule: each thread sums a run of items, and the one whose run holds
+  // this share's first unit looks it up, for itself and for the join.
+  const int items = p.B * (p.Hk / p.hc), per = cdiv(items, D_THREADS);
+  const int i0 = min(items, tid * per), i1 = min(items, i0 + per);
+  int local = 0;
+  for (int i = i0; i < i1; ++i) local += few_item(p, i, 0).tiles;
+  int incl = local;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) s_sums[warp] = incl;
+  __syncthreads();
+  int before = incl - local, total = 0;
+#pragma unroll
+  for (int w = 0; w <= DW; ++w) {
+    if (w < warp) before += s_sums[w];
+    total += s_sums[w];
+  }
+  const Header head = cut(p, total);
   const int share = blockIdx.x;
-  if (share >= head.shares || head.total == 0) return;
+  if (total == 0 && tid == 0 && share == 0) *p.head = head;
+  if (share >= head.shares || total == 0) return;
   const int x0 = share_begin(head, share), x1 = share_begin(head, share + 1);
+  if (before <= x0 && x0 < before + local) {
+    Item w = few_item(p, i0, before);
+    while (w.first + w.tiles <= x0) w = few_item(p, w.index + 1, w.first + w.tiles);
+    s_start = w;
+    p.starts[share] = w;
+    if (share == 0) *p.head = head;
+  }
+  __syncthreads();
   const int unit = p.unit, hc = p.hc;
   const int br = min(unit, 1 << p.page_shift), nb = unit / br;  // box rows, boxes per unit
 
   if (warp == DW) {
     // Producer: the boxes of K and V (and of both halves of 128-wide heads) are
-    // issued by the lanes in parallel, all counted on the stage's barrier.
-    int it = 0;
+    // issued by the lanes in parallel, all counted on the stage's barrier. An
+    // item's record and queries go to shared memory while the item before it
+    // still streams: a ring that stands still costs bandwidth that does not
+    // come back.
+    int it = 0, published = 0;
     bool ok = true;
-    for (Item w = start; ok;) {
+    Item w = s_start;
+    auto ids_of = [&](const Item& w) {
+      return PageIds(p, w.b, br, nb, unit_at(w, x0), min(w.keys, unit_at(w, x1) * unit));
+    };
+    auto publish = [&](const Item& w) {
+      ok = tc::mbar_wait_w(q_empty, (published & 1) ^ 1, &g_status, 4);
+      if (!ok) return;
+      ++published;
+      const uint32_t bytes = (uint32_t)(hc * p.G * D) * 2u;  // of a token
+      if (lane == 0) {
+        s_item = w;
+        tc::mbar_expect_tx(q_full, bytes * w.ntok);
+      }
+      __syncwarp();
+      for (int t = lane; t < w.ntok; t += 32)
+        tc::bulk_load(sb + lay.q + t * bytes, p.q + ((long long)(w.tok0 + t) * p.H + w.hg * hc * p.G) * D, bytes, q_full);
+    };
+    PageIds ids = ids_of(w);
+    publish(w);
+    while (ok) {
       const int u0 = unit_at(w, x0), u1 = unit_at(w, x1);
-      PageIds ids(p, w.b, br, nb, u0, min(w.keys, u1 * unit));
+      Item next = w;
+      PageIds next_ids = ids;
+      const bool more = w.first + w.tiles < x1;
       for (int u = u0; u < u1; ++u, ++it) {
         const int st = it % stages;
         if (!(ok = tc::mbar_wait_w(empty_bar(st), ((it / stages) & 1) ^ 1, &g_status, 1))) break;
@@ -508,8 +573,18 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
                         pid, full_bar(st));
           }
         }
+        if (more && u == min(u0 + stages, u1) - 1) {  // the units before this item's are consumed
+          do {  // sequences without new tokens have no units
+            few_advance(p, next, x1);
+          } while (next.tiles == 0);
+          next_ids = ids_of(next);
+          publish(next);
+          if (!ok) break;
+        }
       }
-      if (!advance(p, w, x1)) break;
+      if (!ok || !more) break;
+      w = next;
+      ids = next_ids;
     }
     if (!ok)  // a wait gave up: let the copies in flight land before the CTA ends
       for (int f = max(0, it - stages); f < it; ++f) tc::mbar_wait_w(full_bar(f % stages), (f / stages) & 1, &g_status, 3);
@@ -529,12 +604,25 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
   const int G = p.G;
   int it = 0;
   bool ok = true;
-  for (Item w = start;;) {
+  auto finish = [&](const Item& w, int rh, int d4, float mm, float ll, const float4& a) {
+    const int row = rh / hc, h = rh - row * hc;
+    const float inv = ll > 0.f ? 1.f / ll : 0.f;
+    const long long at = (long long)(w.tok0 + row / G) * p.H + (w.hg * hc + h) * G + row % G;
+    uint2 out;
+    out.x = Num16<T>::pack2(a.x * inv, a.y * inv);
+    out.y = Num16<T>::pack2(a.z * inv, a.w * inv);
+    *reinterpret_cast<uint2*>(p.o + at * D + d4 * 4) = out;
+    if (p.lse && d4 == 0) p.lse[at] = lse_of(mm, ll);
+  };
+  Item w = s_start;
+  for (int taken = 0;; ++taken) {
+    // The next item that has units. Where the warps meet inside the loop they
+    // also agree on whether it came.
+    bool came = tc::mbar_wait_w(q_full, taken & 1, &g_status, 5);
+    if (slices > 1) came = all_came(came);
+    if (!came) break;
+    w = s_item;
     const int u0 = unit_at(w, x0), u1 = unit_at(w, x1);
-    if (u0 >= u1) {
-      if (!advance(p, w, x1)) break;
-      continue;
-    }
     const int rows = w.ntok * G, hk = w.hg * hc + hl;
     uint32_t qa[D / 16][4];
     int lim[2];
@@ -543,13 +631,15 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
       const int r = g4 + 8 * e, t = r / G;
       const bool live = r < rows && (R16 || e == 0);
       lim[e] = live ? min(w.pos0 + t + 1, w.keys) : 0;
-      const uint16_t* qrow = p.q + ((long long)(w.tok0 + t) * p.H + hk * G + r % G) * D + 2 * c4;
+      const uint32_t qrow = sb + lay.q + (uint32_t)((t * hc + hl) * G + r % G) * (2u * D) + 4u * c4;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        qa[kk][e] = live ? *reinterpret_cast<const uint32_t*>(qrow + kk * 16) : 0u;
-        qa[kk][2 + e] = live ? *reinterpret_cast<const uint32_t*>(qrow + kk * 16 + 8) : 0u;
+        qa[kk][e] = live ? lds32(qrow + kk * 32) : 0u;
+        qa[kk][2 + e] = live ? lds32(qrow + kk * 32 + 16) : 0u;
       }
     }
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(q_empty);
     float o[D / 8][4];
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -631,16 +721,6 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
     }
     const bool cut = u0 > 0 || u1 < w.tiles;
     const int slot = slot_of(head, w, share);
-    auto finish = [&](int row, int h, int d4, float mm, float ll, const float4& a) {
-      const float inv = ll > 0.f ? 1.f / ll : 0.f;
-      const long long at = (long long)(w.tok0 + row / G) * p.H + (w.hg * hc + h) * G + row % G;
-      uint2 out;
-      out.x = Num16<T>::pack2(a.x * inv, a.y * inv);
-      out.y = Num16<T>::pack2(a.z * inv, a.w * inv);
-      *reinterpret_cast<uint2*>(p.o + at * D + d4 * 4) = out;
-      if (p.lse && d4 == 0) p.lse[at] = lse_of(mm, ll);
-    };
-    auto finish_row = [&](int rh, int d4, float mm, float ll, const float4& a) { finish(rh / hc, rh % hc, d4, mm, ll, a); };
     if (slices == 1) {
 #pragma unroll
       for (int e = 0; e < (R16 ? 2 : 1); ++e) {
@@ -690,7 +770,7 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
           a.z = fmaf(v4.z, wgt, a.z), a.w = fmaf(v4.w, wgt, a.w);
         }
         if (!cut) {
-          finish_row(rh, d4, mm, ll, a);
+          finish(w, rh, d4, mm, ll, a);
         } else {
           const long long at = (long long)slot * p.part_rows + r * hc + h;
           *reinterpret_cast<float4*>(p.part_o + at * D + d4 * 4) = a;
@@ -699,10 +779,7 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
       }
       if (!cut) asm volatile("bar.sync 1, 256;\n" ::: "memory");  // before the area is written again
     }
-    if (cut)
-      join_cut<D, false, 1, 8>(p, head, w, share, rows * hc, tid, &s_flag,
-                            [&](int rh, int d4, float mm, float ll, const float4* a) { finish_row(rh, d4, mm, ll, *a); });
-    if (!advance(p, w, x1)) break;
+    if (w.first + w.tiles >= x1) break;
   }
 }
 
@@ -863,7 +940,6 @@ __global__ void __launch_bounds__(T_THREADS, 1)
   auto pv_done = [&](int g) { return q_full + 24 + 8u * (2 * S::NB + g); };
   const uint32_t o_free = pv_done(2), done_bar = o_free + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 8 * S::NBARS);
-  __shared__ int s_flag;
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   int* status = &g_status;
 
@@ -1044,18 +1120,26 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     int nj0 = 0, nj1 = 0;  // jobs each group has had
     int buf = 0, ph = 0;   // buffer and phase of the item's job 0
     bool ok = true;
-    for (Item w = start; !idle;) {
-      const int j0 = unit_at(w, x0), j1 = unit_at(w, x1), n = j1 - j0;
-      if (n <= 0) {
-        if (!advance(p, w, x1)) break;
-        continue;
+    // The item's record is read again behind the jobs: its registers are needed there.
+    for (int index = start.index; !idle; ++index) {
+      int j0, n, limit;
+      bool dual, live;
+      const int row_tok = r / G;
+      {
+        const Item w = p.items[index];
+        j0 = unit_at(w, x0);
+        n = unit_at(w, x1) - j0;
+        if (n <= 0) {
+          if (w.first + (w.tiles << w.shift) >= x1) break;
+          continue;
+        }
+        dual = w.ntok > tpt;
+        const int t = (dual ? grp * tpt : 0) + row_tok;
+        live = r < tpt * G && t < w.ntok;
+        // Keys this row sees; rows that do not exist mask nothing and are never read.
+        limit = live ? min(w.pos0 + t + 1, w.keys) : 0x7fffffff;
       }
-      const bool dual = w.ntok > tpt;
-      const int t = (dual ? grp * tpt : 0) + r / G;
-      const bool live = r < tpt * G && t < w.ntok;
       const bool warp_live = __any_sync(0xffffffffu, live);
-      // Keys this row sees; rows that do not exist mask nothing and are never read.
-      const int limit = live ? min(w.pos0 + t + 1, w.keys) : 0x7fffffff;
       float M = -INFINITY;
       uint64_t l2 = pair(0.f, 0.f);
       const int jobs = dual ? 2 * n : n;
@@ -1156,10 +1240,12 @@ __global__ void __launch_bounds__(T_THREADS, 1)
       if (buf >= S::NB) buf -= S::NB, ph ^= 1;
       const float2 lv = unpair(l2);
       float l = lv.x + lv.y;
+      const Item w = p.items[index];
+      const int t = (dual ? grp * tpt : 0) + row_tok;
 
       // Epilogue: this group's rows (dual), or both groups' accumulators of
       // the same rows joined by group 0.
-      const bool has1 = dual || n > 1, cut = j0 > 0 || j1 < w.tiles;
+      const bool has1 = dual || n > 1, cut = j0 > 0 || j0 + n < w.tiles;
       nj0 += (jobs + 1) / 2;
       nj1 += jobs / 2;
       float a0 = 1.f, a1 = 0.f;
@@ -1229,22 +1315,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
         }
       }
       tc::mbar_arrive(o_free);
-      if (cut)
-        join_cut<D, true, 4, 4>(p, head, w, share, w.ntok * G, tid, &s_flag,
-                             [&](int row, int d4, float mm, float ll, const float4* a) {
-                               const float inv = ll > 0.f ? 1.f / ll : 0.f;
-                               const long long at = (long long)(w.tok0 + row / G) * p.H + w.hg * G + row % G;
-                               uint4* dst = reinterpret_cast<uint4*>(p.o + at * D + d4 * 4);
-#pragma unroll
-                               for (int u = 0; u < 2; ++u) {
-                                 const float f[8] = {a[2 * u].x * inv,     a[2 * u].y * inv,     a[2 * u].z * inv,
-                                                     a[2 * u].w * inv,     a[2 * u + 1].x * inv, a[2 * u + 1].y * inv,
-                                                     a[2 * u + 1].z * inv, a[2 * u + 1].w * inv};
-                                 dst[u] = pack16x8<T>(f);
-                               }
-                               if (p.lse && d4 == 0) p.lse[at] = lse_of(mm, ll);
-                             });
-      if (!advance(p, w, x1)) break;
+      if (w.first + (w.tiles << w.shift) >= x1) break;
     }
   }
   tc::tc_fence_before();
@@ -1260,7 +1331,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
 // ---------------------------------------------------------------------------
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-constexpr size_t MAX_SMEM = 227 * 1024 - 64;  // dynamic part of a CTA's shared memory
+constexpr size_t MAX_SMEM = 227 * 1024 - 256;  // dynamic part of a CTA's shared memory
 constexpr int FEW_ROWS = 16;  // query rows per KV head the warp-level kernel takes
 
 struct Plan {
@@ -1278,7 +1349,7 @@ Plan plan(int N, int B, int max_q, int H, int Hk, int D) {
     pl.unit = 128 / pl.hc;
     pl.tok_item = max_q;
     pl.grid_cap = 2 * MAX_SMS;
-    pl.max_items = B * (Hk / pl.hc);
+    pl.max_items = 0;  // not listed: every CTA finds its own
     pl.part_rows = max_q * G * pl.hc;
   } else {
     pl.hc = 1;
@@ -1288,9 +1359,8 @@ Plan plan(int N, int B, int max_q, int H, int Hk, int D) {
     pl.max_items = Hk * (N / pl.tok_item + B);
     pl.part_rows = 256;
   }
-  pl.slots = 2 * pl.grid_cap + 2 * (pl.grid_cap / JOIN + 1);
-  pl.bytes = 256 + align256(sizeof(Item) * (size_t)pl.max_items) + align256(sizeof(int) * (size_t)pl.max_items) +
-             align256(sizeof(Item) * (size_t)pl.grid_cap) + align256(sizeof(int) * 2 * (size_t)pl.grid_cap) +
+  pl.slots = 2 * pl.grid_cap;
+  pl.bytes = 256 + align256(sizeof(Item) * (size_t)pl.max_items) + align256(sizeof(Item) * (size_t)pl.grid_cap) +
              align256(sizeof(float) * (size_t)pl.slots * pl.part_rows * D) +
              align256(sizeof(float2) * (size_t)pl.slots * pl.part_rows);
   return pl;
@@ -1305,9 +1375,7 @@ void carve(Params& p, const Plan& pl, void* base, int D) {
   };
   p.head = reinterpret_cast<Header*>(take(sizeof(Header)));
   p.items = reinterpret_cast<Item*>(take(sizeof(Item) * (size_t)pl.max_items));
-  p.tickets = reinterpret_cast<int*>(take(sizeof(int) * (size_t)pl.max_items));
   p.starts = reinterpret_cast<Item*>(take(sizeof(Item) * (size_t)pl.grid_cap));
-  p.tickets_g = reinterpret_cast<int*>(take(sizeof(int) * 2 * (size_t)pl.grid_cap));
   p.part_o = reinterpret_cast<float*>(take(sizeof(float) * (size_t)pl.slots * pl.part_rows * D));
   p.part_ml = reinterpret_cast<float2*>(take(sizeof(float2) * (size_t)pl.slots * pl.part_rows));
 }
@@ -1322,6 +1390,28 @@ int make_tmap_pages(CUtensorMap* map, const void* base, bool bf, int D, int page
   return tc::make_tmap_16(map, base, bf, 4, dims, strides, box);
 }
 
+// Launches a kernel whose prologue may overlap the kernel before it.
+template <typename... Formal, typename... Actual>
+int launch_dependent(void (*kernel)(Formal...), int grid, int threads, size_t smem, cudaStream_t s, Actual&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MFB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return MFB_OK;
+}
+
+template <typename T, int D, bool ROWS32>
+int run_join(const Params& p, int chunks, int sms, cudaStream_t s) {
+  return launch_dependent(join_kernel<T, D, ROWS32, 8>, std::min(p.grid * chunks, 8 * sms), JOIN_THREADS, 0, s, p, chunks);
+}
+
 template <typename T, int D, bool R16>
 int run_few(Params& p, const Plan& pl, const CUtensorMap& tk, const CUtensorMap& tv, int sms, cudaStream_t s) {
   const int rows = p.max_q * p.G;
@@ -1331,20 +1421,9 @@ int run_few(Params& p, const Plan& pl, const CUtensorMap& tk, const CUtensorMap&
   MFB_CUDA_TRY(cudaFuncSetAttribute(few_rows_kernel<T, D, R16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MAX_SMEM));
   const int per_sm = 2 * smem + 4096 <= 228 * 1024 ? 2 : 1;
   p.grid = std::min(per_sm * sms, pl.grid_cap);
-  schedule_kernel<true><<<1, SCHED_THREADS, 0, s>>>(p);
-  MFB_LAUNCH_CHECK("paged attention schedule");
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.grid);
-  cfg.blockDim = dim3(D_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  MFB_CUDA_TRY(cudaLaunchKernelEx(&cfg, few_rows_kernel<T, D, R16>, tk, tv, p, stages, rows));
-  return MFB_OK;
+  few_rows_kernel<T, D, R16><<<p.grid, D_THREADS, smem, s>>>(tk, tv, p, stages, rows);
+  MFB_LAUNCH_CHECK("paged attention (few rows)");
+  return run_join<T, D, false>(p, cdiv(pl.part_rows, 4), sms, s);
 }
 
 template <typename T, int D>
@@ -1372,20 +1451,10 @@ int run(Params& p, const Plan& pl, const void* q, const void* kp, const void* vp
   static_assert(smem <= MAX_SMEM, "chunk kernel shared memory");
   MFB_CUDA_TRY(cudaFuncSetAttribute(chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   p.grid = sms;
-  schedule_kernel<false><<<1, SCHED_THREADS, sizeof(int) * (size_t)(p.B + 1), s>>>(p);
+  schedule_kernel<<<1, SCHED_THREADS, sizeof(int) * (size_t)(p.B + 1), s>>>(p);
   MFB_LAUNCH_CHECK("paged attention schedule");
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.grid);
-  cfg.blockDim = dim3(T_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  MFB_CUDA_TRY(cudaLaunchKernelEx(&cfg, chunk_kernel<T, D>, tq, tk, tv, p));
-  return MFB_OK;
+  if ((st = launch_dependent(chunk_kernel<T, D>, p.grid, T_THREADS, smem, s, tq, tk, tv, p))) return st;
+  return run_join<T, D, true>(p, 16, sms, s);
 }
 
 }  // namespace paged
