@@ -55,6 +55,7 @@ struct __align__(16) Item {
 // longer than `base`. A unit belongs to the share its weight starts in.
 struct Header {
   int total, shares, base, rest;
+  int cuts, pad[3];  // items of more than one share
 };
 
 struct Params {
@@ -67,6 +68,7 @@ struct Params {
   Header* head;
   Item* items;
   Item* starts;    // [grid] each share's first item
+  Item* cuts;      // [grid] the items of more than one share, in any order
   float* part_o;   // [slots][part_rows] x D
   float2* part_ml; // [slots][part_rows]
   int N, B, H, Hk, G, max_q, max_pages, num_pages, page_shift;
@@ -127,6 +129,7 @@ __device__ __forceinline__ Header cut(const Params& p, int total) {
   h.shares = max(1, min(p.grid, total / p.min_share));
   h.base = total / h.shares;
   h.rest = total - h.base * h.shares;
+  h.cuts = h.pad[0] = h.pad[1] = h.pad[2] = 0;
   return h;
 }
 __device__ __forceinline__ int share_begin(const Header& h, int i) { return i * h.base + min(i, h.rest); }
@@ -159,8 +162,9 @@ __device__ __forceinline__ void sequence(const Params& p, int b, int* q0, int* n
 __global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
   allow_dependents();
   extern __shared__ int item_base[];  // [B] items before each sequence
-  __shared__ int warp_sums[32];
+  __shared__ int warp_sums[32], s_cuts;
   const int tid = threadIdx.x;
+  if (tid == 0) s_cuts = 0;
   int carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += SCHED_THREADS) {
     const int b = b0 + tid;
@@ -206,8 +210,7 @@ __global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
     pre = block_scan(i < items ? mine.tiles << mine.shift : 0, warp_sums, &sum);
     total += sum;
   }
-  const Header h = cut(p, total);
-  if (tid == 0) *p.head = h;
+  Header h = cut(p, total);
   carry = 0;
   for (int i0 = 0; i0 < items; i0 += SCHED_THREADS) {
     const int i = i0 + tid;
@@ -222,12 +225,16 @@ __global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
       const int end = mine.first + (mine.tiles << mine.shift);
       if (mine.tiles) {
         int s = share_of(h, mine.first);
+        if (s != share_of(h, last_weight(mine))) p.cuts[atomicAdd(&s_cuts, 1)] = mine;
         if (share_begin(h, s) < mine.first) ++s;
         for (; s < h.shares && share_begin(h, s) < end; ++s) p.starts[s] = mine;
       }
     }
     carry += sum;
   }
+  __syncthreads();
+  h.cuts = s_cuts;
+  if (tid == 0) *p.head = h;
 }
 
 // ---------------------------------------------------------------------------
@@ -251,98 +258,119 @@ __device__ __forceinline__ long long part_at(const Params& p, int slot, int row,
 
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY; }
 
-// Joins the cut items. A work unit is one of `chunks` runs of rows of the item
-// that share s is the second of; its threads are float4 columns x lanes, a lane
-// taking every lanes-th part, K of them in flight: the loads' latency is what a
-// join waits for. The lanes meet in shared memory, in lane order.
+// Joins the cut items. Each is split by rows over an equal part of the blocks;
+// a block's threads are float4 columns x lanes, a lane taking every lanes-th
+// part. U columns x K parts are in flight per thread: a join waits for the
+// latency of its loads. The lanes meet in shared memory, in lane order.
 constexpr int JOIN_THREADS = 256;
 
-template <typename T, int D, bool ROWS32, int K>
-__global__ void __launch_bounds__(JOIN_THREADS, 4) join_kernel(Params p, int chunks) {
+template <typename T, int D, bool ROWS32, int U, int K>
+__device__ __forceinline__ void join_rows(const Params& p, const Header& h, const Item& w, int c0, int n, int r0,
+                                          int r1, float4* s_o, float2* s_ml) {
+  const int tid = threadIdx.x, cols = (r1 - r0) * (D / 4), nrow = r1 - r0;
+  int lanes = 1;
+  while (U == 1 && lanes * 2 * cols <= JOIN_THREADS && lanes * K < n) lanes *= 2;
+  const int wide = JOIN_THREADS / lanes, lane = tid / wide;
+  for (int x0 = tid % wide; x0 - tid % wide < cols; x0 += U * wide) {
+    int row[U], d4[U];
+    float m[U], l[U];
+    float4 acc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int x = min(x0 + u * wide, cols - 1);
+      // Rows run fastest where they do in the slot.
+      const int q = ROWS32 ? x / nrow : x / (D / 4);
+      row[u] = r0 + (ROWS32 ? x - q * nrow : q);
+      d4[u] = ROWS32 ? q : x - q * (D / 4);
+      m[u] = -INFINITY;
+      l[u] = 0.f;
+      acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int k0 = lane; k0 < n; k0 += K * lanes) {
+      float2 ml[K][U];
+      float4 ov[K][U];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int part = k0 + k * lanes;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          ml[k][u] = make_float2(-INFINITY, 0.f);
+          ov[k][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (part < n) {
+            const int slot = slot_of(h, w, c0 + part);
+            ml[k][u] = p.part_ml[(long long)slot * p.part_rows + row[u]];
+            ov[k][u] = reinterpret_cast<const float4*>(p.part_o)[part_at<D, ROWS32>(p, slot, row[u], d4[u])];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float mn = m[u];
+#pragma unroll
+        for (int k = 0; k < K; ++k) mn = fmaxf(mn, ml[k][u].x);
+        const float ref = mn == -INFINITY ? 0.f : mn, a = ex2(m[u] - ref);
+        l[u] *= a, acc[u].x *= a, acc[u].y *= a, acc[u].z *= a, acc[u].w *= a;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const float g = ex2(ml[k][u].x - ref);
+          l[u] = fmaf(ml[k][u].y, g, l[u]);
+          acc[u].x = fmaf(ov[k][u].x, g, acc[u].x);
+          acc[u].y = fmaf(ov[k][u].y, g, acc[u].y);
+          acc[u].z = fmaf(ov[k][u].z, g, acc[u].z);
+          acc[u].w = fmaf(ov[k][u].w, g, acc[u].w);
+        }
+        m[u] = mn;
+      }
+    }
+    if (lanes > 1) {  // U == 1
+      __syncthreads();
+      s_o[tid] = acc[0];
+      s_ml[tid] = make_float2(m[0], l[0]);
+      __syncthreads();
+      for (int k = 1; lane == 0 && k < lanes; ++k) {
+        const float2 o = s_ml[tid + k * wide];
+        const float4 v = s_o[tid + k * wide];
+        const float mn = fmaxf(m[0], o.x), ref = mn == -INFINITY ? 0.f : mn, a = ex2(m[0] - ref), g = ex2(o.x - ref);
+        l[0] = l[0] * a + o.y * g;
+        acc[0] = make_float4(acc[0].x * a + v.x * g, acc[0].y * a + v.y * g, acc[0].z * a + v.z * g,
+                             acc[0].w * a + v.w * g);
+        m[0] = mn;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (lane > 0 || x0 + u * wide >= cols) continue;
+      // Row of the slot: (token x group, KV head of the item).
+      const int rt = row[u] / p.hc, hh = row[u] - rt * p.hc, t = rt / p.G;
+      const long long at = (long long)(w.tok0 + t) * p.H + (w.hg * p.hc + hh) * p.G + (rt - t * p.G);
+      const float inv = l[u] > 0.f ? 1.f / l[u] : 0.f;
+      uint2 out;
+      out.x = Num16<T>::pack2(acc[u].x * inv, acc[u].y * inv);
+      out.y = Num16<T>::pack2(acc[u].z * inv, acc[u].w * inv);
+      *reinterpret_cast<uint2*>(p.o + at * D + d4[u] * 4) = out;
+      if (p.lse && d4[u] == 0) p.lse[at] = lse_of(m[u], l[u]);
+    }
+  }
+}
+
+template <typename T, int D, bool ROWS32>
+__global__ void __launch_bounds__(JOIN_THREADS, 4) join_kernel(Params p) {
   __shared__ float4 s_o[JOIN_THREADS];
   __shared__ float2 s_ml[JOIN_THREADS];
   allow_dependents();
   wait_prerequisites();
   const Header h = *p.head;
-  if (h.total == 0) return;
-  const int tid = threadIdx.x;
-  for (int u = blockIdx.x; u < h.shares * chunks; u += gridDim.x) {
-    const int s = u / chunks, chunk = u - s * chunks;
-    if (s == 0) continue;
-    const Item w = p.starts[s];
-    const int c0 = share_of(h, w.first), c1 = share_of(h, last_weight(w));
-    if (c0 != s - 1 || c1 < s) continue;
-    const int n = c1 - c0 + 1, rows = w.ntok * p.G * p.hc, per = cdiv(rows, chunks);
-    const int r0 = chunk * per, r1 = min(rows, r0 + per), cols = (r1 - r0) * (D / 4);
-    // Lanes: the power of two that fits the threads, no more than the parts.
-    int lanes = 1;
-    while (lanes * 2 * cols <= JOIN_THREADS && lanes < n) lanes *= 2;
-    for (int x0 = 0; x0 < cols; x0 += JOIN_THREADS / lanes) {
-      const int x = x0 + tid % (JOIN_THREADS / lanes), lane = tid / (JOIN_THREADS / lanes);
-      const bool live = x < cols;
-      // Rows run fastest where they do in the slot.
-      const int row = r0 + (ROWS32 ? x % (r1 - r0) : x / (D / 4)), d4 = ROWS32 ? x / (r1 - r0) : x % (D / 4);
-      float m = -INFINITY, l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k0 = lane; live && k0 < n; k0 += K * lanes) {
-        float2 ml[K];
-        float4 ov[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int part = k0 + k * lanes;
-          ml[k] = make_float2(-INFINITY, 0.f);
-          ov[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (part < n) {
-            const int slot = slot_of(h, w, c0 + part);
-            ml[k] = p.part_ml[(long long)slot * p.part_rows + row];
-            ov[k] = reinterpret_cast<const float4*>(p.part_o)[part_at<D, ROWS32>(p, slot, row, d4)];
-          }
-        }
-        float mn = m;
-#pragma unroll
-        for (int k = 0; k < K; ++k) mn = fmaxf(mn, ml[k].x);
-        const float ref = mn == -INFINITY ? 0.f : mn, a = ex2(m - ref);
-        l *= a, acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const float g = ex2(ml[k].x - ref);
-          l = fmaf(ml[k].y, g, l);
-          acc.x = fmaf(ov[k].x, g, acc.x);
-          acc.y = fmaf(ov[k].y, g, acc.y);
-          acc.z = fmaf(ov[k].z, g, acc.z);
-          acc.w = fmaf(ov[k].w, g, acc.w);
-        }
-        m = mn;
-      }
-      if (lanes > 1) {
-        __syncthreads();
-        s_o[tid] = acc;
-        s_ml[tid] = make_float2(m, l);
-        __syncthreads();
-        if (lane == 0) {
-          for (int k = 1; k < lanes; ++k) {
-            const float2 o = s_ml[tid + k * (JOIN_THREADS / lanes)];
-            const float4 v = s_o[tid + k * (JOIN_THREADS / lanes)];
-            const float mn = fmaxf(m, o.x), ref = mn == -INFINITY ? 0.f : mn, a = ex2(m - ref), g = ex2(o.x - ref);
-            l = l * a + o.y * g;
-            acc = make_float4(acc.x * a + v.x * g, acc.y * a + v.y * g, acc.z * a + v.z * g, acc.w * a + v.w * g);
-            m = mn;
-          }
-        }
-      }
-      if (live && lane == 0) {
-        // Row of the slot: (token, head of the item) or (token x group, KV head).
-        const int rt = row / p.hc, hh = row - rt * p.hc, t = rt / p.G;
-        const long long at = (long long)(w.tok0 + t) * p.H + (w.hg * p.hc + hh) * p.G + (rt - t * p.G);
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        uint2 out;
-        out.x = Num16<T>::pack2(acc.x * inv, acc.y * inv);
-        out.y = Num16<T>::pack2(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(p.o + at * D + d4 * 4) = out;
-        if (p.lse && d4 == 0) p.lse[at] = lse_of(m, l);
-      }
-    }
-  }
+  if (h.cuts == 0) return;
+  const int chunks = max(1, (int)gridDim.x / h.cuts);  // blocks per item (cuts <= gridDim.x: fewer than shares)
+  const int k = blockIdx.x / chunks, chunk = blockIdx.x - k * chunks;
+  if (k >= h.cuts) return;
+  const Item w = p.cuts[k];
+  const int rows = w.ntok * p.G * p.hc, per = cdiv(rows, chunks), r0 = chunk * per, r1 = min(rows, r0 + per);
+  if (r0 >= r1) return;
+  const int c0 = share_of(h, w.first), n = share_of(h, last_weight(w)) - c0 + 1;
+  if (n <= 2) join_rows<T, D, ROWS32, 4, 2>(p, h, w, c0, n, r0, r1, s_o, s_ml);
+  else if (n <= 4) join_rows<T, D, ROWS32, 2, 4>(p, h, w, c0, n, r0, r1, s_o, s_ml);
+  else join_rows<T, D, ROWS32, 1, 8>(p, h, w, c0, n, r0, r1, s_o, s_ml);
 }
 
 // Key tile boxes of one unit: rows of a page, at most the unit's.
@@ -470,7 +498,7 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
   const uint32_t sb = smem_u32(smem);
   const DLayout lay = dlayout(D, stages, rows_max, p.hc);
   float* merge = reinterpret_cast<float*>(smem + lay.merge);
-  __shared__ int s_sums[DW + 1];
+  __shared__ int s_sums[DW + 1], s_cuts;
   __shared__ Item s_start, s_item;  // the share's first item, and the one whose queries lie in shared memory
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto full_bar = [&](int s) { return sb + lay.bars + 8u * s; };
@@ -489,7 +517,7 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
   }
   allow_dependents();
   // The schedule: each thread sums a run of items, and the one whose run holds
-  // this share's first unit looks it up, for itself and for the join.
+  // this share's first unit looks it up.
   const int items = p.B * (p.Hk / p.hc), per = cdiv(items, D_THREADS);
   const int i0 = min(items, tid * per), i1 = min(items, i0 + per);
   int local = 0;
@@ -510,15 +538,28 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
   }
   const Header head = cut(p, total);
   const int share = blockIdx.x;
-  if (total == 0 && tid == 0 && share == 0) *p.head = head;
+  if (share == 0) {
+    // The first CTA lists the cut items for the join.
+    if (tid == 0) s_cuts = 0;
+    __syncthreads();
+    for (int i = i0, first = before; total && i < i1; ++i) {
+      const Item w = few_item(p, i, first);
+      first += w.tiles;
+      if (w.tiles && share_of(head, w.first) != share_of(head, last_weight(w))) p.cuts[atomicAdd(&s_cuts, 1)] = w;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      Header h = head;
+      h.cuts = s_cuts;
+      *p.head = h;
+    }
+  }
   if (share >= head.shares || total == 0) return;
   const int x0 = share_begin(head, share), x1 = share_begin(head, share + 1);
   if (before <= x0 && x0 < before + local) {
     Item w = few_item(p, i0, before);
     while (w.first + w.tiles <= x0) w = few_item(p, w.index + 1, w.first + w.tiles);
     s_start = w;
-    p.starts[share] = w;
-    if (share == 0) *p.head = head;
   }
   __syncthreads();
   const int unit = p.unit, hc = p.hc;
@@ -1360,7 +1401,7 @@ Plan plan(int N, int B, int max_q, int H, int Hk, int D) {
     pl.part_rows = 256;
   }
   pl.slots = 2 * pl.grid_cap;
-  pl.bytes = 256 + align256(sizeof(Item) * (size_t)pl.max_items) + align256(sizeof(Item) * (size_t)pl.grid_cap) +
+  pl.bytes = 256 + align256(sizeof(Item) * (size_t)pl.max_items) + 2 * align256(sizeof(Item) * (size_t)pl.grid_cap) +
              align256(sizeof(float) * (size_t)pl.slots * pl.part_rows * D) +
              align256(sizeof(float2) * (size_t)pl.slots * pl.part_rows);
   return pl;
@@ -1376,6 +1417,7 @@ void carve(Params& p, const Plan& pl, void* base, int D) {
   p.head = reinterpret_cast<Header*>(take(sizeof(Header)));
   p.items = reinterpret_cast<Item*>(take(sizeof(Item) * (size_t)pl.max_items));
   p.starts = reinterpret_cast<Item*>(take(sizeof(Item) * (size_t)pl.grid_cap));
+  p.cuts = reinterpret_cast<Item*>(take(sizeof(Item) * (size_t)pl.grid_cap));
   p.part_o = reinterpret_cast<float*>(take(sizeof(float) * (size_t)pl.slots * pl.part_rows * D));
   p.part_ml = reinterpret_cast<float2*>(take(sizeof(float2) * (size_t)pl.slots * pl.part_rows));
 }
@@ -1408,8 +1450,8 @@ int launch_dependent(void (*kernel)(Formal...), int grid, int threads, size_t sm
 }
 
 template <typename T, int D, bool ROWS32>
-int run_join(const Params& p, int chunks, int sms, cudaStream_t s) {
-  return launch_dependent(join_kernel<T, D, ROWS32, 8>, std::min(p.grid * chunks, 8 * sms), JOIN_THREADS, 0, s, p, chunks);
+int run_join(const Params& p, int sms, cudaStream_t s) {
+  return launch_dependent(join_kernel<T, D, ROWS32>, 4 * sms, JOIN_THREADS, 0, s, p);
 }
 
 template <typename T, int D, bool R16>
@@ -1423,7 +1465,7 @@ int run_few(Params& p, const Plan& pl, const CUtensorMap& tk, const CUtensorMap&
   p.grid = std::min(per_sm * sms, pl.grid_cap);
   few_rows_kernel<T, D, R16><<<p.grid, D_THREADS, smem, s>>>(tk, tv, p, stages, rows);
   MFB_LAUNCH_CHECK("paged attention (few rows)");
-  return run_join<T, D, false>(p, cdiv(pl.part_rows, 4), sms, s);
+  return run_join<T, D, false>(p, sms, s);
 }
 
 template <typename T, int D>
@@ -1454,7 +1496,7 @@ int run(Params& p, const Plan& pl, const void* q, const void* kp, const void* vp
   schedule_kernel<<<1, SCHED_THREADS, sizeof(int) * (size_t)(p.B + 1), s>>>(p);
   MFB_LAUNCH_CHECK("paged attention schedule");
   if ((st = launch_dependent(chunk_kernel<T, D>, p.grid, T_THREADS, smem, s, tq, tk, tv, p))) return st;
-  return run_join<T, D, true>(p, 16, sms, s);
+  return run_join<T, D, true>(p, sms, s);
 }
 
 }  // namespace paged
