@@ -19,8 +19,49 @@ def _per_row(x, rows, dtype, what, stream):
     return x.ptr, x
 
 
-def process_logits(logits, *, history=None, prompt_len=None, history_len=None, repetition=None, frequency=None,
-                   presence=None, bias_ids=None, bias_values=None, mask=None, mask_rows=None, out=None, stream=None):
+def prepare_controls(rows, vocab, *, history=None, prompt_len=None, history_len=None, repetition=None, frequency=None,
+                     presence=None, bias_ids=None, bias_values=None, mask=None, mask_rows=None, stream=None):
+    """The checked controls of ``process_logits`` for [rows, vocab] logits, on the device.
+
+    A caller that must know before its own work that they will be taken checks
+    them here, then passes the result on as ``controls``.
+    """
+    capacity = biases = masks = 0
+    if history is not None:
+        history = as_device(history, "int32", stream)
+        if history.ndim != 2 or history.shape[0] != rows:
+            raise ValueError("history must be [rows, tokens]")
+        capacity = history.shape[1]
+        if capacity >= 1 << 20:
+            raise ValueError(f"history of {capacity} tokens unsupported (0 to {(1 << 20) - 1})")
+    elif any(x is not None for x in (prompt_len, history_len, repetition, frequency, presence)):
+        raise ValueError("penalties and lengths need a history")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values must both be given or both be None")
+    if bias_ids is not None:
+        bias_ids, bias_values = as_device(bias_ids, "int32", stream), as_device(bias_values, "float32", stream)
+        if bias_ids.ndim != 2 or bias_ids.shape[0] != rows or bias_values.shape != bias_ids.shape:
+            raise ValueError("bias_ids and bias_values must be [rows, entries]")
+        biases = bias_ids.shape[1]
+        if biases > 2047:
+            raise ValueError(f"{biases} bias entries unsupported (0 to 2047)")
+    if mask is not None:
+        mask = as_device(mask, "int32", stream)
+        if mask.ndim != 2 or mask.shape[1] != (vocab + 31) // 32:
+            raise ValueError("mask must be [grammars, ceil(vocab / 32)]")
+        masks = mask.shape[0]
+        if mask_rows is None and masks < rows:
+            raise ValueError("a mask without mask_rows needs one row per logits row")
+    elif mask_rows is not None:
+        raise ValueError("mask_rows needs a mask")
+    held = [_per_row(x, rows, t, what, stream) for x, t, what in (
+        (prompt_len, "int32", "prompt_len"), (history_len, "int32", "history_len"),
+        (repetition, "float32", "repetition"), (frequency, "float32", "frequency"),
+        (presence, "float32", "presence"), (mask_rows, "int32", "mask_rows"))]
+    return rows, vocab, history, capacity, held, bias_ids, bias_values, biases, mask, masks
+
+
+def process_logits(logits, *, out=None, stream=None, controls=None, **kwargs):
     """float32 [rows, vocab] logits under the rows' controls, each optional.
 
     ``history`` (int32 [rows, n]) holds each row's token ids: the first
@@ -37,6 +78,7 @@ def process_logits(logits, *, history=None, prompt_len=None, history_len=None, r
       row's grammar (default: row i's is i); an index outside leaves it free.
 
     ``logits`` are bfloat16, float16 or float32; float32 logits may be ``out``.
+    ``controls`` are ``prepare_controls``' in place of these arguments.
     """
     if not isinstance(logits, DeviceArray):
         logits = as_device(logits, "float32", stream)
@@ -44,34 +86,13 @@ def process_logits(logits, *, history=None, prompt_len=None, history_len=None, r
         raise ValueError("logits must be [rows, vocab] in bfloat16, float16 or float32")
     rows, vocab = logits.shape
     out = check_out(out, (rows, vocab), "float32", "out")
-    capacity = biases = masks = 0
-    if history is not None:
-        history = as_device(history, "int32", stream)
-        if history.ndim != 2 or history.shape[0] != rows:
-            raise ValueError("history must be [rows, tokens]")
-        capacity = history.shape[1]
-    elif any(x is not None for x in (prompt_len, history_len, repetition, frequency, presence)):
-        raise ValueError("penalties and lengths need a history")
-    if (bias_ids is None) != (bias_values is None):
-        raise ValueError("bias_ids and bias_values must both be given or both be None")
-    if bias_ids is not None:
-        bias_ids, bias_values = as_device(bias_ids, "int32", stream), as_device(bias_values, "float32", stream)
-        if bias_ids.ndim != 2 or bias_ids.shape[0] != rows or bias_values.shape != bias_ids.shape:
-            raise ValueError("bias_ids and bias_values must be [rows, entries]")
-        biases = bias_ids.shape[1]
-    if mask is not None:
-        mask = as_device(mask, "int32", stream)
-        if mask.ndim != 2 or mask.shape[1] != (vocab + 31) // 32:
-            raise ValueError("mask must be [grammars, ceil(vocab / 32)]")
-        masks = mask.shape[0]
-        if mask_rows is None and masks < rows:
-            raise ValueError("a mask without mask_rows needs one row per logits row")
-    elif mask_rows is not None:
-        raise ValueError("mask_rows needs a mask")
-    held = [_per_row(x, rows, t, what, stream) for x, t, what in (
-        (prompt_len, "int32", "prompt_len"), (history_len, "int32", "history_len"),
-        (repetition, "float32", "repetition"), (frequency, "float32", "frequency"),
-        (presence, "float32", "presence"), (mask_rows, "int32", "mask_rows"))]
+    if controls is None:
+        controls = prepare_controls(rows, vocab, stream=stream, **kwargs)
+    elif kwargs:
+        raise TypeError("prepared controls take no further arguments")
+    r, v, history, capacity, held, bias_ids, bias_values, biases, mask, masks = controls
+    if (r, v) != (rows, vocab):
+        raise ValueError(f"controls were prepared for [{r}, {v}] logits")
     pl, hl, rep, freq, pres, mr = (x[0] if x is not None else None for x in held)
     if rows and vocab:
         _lib.call("mfb_logits_process", logits.ptr, DTYPE_CODES[logits.dtype],
@@ -82,4 +103,4 @@ def process_logits(logits, *, history=None, prompt_len=None, history_len=None, r
     return out
 
 
-__all__ = ["process_logits"]
+__all__ = ["prepare_controls", "process_logits"]

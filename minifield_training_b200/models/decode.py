@@ -29,6 +29,19 @@ at its own length here. Decode, per block:
   then       residual + RMSNorm (one kernel) -> fused w1|w3 GEMM -> SwiGLU ->
              w2 GEMM, the residual folded into the next block's norm.
 
+``Decoder.extend`` runs a chunk of one or more tokens per row over a
+``PagedState``, whose rows keep their keys and values in pages of a pool shared
+by all rows (and have lengths of their own): per attention block the q/k norm,
+rotation and append are one pass (kernels.paged.paged_append) and the chunk
+attends to the pages (paged_attention). A prompt is prefilled by one call or by
+several chunks; one token per row is a decode step. The rotation's angles and
+the norms are FP32, rounded once, so logits differ from the fixed-capacity
+path's, which rounds step by step as the reference does, by bf16 roundings.
+
+``controls`` of ``decode_one`` and ``extend`` (penalties, biases, grammar masks:
+the keyword arguments of kernels.logits.process_logits) are applied in the pass
+that widens the logits.
+
 The masters are cast to bf16 once at construction (full_linear's cast,
 kernels/linear.py:11); the q|k|v and w1|w3 products are single GEMMs over
 concatenated rows.
@@ -40,6 +53,8 @@ import numpy as np
 
 from .. import _lib
 from ..device import DeviceArray
+from ..kernels import logits as logit_controls
+from ..kernels import paged
 from .encoder import _fwd, rope_freqs
 
 P = ctypes.c_void_p
@@ -114,6 +129,74 @@ def new_state(cfg, batch_size: int, capacity: int) -> DecodeState:
     return DecodeState(cfg, batch_size, capacity)
 
 
+class PagedState:
+    """Rows over a shared pool of pages (no counterpart in the reference).
+
+    Every attention layer has a ``paged.PagedCache`` of ``num_pages`` pages of
+    ``page_size`` tokens; a row takes pages as it grows, the same ones in every
+    layer, up to ``max_pages`` (default: the whole pool), and gives them back on
+    ``release``. ``lengths`` holds each row's tokens; ``history`` the conv
+    layers' two preceding inputs per row.
+    """
+
+    def __init__(self, cfg, batch_size: int, num_pages: int, page_size: int = 64, max_pages: int | None = None):
+        for name, n in (("batch_size", batch_size), ("num_pages", num_pages), ("page_size", page_size),
+                        ("max_pages", 1 if max_pages is None else max_pages)):
+            if isinstance(n, bool) or not isinstance(n, int) or n <= 0:
+                raise ValueError(f"{name} must be a positive integer")
+        if page_size < 8 or page_size & (page_size - 1):
+            raise ValueError("page_size must be a power of two of at least 8")
+        self.cfg, self.batch, self.page_size, self.num_pages = cfg, batch_size, page_size, num_pages
+        self.max_pages = min(max_pages or num_pages, num_pages)
+        self.lengths = [0] * batch_size
+        self.table = np.full((batch_size, self.max_pages), -1, np.int32)
+        self._free = list(range(num_pages - 1, -1, -1))
+        self.caches, self.history = [], []
+        for kind in cfg.layer_types:
+            if kind == "full_attention":
+                self.caches.append(paged.PagedCache.zeros(num_pages, page_size, cfg.kv_heads, cfg.head_dim))
+                self.history.append(None)
+            else:
+                self.caches.append(None)
+                self.history.append(DeviceArray.zeros((batch_size, cfg.conv_kernel - 1, cfg.hidden), "bfloat16"))
+        _lib.call("mfb_stream_sync", None)  # any stream may use the pool from here on
+
+    def pages(self, tokens: int) -> int:
+        """Pages that hold ``tokens`` tokens of a row."""
+        return -(-tokens // self.page_size)
+
+    def grow(self, rows, tokens: int) -> None:
+        """Takes the pages for ``tokens`` more tokens of each of ``rows``, or none at all (DecodeOverflow)."""
+        need = []
+        for row in rows:
+            total = self.lengths[row] + tokens
+            if total > self.cfg.max_position_embeddings:
+                raise ValueError("Logical length exceeds model max_position_embeddings")
+            if self.pages(total) > self.max_pages:
+                raise DecodeOverflow(f"Row {row} needs {self.pages(total)} pages of {self.page_size} tokens; "
+                                     f"it may take {self.max_pages}")
+            need.append(self.pages(total) - self.pages(self.lengths[row]))
+        if sum(need) > len(self._free):
+            raise DecodeOverflow(f"{sum(need)} pages needed, {len(self._free)} of {self.num_pages} free")
+        for row, count in zip(rows, need):
+            held = self.pages(self.lengths[row])
+            self.table[row, held:held + count] = [self._free.pop() for _ in range(count)]
+            self.lengths[row] += tokens
+
+    def release(self, row: int) -> None:
+        """Empties ``row`` for a new sequence: its pages go back to the pool."""
+        if isinstance(row, bool) or not isinstance(row, int) or not 0 <= row < self.batch:
+            raise ValueError(f"row {row} outside the batch of {self.batch}")
+        self._free.extend(int(p) for p in self.table[row, :self.pages(self.lengths[row])][::-1])
+        self.table[row] = -1
+        self.lengths[row] = 0
+
+
+def new_paged_state(cfg, batch_size: int, num_pages: int, page_size: int = 64, max_pages: int | None = None):
+    """An empty PagedState of ``batch_size`` rows over ``num_pages`` pages of ``page_size`` tokens."""
+    return PagedState(cfg, batch_size, num_pages, page_size, max_pages)
+
+
 class Decoder:
     """Device weights of the decoder and the single-token step over a DecodeState."""
 
@@ -159,7 +242,7 @@ class Decoder:
                 L["kn"] = f32(parameters[p + "self_attn.k_layernorm.weight"])
             self.layers.append(L)
         _lib.call("mfb_device_sync")
-        self._scratch, self._graphs, self._prefill_scratch = {}, {}, {}
+        self._scratch, self._graphs, self._prefill_scratch, self._extend_scratch = {}, {}, {}, {}
 
     def _buffers(self, batch: int, capacity: int):
         key = (batch, capacity)
@@ -299,7 +382,133 @@ class Decoder:
         state.valid_length = t
         return logits
 
-    def decode_one(self, input_ids, state: DecodeState, *, out=None, graph: bool = False):
+    def extend(self, input_ids, state: PagedState, *, rows=None, controls=None, out=None):
+        """FP32 logits [R, vocab] after the last of T new tokens per row; fills pages and advances the state.
+
+        ``input_ids`` [R, T] int32 continue ``rows`` (a range of state rows, all
+        by default), each at its own length: a prompt or a part of one, or one
+        decoded token. DecodeOverflow when the pool or a row's table is full,
+        like any other refusal, comes before anything runs and leaves the state
+        as it was. ``controls``: keyword arguments of
+        kernels.logits.process_logits for the returned logits. ``out`` (a
+        float32 [R, vocab] DeviceArray) receives them.
+        """
+        cfg, s = self.cfg, self.stream
+        if state.cfg != cfg:
+            raise ValueError("Decode state does not match the decoder config")
+        rows = range(state.batch) if rows is None else rows
+        if not isinstance(rows, range) or rows.step != 1 or not rows or rows.start < 0 or rows.stop > state.batch:
+            raise ValueError(f"rows must be a non-empty range of step 1 within the {state.batch} rows of the state")
+        ids = np.asarray(input_ids)
+        if ids.ndim != 2 or ids.shape[0] != len(rows) or ids.shape[1] <= 0:
+            raise ValueError("extend input_ids must have shape [rows, tokens] matching the rows of the state")
+        b, t = ids.shape
+        if out is not None and (tuple(out.shape) != (b, cfg.vocab) or out.dtype != "float32"):
+            raise ValueError("out must be a float32 [rows, vocab] device array")
+        controls = self._controls(controls, b)
+        fresh = [row for row in rows if state.lengths[row] == 0]
+        state.grow(rows, t)
+        c, f, h, hk, hd = cfg.hidden, cfg.ffn, cfg.heads, cfg.kv_heads, cfg.head_dim
+        m, nq, r0, r1 = b * t, (h + 2 * hk) * hd, rows.start, rows.stop
+        B = self._extend_buffers(b, t, state.max_pages)
+        meta = np.concatenate([ids.reshape(-1).astype(np.int32), np.arange(b + 1, dtype=np.int32) * t,
+                               np.asarray(state.lengths[r0:r1], np.int32), state.table[r0:r1].reshape(-1)])
+        _lib.call("mfb_memcpy_h2d", P(B["meta"].ptr), meta.ctypes.data_as(P), meta.nbytes, s)
+        ids_d, cu = B["meta"].view(0, (m,)), B["meta"].view(m, (b + 1,))
+        lens, table = B["meta"].view(m + b + 1, (b,)), B["meta"].view(m + 2 * b + 1, (b, state.max_pages))
+
+        def proj(x, w, y, n, k):
+            if m <= 64:
+                self._proj(x, w, y, m, n, k, B)
+            else:
+                _fwd(x, w, y, m, n, k, s)
+
+        x, spare, prev_mid, prev_y = B["x"], B["xb"], None, None
+        _lib.call("mfb_embed_gather", P(self.embed.ptr), P(ids_d.ptr), P(x.ptr), m, c, cfg.vocab, s)
+        for i, L in enumerate(self.layers):
+            if prev_mid is None:
+                self._rms(x, None, L["op_norm"], None, B["hn"], B["rstd"], m)
+            else:
+                self._rms(prev_mid, prev_y, L["op_norm"], x, B["hn"], B["rstd"], m)
+            if L["kind"] == "conv":
+                proj(B["hn"], L["w_in"], B["proj"], 3 * c, c)
+                nbytes = state.history[i].nbytes // state.batch
+                history = state.history[i].ptr + r0 * nbytes
+                for row in fresh:
+                    _lib.call("mfb_memset", P(history + (row - r0) * nbytes), 0, nbytes, s)
+                if t == 1:
+                    _lib.call("mfb_conv_step", P(B["proj"].ptr), P(L["taps"].ptr), P(history), P(B["mixed"].ptr),
+                              b, c, s)
+                else:  # the tail it leaves must not alias the history it starts from
+                    _lib.call("mfb_conv_causal", P(B["proj"].ptr), P(L["taps"].ptr), P(history), P(B["tail"].ptr),
+                              P(B["mixed"].ptr), b, t, c, s)
+                    _lib.call("mfb_memcpy_d2d", P(history), P(B["tail"].ptr), b * nbytes, s)
+                proj(B["mixed"], L["w_out"], B["r"], c, c)
+            else:
+                proj(B["hn"], L["w_in"], B["proj"], nq, c)
+                qkv, q, o = B["proj"].view(0, (m, nq)), B["q"].view(0, (m, h, hd)), B["o"].view(0, (m, h, hd))
+                paged.paged_append(qkv, state.caches[i], cu, lens, table, heads=h, freqs=self.freqs,
+                                   q_weight=L["qn"], k_weight=L["kn"], eps=cfg.norm_eps, out=q, stream=s)
+                paged.paged_attention(q, state.caches[i], cu, lens, table, max_q=t, out=o, workspace=B["ws"],
+                                      stream=s)
+                proj(B["o"], L["w_out"], B["r"], c, h * hd)
+            self._rms(x, B["r"], L["ffn_norm"], B["mid"], B["h2"], B["rstd"], m)
+            proj(B["h2"], L["w13"], B["gu"], 2 * f, c)
+            _lib.call("mfb_swiglu_fwd", P(B["gu"].ptr), P(B["a"].ptr), m, f, s)
+            proj(B["a"], L["w2"], B["y"], c, f)
+            prev_mid, prev_y = B["mid"], B["y"]
+            x, spare = spare, x
+        self._rms(prev_mid, prev_y, self.final_norm, x, B["enc"], B["rstd"], m)
+        # Logits of the last token of every row.
+        _lib.call("mfb_memcpy2d_d2d", P(B["last"].ptr), c * 2, P(B["enc"].ptr + (t - 1) * c * 2), t * c * 2, c * 2,
+                  b, s)
+        if b <= 64:
+            self._proj(B["last"], self.head, B["logits16"], b, cfg.vocab, c, B)
+        else:
+            _fwd(B["last"], self.head, B["logits16"], b, cfg.vocab, c, s)
+        logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")
+        return self._widen(B["logits16"], logits, controls)
+
+    def _extend_buffers(self, b: int, t: int, max_pages: int):
+        """Scratch of ``extend`` for b x t tokens, kept per batch, power of two that holds t, and table width."""
+        cfg, E = self.cfg, DeviceArray
+        c, f, h, hk, hd = cfg.hidden, cfg.ffn, cfg.heads, cfg.kv_heads, cfg.head_dim
+        bucket = 1 << (t - 1).bit_length()
+        key, n, nq = (b, bucket, max_pages), b * bucket, (h + 2 * hk) * hd
+        B = self._extend_scratch.get(key)
+        if B is None:
+            def bf(cols, rows=n):
+                return E((rows, cols), "bfloat16")
+
+            size = _lib.lib().mfb_gemm_workspace_size
+            gemm = [int(size(min(n, 64), w, k)) for w, k in (
+                (3 * c, c), (c, c), (nq, c), (c, h * hd), (2 * f, c), (c, f))]
+            gemm.append(int(size(min(b, 64), cfg.vocab, c)))
+            B = self._extend_scratch[key] = dict(
+                meta=E((n + 2 * b + 1 + b * max_pages,), "int32"), x=bf(c), xb=bf(c), hn=bf(c),
+                proj=E((n * max(3 * c, nq),), "bfloat16"), mixed=bf(c), tail=bf((cfg.conv_kernel - 1) * c, b),
+                r=bf(c), mid=bf(c), h2=bf(c), gu=bf(2 * f), a=bf(f), y=bf(c), q=bf(h * hd), o=bf(h * hd),
+                rstd=E((n,), "float32"), enc=bf(c), last=bf(c, b), logits16=bf(cfg.vocab, b),
+                gemm_ws=E((max(*gemm, 16),), "uint8"), ws=E((16,), "uint8"))
+        need = paged.paged_attention_workspace_size(b * t, b, t, h, hk, hd)
+        if B["ws"].nbytes < need:
+            B["ws"] = E((need,), "uint8")
+        return B
+
+    def _controls(self, controls, rows: int):
+        """Checked controls, before the state changes."""
+        if not controls:
+            return None
+        return logit_controls.prepare_controls(rows, self.cfg.vocab, stream=self.stream, **controls)
+
+    def _widen(self, logits16, logits, controls):
+        """FP32 ``logits`` of the bf16 ones, under ``controls`` when given."""
+        if controls is not None:
+            return logit_controls.process_logits(logits16, out=logits, stream=self.stream, controls=controls)
+        _lib.call("mfb_cast_bf16_f32", P(logits16.ptr), P(logits.ptr), logits.size, self.stream)
+        return logits
+
+    def decode_one(self, input_ids, state: DecodeState, *, out=None, graph: bool = False, controls=None):
         """FP32 logits [B, vocab] of the next token for each row; writes the caches and advances the state.
 
         ``out`` (a float32 [B, vocab] DeviceArray) receives the logits instead
@@ -307,7 +516,8 @@ class Decoder:
         captured on the first call for this state's caches (needs a created
         stream); the step reads its token ids, positions and lengths from
         device buffers uploaded before each replay, so one graph serves every
-        step.
+        step. ``controls``: keyword arguments of kernels.logits.process_logits
+        for the returned logits.
         """
         cfg, s = self.cfg, self.stream
         if state.cfg != cfg:
@@ -326,6 +536,7 @@ class Decoder:
             raise ValueError("out must be a float32 [batch, vocab] device array")
         if graph and not s:
             raise ValueError("graph replay needs Decoder(stream=...) from mfb_stream_create")
+        controls = self._controls(controls, b)
         B = self._buffers(b, state.capacity)
         pos = state.valid_length
         meta = np.ascontiguousarray(np.stack([ids, np.full(b, pos, np.int32), np.full(b, pos + 1, np.int32)]))
@@ -344,9 +555,12 @@ class Decoder:
                     _lib.call("mfb_graph_end", P(s), ctypes.byref(g_))
                 g = self._graphs[key] = g_.value
             _lib.call("mfb_graph_launch", P(g), P(s))
-            _lib.call("mfb_memcpy_d2d", P(logits.ptr), P(B["logits"].ptr), logits.nbytes, s)
+            if controls is None:
+                _lib.call("mfb_memcpy_d2d", P(logits.ptr), P(B["logits"].ptr), logits.nbytes, s)
         else:
-            self._step(B, state, logits)
+            self._step(B, state, logits if controls is None else None)
+        if controls is not None:
+            self._widen(B["logits16"], logits, controls)
         state.valid_length = pos + 1
         return logits
 
@@ -386,7 +600,8 @@ class Decoder:
             x = B["xb"] if x is B["x"] else B["x"]  # the next block's input buffer (ping-pong)
         self._rms(prev_mid, prev_y, self.final_norm, x, B["enc"], B["rstd"], b)
         self._proj(B["enc"], self.head, B["logits16"], b, cfg.vocab, c, B)
-        _lib.call("mfb_cast_bf16_f32", P(B["logits16"].ptr), P(logits.ptr), b * cfg.vocab, s)
+        if logits is not None:
+            _lib.call("mfb_cast_bf16_f32", P(B["logits16"].ptr), P(logits.ptr), b * cfg.vocab, s)
 
     def close(self):
         """Release the captured decode graphs."""
@@ -412,5 +627,10 @@ def decode_one(decoder: Decoder, input_ids, state: DecodeState):
     return decoder.decode_one(input_ids, state), state
 
 
-__all__ = ["DecodeOverflow", "DecodeState", "Decoder", "decode_one", "init_parameters", "new_state", "prefill",
-           "parameter_shapes"]
+def extend(decoder: Decoder, input_ids, state: PagedState, *, rows=None, controls=None):
+    """``(logits, state)`` of ``Decoder.extend``."""
+    return decoder.extend(input_ids, state, rows=rows, controls=controls), state
+
+
+__all__ = ["DecodeOverflow", "DecodeState", "Decoder", "PagedState", "decode_one", "extend", "init_parameters",
+           "new_paged_state", "new_state", "prefill", "parameter_shapes"]
