@@ -441,8 +441,9 @@ int mfb_paged_append(const void* qkv, int ld_qkv, const float* wq, const float* 
  * it). Device arguments that contradict each other (cu_q outside [0, N], more
  * than max_q new tokens, lengths outside the table, a used page id outside the
  * pool: read as zeros) are clamped and recorded in the status word, never
- * followed out of the buffers. The workspace holds the schedule and the
- * partials; calls that share one must not overlap. */
+ * followed out of the buffers. scale is positive. Sequences x KV heads x query
+ * blocks x key tiles of the whole table stay below 2^31. The workspace holds the
+ * schedule and the partials; calls that share one must not overlap. */
 size_t mfb_paged_attn_workspace_size(int N, int B, int max_q, int H, int Hk, int D);
 int mfb_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* cu_q,
                    const int32_t* seq_lens, const int32_t* page_table, void* o, float* lse, int N, int B, int max_q,

@@ -1377,8 +1377,14 @@ constexpr int FEW_ROWS = 16;  // query rows per KV head the warp-level kernel ta
 
 struct Plan {
   bool few;
-  int hc, unit, tok_item, grid_cap, max_items, part_rows, slots;
+  int hc, unit, tok_item, grid_cap, part_rows, slots;
+  long long max_items;  // listed items
   size_t bytes;
+  // The items' total weight is counted in 32 bits: its bound for a table of `span` positions per sequence.
+  double max_weight(int B, int Hk, long long span) const {
+    const double units = (double)((span + unit - 1) / unit);
+    return few ? (double)B * (Hk / hc) * units : 2.0 * max_items * units;
+  }
 };
 
 Plan plan(int N, int B, int max_q, int H, int Hk, int D) {
@@ -1397,7 +1403,7 @@ Plan plan(int N, int B, int max_q, int H, int Hk, int D) {
     pl.unit = 128;
     pl.tok_item = 2 * (128 / G);
     pl.grid_cap = MAX_SMS;
-    pl.max_items = Hk * (N / pl.tok_item + B);
+    pl.max_items = (long long)Hk * (N / pl.tok_item + B);
     pl.part_rows = 256;
   }
   pl.slots = 2 * pl.grid_cap;
@@ -1531,7 +1537,11 @@ extern "C" int mfb_paged_attn(const void* q, const void* k_pages, const void* v_
   MFB_CHECK_ARG(q && k_pages && v_pages && cu_q && seq_lens && page_table && o, "NULL paged attention argument");
   MFB_CHECK_ARG((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o) & 15) == 0,
                 "q, the pages and o must be 16-byte aligned");
+  MFB_CHECK_ARG(isfinite(scale) && scale > 0.f, "paged attention scale must be positive and finite");
   const paged::Plan pl = paged::plan(N, B, max_q, H, Hk, D);
+  MFB_CHECK_ARG(pl.max_weight(B, Hk, (long long)max_pages * page_size) < 2147483647.0,
+                "paged attention of %d tokens over tables of %lld positions exceeds 2^31 key tiles", N,
+                (long long)max_pages * page_size);
   if (!workspace || workspace_bytes < pl.bytes)
     return set_error(MFB_ERR_WORKSPACE, "paged attention workspace needs %zu bytes", pl.bytes);
   MFB_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");
@@ -1554,7 +1564,7 @@ extern "C" int mfb_paged_attn(const void* q, const void* k_pages, const void* v_
   p.tok_item = pl.tok_item;
   p.hc = pl.hc;
   p.unit = pl.unit;
-  p.max_items = pl.max_items;
+  p.max_items = (int)pl.max_items;
   p.part_rows = pl.part_rows;
   p.scale_log2 = scale * kLog2e;
   paged::carve(p, pl, workspace, D);

@@ -89,7 +89,7 @@ def paged_attention(q, cache: PagedCache, cu_q, seq_lens, page_table, *, max_q, 
     Causal: the i-th of a sequence's n new tokens sees its first
     ``seq_lens[b] - n + i + 1`` tokens; one that sees none gets zeros. ``max_q``
     is an upper bound of any sequence's new tokens (1 in a decode step).
-    ``scale`` defaults to head_dim ** -0.5. ``lse`` (float32 [N, heads], optional) receives the
+    ``scale`` (positive) defaults to head_dim ** -0.5. ``lse`` (float32 [N, heads], optional) receives the
     natural log-sum-exp of the scaled scores. Calls on one ``workspace``
     (``paged_attention_workspace_size`` bytes) must not overlap; the default
     one belongs to the stream, and a captured call needs its own.

@@ -144,6 +144,13 @@ def attention_call(**kw):
     (dict(lse=fake((4, 8), "float32")), "lse must be"),
     (dict(q=fake((4, 16, 64), "bfloat16", ptr=(1 << 20) + 2)), "16-byte aligned"),
     (dict(table=fake((2, 1 << 28), "int32")), "positions"),
+    (dict(scale=0.0), "positive and finite"),
+    (dict(scale=-0.125), "positive and finite"),
+    (dict(scale=float("nan")), "positive and finite"),
+    (dict(cu_q=fake((8001,), "int32"), seq_lens=fake((8000,), "int32"), table=fake((8000, 1 << 20), "int32")),
+     "exceeds 2"),
+    (dict(table=fake((2, 1 << 26), "int32"), q=fake((1 << 20, 16, 64), "bfloat16"), max_q=1 << 19,
+          out=fake((1 << 20, 16, 64), "bfloat16")), "exceeds 2"),
     (dict(cache=paged.PagedCache(*[fake((9, 16, 8, 32), "bfloat16")] * 2), q=fake((4, 16, 32), "bfloat16"),
           out=fake((4, 16, 32), "bfloat16")), "head_dim 32"),
 ])
@@ -208,3 +215,30 @@ def test_workspace_sizes_cover_odd_shapes():
     flag = ctypes.c_int(5)
     assert _lib.lib().mfb_stream_is_capturing(None, None) == _lib.ERR_INVALID
     assert flag.value == 5
+
+
+@pytest.mark.parametrize("kw, match", [
+    (dict(batch_size=0), "batch_size"),
+    (dict(num_pages=-1), "num_pages"),
+    (dict(num_pages=True), "num_pages"),
+    (dict(page_size=12), "power of two"),
+    (dict(page_size=4), "power of two"),
+    (dict(max_pages=0), "max_pages"),
+])
+def test_paged_state_refuses(kw, match):
+    from minifield_training_b200 import workloads
+    from minifield_training_b200.models import decode
+    with pytest.raises(ValueError, match=match):
+        decode.new_paged_state(workloads.DECODER, **{**dict(batch_size=2, num_pages=4), **kw})
+
+
+def test_prepared_controls_refuse():
+    with pytest.raises(ValueError, match="history must be"):
+        lg.prepare_controls(2, 100, history=fake((3, 8), "int32"))
+    ready = lg.prepare_controls(2, 100, history=fake((2, 8), "int32"))
+    logits, out = fake((3, 100), "bfloat16"), fake((3, 100), "float32")
+    with pytest.raises(ValueError, match="prepared for"):
+        lg.process_logits(logits, out=out, controls=ready)
+    with pytest.raises(TypeError, match="no further"):
+        lg.process_logits(fake((2, 100), "bfloat16"), out=fake((2, 100), "float32"), controls=ready,
+                          mask=fake((2, 4), "int32"))
