@@ -474,6 +474,20 @@ int mfb_logits_process(const void* logits, int dtype, const int32_t* history, in
                        const float* bias_values, int bias_count, const uint32_t* mask, const int32_t* mask_rows,
                        int mask_count, float* out, int B, int V, void* stream);
 
+/* ---- Packed calls ----------------------------------------------------------------
+ * The same entry points with their arguments in one block of 8-byte slots, for
+ * callers whose foreign calls cost by the argument: slot 0 holds flags, slot 1 +
+ * i argument i of the plain entry point (pointers and size_t unsigned, integers
+ * signed and within their parameter's range, floats as doubles).
+ * MFB_PACKED_SHARED_WORKSPACE: the workspace is shared with later calls, so a
+ * call on a capturing stream is refused (MFB_ERR_INVALID). */
+enum mfb_packed_flags { MFB_PACKED_SHARED_WORKSPACE = 1 };
+int mfb_qk_rotary_fwd_packed(const void* slots);
+int mfb_qk_rotary_bwd_packed(const void* slots);
+int mfb_paged_append_packed(const void* slots);
+int mfb_paged_attn_packed(const void* slots);
+int mfb_logits_process_packed(const void* slots);
+
 /* ---- NCCL communicator (data-parallel exchange) -------------------------------
  * The psum of (loss, count, gradient tree) over the data axis of the
  * reference's training step (src/minifield_training/engine/step.py:36-78,

@@ -9,6 +9,7 @@ everything else -> RuntimeError.
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmfb200.so")
@@ -122,7 +123,17 @@ SIGNATURES = {
     "mfb_paged_attn": (I, [P] * 8 + [I] * 11 + [F, P, SZ, P]),
     "mfb_paged_attn_status": (I, [IP]),
     "mfb_logits_process": (I, [P, I, P, I] + [P] * 7 + [I, P, P, I, P, I, I, P]),
+    "mfb_qk_rotary_fwd_packed": (I, [ctypes.c_char_p]),
+    "mfb_qk_rotary_bwd_packed": (I, [ctypes.c_char_p]),
+    "mfb_paged_append_packed": (I, [ctypes.c_char_p]),
+    "mfb_paged_attn_packed": (I, [ctypes.c_char_p]),
+    "mfb_logits_process_packed": (I, [ctypes.c_char_p]),
 }
+PACKED_SHARED_WORKSPACE = 1
+# Slot formats of the packed entry points: flags, then the plain one's arguments.
+_SLOTS = {P: "Q", SZ: "Q", I: "q", LL: "q", F: "d"}
+_PACK = {name: struct.Struct("=q" + "".join(_SLOTS[a] for a in SIGNATURES[name][1])).pack
+         for name in (n[:-len("_packed")] for n in SIGNATURES if n.endswith("_packed"))}
 
 _lib = None
 
@@ -161,4 +172,13 @@ def check(status: int, what: str = "") -> None:
 
 def call(name: str, *args):
     """Call ``name`` and raise on a nonzero status."""
-    check(getattr(lib(), name)(*args), name)
+    status = getattr(_lib or lib(), name)(*args)
+    if status:
+        check(status, name)
+
+
+def call_packed(name: str, flags: int, *args, stream=None):
+    """``call`` with the arguments (0 for a NULL pointer) in one block: 1 us of conversion instead of 5."""
+    status = getattr(_lib or lib(), name + "_packed")(_PACK[name](flags, *args, getattr(stream, "value", stream) or 0))
+    if status:
+        check(status, name)

@@ -145,7 +145,7 @@ class DeviceArray:
 def as_device(x, dtype, stream=None) -> DeviceArray:
     """Return ``x`` as a DeviceArray of ``dtype`` (uploading host arrays)."""
     if isinstance(x, DeviceArray):
-        if x.dtype != _canon(dtype):
+        if x.dtype != dtype and x.dtype != _canon(dtype):
             raise TypeError(f"expected {dtype} device array, got {x.dtype}")
         return x
     return DeviceArray.from_numpy(np.asarray(x), dtype, stream)
@@ -207,16 +207,17 @@ _STREAM_WORKSPACES = {}
 def stream_workspace(tag: str, nbytes: int, stream=None) -> DeviceArray:
     """Grow-only scratch of one stream: calls on different streams never share it.
 
-    A call recorded into a CUDA graph is refused: the graph outlives the call
-    and may replay beside later ones, so it needs a workspace of its own.
+    A call recorded into a CUDA graph must not use it (the graph outlives the
+    call and may replay beside later ones): callers pass
+    ``PACKED_SHARED_WORKSPACE``, and growing is refused here.
     """
-    flag = ctypes.c_int()
-    _lib.call("mfb_stream_is_capturing", stream, ctypes.byref(flag))
-    if flag.value:
-        raise ValueError(f"a captured {tag} call needs its own workspace (workspace=)")
     key = (tag, getattr(stream, "value", stream))
     entry = _STREAM_WORKSPACES.get(key)
     if entry is None or entry[1] < nbytes:
+        flag = ctypes.c_int()
+        _lib.call("mfb_stream_is_capturing", stream, ctypes.byref(flag))
+        if flag.value:
+            raise ValueError(f"a captured {tag} call needs its own workspace (workspace=)")
         size = max(int(nbytes), 2 * entry[1] if entry else 256)
         entry = _STREAM_WORKSPACES[key] = (DeviceArray((size,), "uint8"), size)
     return entry[0]

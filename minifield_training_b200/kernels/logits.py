@@ -11,12 +11,15 @@ from .rotary import DTYPE_CODES, check_out
 
 
 def _per_row(x, rows, dtype, what, stream):
-    if x is None:
-        return None
-    x = as_device(x, dtype, stream)
-    if x.shape != (rows,):
-        raise ValueError(f"{what} must be [rows]")
-    return x.ptr, x
+    if x is not None:
+        x = as_device(x, dtype, stream)
+        if x.shape != (rows,):
+            raise ValueError(f"{what} must be [rows]")
+    return x
+
+
+def _ptr(x):
+    return x.ptr if x is not None else 0
 
 
 def prepare_controls(rows, vocab, *, history=None, prompt_len=None, history_len=None, repetition=None, frequency=None,
@@ -54,11 +57,12 @@ def prepare_controls(rows, vocab, *, history=None, prompt_len=None, history_len=
             raise ValueError("a mask without mask_rows needs one row per logits row")
     elif mask_rows is not None:
         raise ValueError("mask_rows needs a mask")
-    held = [_per_row(x, rows, t, what, stream) for x, t, what in (
-        (prompt_len, "int32", "prompt_len"), (history_len, "int32", "history_len"),
-        (repetition, "float32", "repetition"), (frequency, "float32", "frequency"),
-        (presence, "float32", "presence"), (mask_rows, "int32", "mask_rows"))]
-    return rows, vocab, history, capacity, held, bias_ids, bias_values, biases, mask, masks
+    return (rows, vocab, history, capacity, _per_row(prompt_len, rows, "int32", "prompt_len", stream),
+            _per_row(history_len, rows, "int32", "history_len", stream),
+            _per_row(repetition, rows, "float32", "repetition", stream),
+            _per_row(frequency, rows, "float32", "frequency", stream),
+            _per_row(presence, rows, "float32", "presence", stream), bias_ids, bias_values, biases, mask,
+            _per_row(mask_rows, rows, "int32", "mask_rows", stream), masks)
 
 
 def process_logits(logits, *, out=None, stream=None, controls=None, **kwargs):
@@ -90,16 +94,15 @@ def process_logits(logits, *, out=None, stream=None, controls=None, **kwargs):
         controls = prepare_controls(rows, vocab, stream=stream, **kwargs)
     elif kwargs:
         raise TypeError("prepared controls take no further arguments")
-    r, v, history, capacity, held, bias_ids, bias_values, biases, mask, masks = controls
-    if (r, v) != (rows, vocab):
+    (r, v, history, capacity, prompt_len, history_len, repetition, frequency, presence, bias_ids, bias_values, biases,
+     mask, mask_rows, masks) = controls
+    if r != rows or v != vocab:
         raise ValueError(f"controls were prepared for [{r}, {v}] logits")
-    pl, hl, rep, freq, pres, mr = (x[0] if x is not None else None for x in held)
     if rows and vocab:
-        _lib.call("mfb_logits_process", logits.ptr, DTYPE_CODES[logits.dtype],
-                  history.ptr if history is not None else None, capacity, pl, hl, rep, freq, pres,
-                  bias_ids.ptr if bias_ids is not None else None,
-                  bias_values.ptr if bias_values is not None else None, biases,
-                  mask.ptr if mask is not None else None, mr, masks, out.ptr, rows, vocab, stream)
+        _lib.call_packed("mfb_logits_process", 0, logits.ptr, DTYPE_CODES[logits.dtype], _ptr(history), capacity,
+                         _ptr(prompt_len), _ptr(history_len), _ptr(repetition), _ptr(frequency), _ptr(presence),
+                         _ptr(bias_ids), _ptr(bias_values), biases, _ptr(mask), _ptr(mask_rows), masks, out.ptr, rows,
+                         vocab, stream=stream)
     return out
 
 

@@ -10,6 +10,7 @@ as they were), and are the last of its ``seq_lens[b]`` tokens.
 """
 
 import ctypes
+import functools
 
 from .. import _lib
 from ..device import DeviceArray, as_device, stream_workspace
@@ -69,14 +70,15 @@ def paged_append(qkv, cache: PagedCache, cu_q, seq_lens, page_table, *, heads, f
     q = check_out(out, (n, heads, d), qkv.dtype, "out")
     b, max_pages = page_table.shape
     if n and b and max_pages and cache.num_pages:
-        _lib.call("mfb_paged_append", qkv.ptr, ld, wq.ptr if wq is not None else None,
-                  wk.ptr if wk is not None else None, freqs.ptr, cu_q.ptr, seq_lens.ptr, page_table.ptr, q.ptr,
+        _lib.call_packed("mfb_paged_append", 0, qkv.ptr, ld, wq.ptr if wq is not None else 0,
+                  wk.ptr if wk is not None else 0, freqs.ptr, cu_q.ptr, seq_lens.ptr, page_table.ptr, q.ptr,
                   cache.keys.ptr, cache.values.ptr, n, b, max_pages, cache.num_pages, cache.page_size, heads,
                   cache.kv_heads, d, 2 * freqs.shape[0], int(interleaved), int(cache.head_major),
-                  DTYPE_CODES[qkv.dtype], amplitude, eps, stream)
+                  DTYPE_CODES[qkv.dtype], amplitude, eps, stream=stream)
     return q
 
 
+@functools.lru_cache(maxsize=4096)
 def paged_attention_workspace_size(tokens, batch, max_q, heads, kv_heads, head_dim) -> int:
     """Bytes ``paged_attention`` needs for up to ``tokens`` new tokens, at most ``max_q`` of a sequence."""
     return int(_lib.lib().mfb_paged_attn_workspace_size(tokens, batch, max_q, heads, kv_heads, head_dim))
@@ -111,13 +113,14 @@ def paged_attention(q, cache: PagedCache, cu_q, seq_lens, page_table, *, max_q, 
         check_out(lse, (n, heads), "float32", "lse")
     b, max_pages = page_table.shape
     if n and b:
-        need = _lib.lib().mfb_paged_attn_workspace_size(n, b, max_q, heads, cache.kv_heads, d)
+        shared = 0
         if workspace is None:
-            workspace = stream_workspace("paged attention", need, stream)
-        _lib.call("mfb_paged_attn", q.ptr, cache.keys.ptr, cache.values.ptr, cu_q.ptr, seq_lens.ptr, page_table.ptr,
-                  out.ptr, lse.ptr if lse is not None else None, n, b, max_q, max_pages, cache.num_pages,
+            need = paged_attention_workspace_size(n, b, max_q, heads, cache.kv_heads, d)
+            workspace, shared = stream_workspace("paged attention", need, stream), _lib.PACKED_SHARED_WORKSPACE
+        _lib.call_packed("mfb_paged_attn", shared, q.ptr, cache.keys.ptr, cache.values.ptr, cu_q.ptr, seq_lens.ptr, page_table.ptr,
+                  out.ptr, lse.ptr if lse is not None else 0, n, b, max_q, max_pages, cache.num_pages,
                   cache.page_size, heads, cache.kv_heads, d, int(cache.head_major), DTYPE_CODES[q.dtype],
-                  d ** -0.5 if scale is None else float(scale), workspace.ptr, workspace.nbytes, stream)
+                  d ** -0.5 if scale is None else float(scale), workspace.ptr, workspace.nbytes, stream=stream)
     return out
 
 

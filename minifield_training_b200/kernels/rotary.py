@@ -9,6 +9,7 @@ once at the output; the reference's own 64-wide bf16 graph, rounded step by
 step, is ``mfb_qknorm_rope_fwd`` / ``_bwd`` (models.encoder).
 """
 
+import functools
 import math
 
 import numpy as np
@@ -98,13 +99,13 @@ def check_out(x, shape, dtype, what):
     """``x`` as an output of ``shape``; a new array where it is None."""
     if x is None:
         return DeviceArray(shape, dtype)
-    if x.dtype != dtype or tuple(x.shape) != tuple(shape):
-        raise ValueError(f"{what} must be a {dtype} device array of shape {tuple(shape)}")
+    if x.dtype != dtype or x.shape != shape:
+        raise ValueError(f"{what} must be a {dtype} device array of shape {shape}")
     return x
 
 
 def _ptr(x):
-    return x.ptr if x is not None else None
+    return x.ptr if x is not None else 0
 
 
 def qk_rotary_fwd(qkv, positions, freqs, *, heads, kv_heads, head_dim=None, interleaved=False, amplitude=1.0,
@@ -124,10 +125,15 @@ def qk_rotary_fwd(qkv, positions, freqs, *, heads, kv_heads, head_dim=None, inte
     k = check_out(k, (m, kv_heads, d), qkv.dtype, "k")
     v = check_out(v, (m, kv_heads, d), qkv.dtype, "v") if out is None or v is not None else None
     if m:
-        _lib.call("mfb_qk_rotary_fwd", qkv.ptr, ld, _ptr(wq), _ptr(wk), positions.ptr, freqs.ptr, q.ptr, k.ptr,
+        _lib.call_packed("mfb_qk_rotary_fwd", 0, qkv.ptr, ld, _ptr(wq), _ptr(wk), positions.ptr, freqs.ptr, q.ptr, k.ptr,
                   _ptr(v), m, heads, kv_heads, d, 2 * freqs.shape[0], int(interleaved), DTYPE_CODES[qkv.dtype],
-                  amplitude, eps, stream)
+                  amplitude, eps, stream=stream)
     return q, k, v
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace_size(head_dim):
+    return _lib.lib().mfb_qk_rotary_workspace_size(head_dim)
 
 
 def qk_rotary_bwd(qkv, positions, freqs, dq, dk, dv, *, head_dim=None, interleaved=False, amplitude=1.0,
@@ -156,16 +162,19 @@ def qk_rotary_bwd(qkv, positions, freqs, dq, dk, dv, *, head_dim=None, interleav
         raise ValueError("accumulate needs weight_grads to add to")
     dqkv = check_out(out, qkv.shape, qkv.dtype, "out")
     dwq = dwk = ws = None
+    shared = 0
     if wq is not None:
         dwq, dwk = weight_grads if weight_grads is not None else (None, None)
         dwq, dwk = check_out(dwq, (d,), "float32", "dq_weight"), check_out(dwk, (d,), "float32", "dk_weight")
-        need = _lib.lib().mfb_qk_rotary_workspace_size(d)
-        ws = workspace if workspace is not None else stream_workspace("rotary", need, stream)
+        if workspace is None:
+            ws, shared = stream_workspace("rotary", _workspace_size(d), stream), _lib.PACKED_SHARED_WORKSPACE
+        else:
+            ws = workspace
     if m:
-        _lib.call("mfb_qk_rotary_bwd", qkv.ptr, ld, _ptr(wq), _ptr(wk), positions.ptr, freqs.ptr, dq.ptr, dk.ptr,
+        _lib.call_packed("mfb_qk_rotary_bwd", shared, qkv.ptr, ld, _ptr(wq), _ptr(wk), positions.ptr, freqs.ptr, dq.ptr, dk.ptr,
                   dv.ptr, dqkv.ptr, _ptr(dwq), _ptr(dwk), int(accumulate), m, heads, kv_heads, d,
                   2 * freqs.shape[0], int(interleaved), DTYPE_CODES[qkv.dtype], amplitude, eps, _ptr(ws),
-                  ws.nbytes if ws is not None else 0, stream)
+                  ws.nbytes if ws is not None else 0, stream=stream)
     elif dwq is not None and not accumulate:
         for x in (dwq, dwk):
             _lib.call("mfb_memset", x.ptr, 0, x.nbytes, stream)
