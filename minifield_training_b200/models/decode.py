@@ -382,7 +382,7 @@ class Decoder:
         state.valid_length = t
         return logits
 
-    def extend(self, input_ids, state: PagedState, *, rows=None, controls=None, out=None):
+    def extend(self, input_ids, state: PagedState, *, rows=None, controls=None, out=None, graph: bool = False):
         """FP32 logits [R, vocab] after the last of T new tokens per row; fills pages and advances the state.
 
         ``input_ids`` [R, T] int32 continue ``rows`` (a range of state rows, all
@@ -391,7 +391,9 @@ class Decoder:
         like any other refusal, comes before anything runs and leaves the state
         as it was. ``controls``: keyword arguments of
         kernels.logits.process_logits for the returned logits. ``out`` (a
-        float32 [R, vocab] DeviceArray) receives them.
+        float32 [R, vocab] DeviceArray) receives them. ``graph=True`` replays a
+        single-token step (T = 1) as one CUDA graph, captured on the first call
+        for these rows of this state (needs a created stream).
         """
         cfg, s = self.cfg, self.stream
         if state.cfg != cfg:
@@ -405,15 +407,44 @@ class Decoder:
         b, t = ids.shape
         if out is not None and (tuple(out.shape) != (b, cfg.vocab) or out.dtype != "float32"):
             raise ValueError("out must be a float32 [rows, vocab] device array")
+        if graph and (not s or t != 1):
+            raise ValueError("graph replay takes single tokens and needs Decoder(stream=...) from mfb_stream_create")
         controls = self._controls(controls, b)
         fresh = [row for row in rows if state.lengths[row] == 0]
         state.grow(rows, t)
-        c, f, h, hk, hd = cfg.hidden, cfg.ffn, cfg.heads, cfg.kv_heads, cfg.head_dim
-        m, nq, r0, r1 = b * t, (h + 2 * hk) * hd, rows.start, rows.stop
         B = self._extend_buffers(b, t, state.max_pages)
         meta = np.concatenate([ids.reshape(-1).astype(np.int32), np.arange(b + 1, dtype=np.int32) * t,
-                               np.asarray(state.lengths[r0:r1], np.int32), state.table[r0:r1].reshape(-1)])
+                               np.asarray(state.lengths[rows.start:rows.stop], np.int32),
+                               state.table[rows.start:rows.stop].reshape(-1)])
         _lib.call("mfb_memcpy_h2d", P(B["meta"].ptr), meta.ctypes.data_as(P), meta.nbytes, s)
+        for history in state.history:
+            if history is not None:
+                nbytes = history.nbytes // state.batch
+                for row in fresh:
+                    _lib.call("mfb_memset", P(history.ptr + row * nbytes), 0, nbytes, s)
+        if graph:
+            key = ("paged", b, rows.start, state.max_pages, state.num_pages, state.page_size) + tuple(
+                h.ptr if c is None else (c.keys.ptr, c.values.ptr) for c, h in zip(state.caches, state.history))
+            g = self._graphs.get(key)
+            if g is None:
+                _lib.call("mfb_graph_begin", P(s))
+                try:
+                    self._extend_layers(B, state, rows, t)
+                finally:
+                    g_ = P()
+                    _lib.call("mfb_graph_end", P(s), ctypes.byref(g_))
+                g = self._graphs[key] = g_.value
+            _lib.call("mfb_graph_launch", P(g), P(s))
+        else:
+            self._extend_layers(B, state, rows, t)
+        logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")
+        return self._widen(B["logits16"], logits, controls)
+
+    def _extend_layers(self, B, state: PagedState, rows, t: int):
+        """Every layer over the ``t`` uploaded tokens of ``rows``; bf16 logits of the last ones in B["logits16"]."""
+        cfg, s, b = self.cfg, self.stream, len(rows)
+        c, f, h, hk, hd = cfg.hidden, cfg.ffn, cfg.heads, cfg.kv_heads, cfg.head_dim
+        m, nq = b * t, (h + 2 * hk) * hd
         ids_d, cu = B["meta"].view(0, (m,)), B["meta"].view(m, (b + 1,))
         lens, table = B["meta"].view(m + b + 1, (b,)), B["meta"].view(m + 2 * b + 1, (b, state.max_pages))
 
@@ -433,9 +464,7 @@ class Decoder:
             if L["kind"] == "conv":
                 proj(B["hn"], L["w_in"], B["proj"], 3 * c, c)
                 nbytes = state.history[i].nbytes // state.batch
-                history = state.history[i].ptr + r0 * nbytes
-                for row in fresh:
-                    _lib.call("mfb_memset", P(history + (row - r0) * nbytes), 0, nbytes, s)
+                history = state.history[i].ptr + rows.start * nbytes
                 if t == 1:
                     _lib.call("mfb_conv_step", P(B["proj"].ptr), P(L["taps"].ptr), P(history), P(B["mixed"].ptr),
                               b, c, s)
@@ -466,8 +495,6 @@ class Decoder:
             self._proj(B["last"], self.head, B["logits16"], b, cfg.vocab, c, B)
         else:
             _fwd(B["last"], self.head, B["logits16"], b, cfg.vocab, c, s)
-        logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")
-        return self._widen(B["logits16"], logits, controls)
 
     def _extend_buffers(self, b: int, t: int, max_pages: int):
         """Scratch of ``extend`` for b x t tokens, kept per batch, power of two that holds t, and table width."""

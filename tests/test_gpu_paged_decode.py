@@ -129,6 +129,35 @@ def test_refusals_leave_the_state_as_it_was(model):
     _feed(model, state, oracles, range(1, 2), np.array([[3, 4]], np.int32))
 
 
+def test_single_tokens_replayed_as_a_graph(model):
+    """The captured step reads lengths, pages and tokens anew: bit-equal to the launched one, pages taken between."""
+    import ctypes
+    from minifield_training_b200 import _lib
+    dm, cfg, params, plain = model
+    stream = ctypes.c_void_p()
+    _lib.call("mfb_stream_create", ctypes.byref(stream))
+    dec = dm.Decoder(cfg, params, stream=stream.value)
+    states = [dm.new_paged_state(cfg, 3, 12, 8) for _ in range(2)]
+    rng = np.random.default_rng(13)
+    prompt = rng.integers(0, cfg.vocab, (3, 6)).astype(np.int32)
+    for state, d in zip(states, (dec, plain)):
+        d.extend(prompt, state)
+        d.extend(prompt[:1, :3], state, rows=range(1, 2))
+    for step in range(6):
+        if step == 4:
+            for state in states:
+                state.release(2)
+        ids = rng.integers(0, cfg.vocab, (3, 1)).astype(np.int32)
+        got = dec.extend(ids, states[0], graph=True)
+        _lib.call("mfb_stream_sync", ctypes.c_void_p(stream.value))
+        assert np.array_equal(got.numpy(), plain.extend(ids, states[1]).numpy()), step
+    assert states[0].lengths == [12, 15, 2]
+    with pytest.raises(ValueError, match="single tokens"):
+        dec.extend(prompt, states[0], graph=True)
+    with pytest.raises(ValueError, match="created stream|stream="):
+        plain.extend(prompt[:, :1], states[1], graph=True)
+
+
 @pytest.mark.parametrize("path", ["extend", "decode_one", "graph"])
 def test_controls_apply_to_the_steps_logits(model, path):
     """Against the float64 controls of the same step's uncontrolled logits (the step is deterministic)."""
