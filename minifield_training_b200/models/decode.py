@@ -144,6 +144,8 @@ class PagedState:
                         ("max_pages", 1 if max_pages is None else max_pages)):
             if isinstance(n, bool) or not isinstance(n, int) or n <= 0:
                 raise ValueError(f"{name} must be a positive integer")
+        if batch_size > 8192:
+            raise ValueError(f"batch_size {batch_size} above the supported 8192 rows")
         if page_size < 8 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two of at least 8")
         self.cfg, self.batch, self.page_size, self.num_pages = cfg, batch_size, page_size, num_pages
@@ -411,8 +413,9 @@ class Decoder:
             raise ValueError("graph replay takes single tokens and needs Decoder(stream=...) from mfb_stream_create")
         controls = self._controls(controls, b)
         fresh = [row for row in rows if state.lengths[row] == 0]
-        state.grow(rows, t)
         B = self._extend_buffers(b, t, state.max_pages)
+        logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")
+        state.grow(rows, t)  # what can fail for lack of memory is behind us
         meta = np.concatenate([ids.reshape(-1).astype(np.int32), np.arange(b + 1, dtype=np.int32) * t,
                                np.asarray(state.lengths[rows.start:rows.stop], np.int32),
                                state.table[rows.start:rows.stop].reshape(-1)])
@@ -437,7 +440,6 @@ class Decoder:
             _lib.call("mfb_graph_launch", P(g), P(s))
         else:
             self._extend_layers(B, state, rows, t)
-        logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")
         return self._widen(B["logits16"], logits, controls)
 
     def _extend_layers(self, B, state: PagedState, rows, t: int):

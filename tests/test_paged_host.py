@@ -219,6 +219,7 @@ def test_workspace_sizes_cover_odd_shapes():
 
 @pytest.mark.parametrize("kw, match", [
     (dict(batch_size=0), "batch_size"),
+    (dict(batch_size=8193), "8192 rows"),
     (dict(num_pages=-1), "num_pages"),
     (dict(num_pages=True), "num_pages"),
     (dict(page_size=12), "power of two"),
