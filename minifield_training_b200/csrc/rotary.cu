@@ -22,11 +22,13 @@
 // and the kind of head are settled once and the rotation needs no exchange
 // between lanes. Every 32-byte sector is still read and written whole. A block
 // takes a few tokens at a time: their heads' loads are under way while the
-// block computes the tokens' rotary_dim/2 angles each into shared memory. The
+// block computes the tokens' rotary_dim/2 angles each into shared memory; their
+// positions and cache rows, a chain of dependent loads, are looked up for 32
+// tokens at a time. The
 // floor is the bytes; what keeps a kernel of this kind above it is the
 // instructions per byte: with a warp per token that loops over the heads, the
 // same arithmetic took three times the instructions and 84 to 111 us where
-// this takes 76 us (16384 tokens of 32 heads, forward and backward).
+// this takes 70 us (16384 tokens of 32 heads, forward and backward).
 #include <algorithm>
 
 #include "types16.cuh"
@@ -40,6 +42,8 @@ constexpr int MAX_D = 128;
 // forward and backward: 8 tokens / 3 blocks forward with 4 / 3 backward 78.7,
 // 4 / 4 with 2 / 4 75.7, 4 / 5 with 2 / 5 83.3, 2 / 6 with 1 / 5 87.2 us.
 constexpr int FWD_TOKENS = 4, BWD_TOKENS = 2, BLOCKS_PER_SM = 4;
+// Tokens whose positions (and cache rows) a block looks up at once.
+constexpr int LOOKUP = 32;
 constexpr int MAX_SMS = 160;
 constexpr int BWD_GRID_MAX = BLOCKS_PER_SM * MAX_SMS;  // blocks of a backward pass: rows of gain-gradient partials
 constexpr double kInvTwoPi = 0.15915494309189533577;
@@ -194,8 +198,8 @@ __device__ __forceinline__ int run_begin(const Params& p, int i) { return (int)(
 template <typename T, int D, bool IL, bool PAGED>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_fwd_kernel(Params p) {
   __shared__ __align__(16) Angles<FWD_TOKENS> angles;
-  __shared__ int s_pos[FWD_TOKENS];
-  __shared__ long long s_place[FWD_TOKENS];  // element offset of a token's first head in k and v; -1: not stored
+  __shared__ int s_pos[LOOKUP];
+  __shared__ long long s_place[LOOKUP];  // element offset of a token's first head in k and v; -1: not stored
   const Place<D, IL> w(p);
   uint64_t gain[4];
   w.gains(p, gain);
@@ -212,32 +216,35 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_fwd_kernel(Para
       src += p.ld;
     });
     __syncthreads();  // the last pass is done with the shared tables
-    if (threadIdx.x < tokens) {
+    const int at = (row0 - begin) % LOOKUP;
+    if (at == 0) {
       const int row = row0 + threadIdx.x;
-      int pos = 0;
-      long long place = -1;
-      if (PAGED) {
-        if (row < p.cu_q[0] || row >= p.cu_q[p.B]) {
-          place = -2;  // padding: nothing is stored
-        } else {
-          const int b = sequence_of(p.cu_q, p.B, row);
-          pos = p.seq_lens[b] - (p.cu_q[b + 1] - row);
-          const int pg = pos >> p.page_shift;
-          if (pos >= 0 && pg < p.max_pages) {
-            const int id = p.page_table[(long long)b * p.max_pages + pg];
-            if ((unsigned)id < (unsigned)p.num_pages)
-              place = (long long)id * p.page_stride + (long long)(pos - (pg << p.page_shift)) * p.token_stride;
+      if (threadIdx.x < LOOKUP && row < end) {
+        int pos = 0;
+        long long place = -1;
+        if (PAGED) {
+          if (row < p.cu_q[0] || row >= p.cu_q[p.B]) {
+            place = -2;  // padding: nothing is stored
+          } else {
+            const int b = sequence_of(p.cu_q, p.B, row);
+            pos = p.seq_lens[b] - (p.cu_q[b + 1] - row);
+            const int pg = pos >> p.page_shift;
+            if (pos >= 0 && pg < p.max_pages) {
+              const int id = p.page_table[(long long)b * p.max_pages + pg];
+              if ((unsigned)id < (unsigned)p.num_pages)
+                place = (long long)id * p.page_stride + (long long)(pos - (pg << p.page_shift)) * p.token_stride;
+            }
           }
+        } else {
+          pos = p.positions[row];
+          place = (long long)row * p.Hk * D;
         }
-      } else {
-        pos = p.positions[row];
-        place = (long long)row * p.Hk * D;
+        s_pos[threadIdx.x] = pos;
+        s_place[threadIdx.x] = place;
       }
-      s_pos[threadIdx.x] = pos;
-      s_place[threadIdx.x] = place;
+      __syncthreads();
     }
-    __syncthreads();
-    angles.fill(p, s_pos, tokens);
+    angles.fill(p, s_pos + at, tokens);
     __syncthreads();
     long long q_to = (long long)row0 * p.H * D;
     over_tokens<FWD_TOKENS>(tokens, [&](int t) {
@@ -258,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_fwd_kernel(Para
           b = pack16x4<T>(x + 2);
         }
       }
-      long long to = s_place[t];
+      long long to = s_place[at + t];
       const bool stored = w.live && to >= (w.kind ? 0 : -1);
       if (w.kind == 0) to = q_to;
       q_to += p.H * D;
@@ -274,7 +281,7 @@ template <typename T, int D, bool IL>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_bwd_kernel(Params p) {
   using W = Place<D, IL>;
   __shared__ __align__(16) Angles<BWD_TOKENS> angles;
-  __shared__ int s_pos[BWD_TOKENS];
+  __shared__ int s_pos[LOOKUP];
   __shared__ float sums[THREADS / W::L][D];
   const W w(p);
   uint64_t gain[4], acc[4];
@@ -301,9 +308,12 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_bwd_kernel(Para
       row += p.ld;
     });
     __syncthreads();
-    if (threadIdx.x < tokens) s_pos[threadIdx.x] = p.positions[row0 + threadIdx.x];
-    __syncthreads();
-    angles.fill(p, s_pos, tokens);
+    const int at = (row0 - begin) % LOOKUP;
+    if (at == 0) {
+      if (threadIdx.x < LOOKUP && row0 + threadIdx.x < end) s_pos[threadIdx.x] = p.positions[row0 + threadIdx.x];
+      __syncthreads();
+    }
+    angles.fill(p, s_pos + at, tokens);
     __syncthreads();
     uint16_t* out = p.dqkv + (long long)row0 * p.ld + w.head * D;
     over_tokens<BWD_TOKENS>(tokens, [&](int t) {
