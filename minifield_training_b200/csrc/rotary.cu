@@ -197,7 +197,7 @@ __device__ __forceinline__ int run_begin(const Params& p, int i) { return (int)(
 
 template <typename T, int D, bool IL, bool PAGED>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_fwd_kernel(Params p) {
-  __shared__ __align__(16) Angles<FWD_TOKENS> angles;
+  __shared__ __align__(16) Angles<FWD_TOKENS> tables[2];  // by turns: a pass needs one barrier
   __shared__ int s_pos[LOOKUP];
   __shared__ long long s_place[LOOKUP];  // element offset of a token's first head in k and v; -1: not stored
   const Place<D, IL> w(p);
@@ -215,9 +215,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_fwd_kernel(Para
       vb[t] = ld8(src + w.ob);
       src += p.ld;
     });
-    __syncthreads();  // the last pass is done with the shared tables
     const int at = (row0 - begin) % LOOKUP;
     if (at == 0) {
+      __syncthreads();  // the last pass is done with the places
       const int row = row0 + threadIdx.x;
       if (threadIdx.x < LOOKUP && row < end) {
         int pos = 0;
@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_fwd_kernel(Para
       }
       __syncthreads();
     }
+    Angles<FWD_TOKENS>& angles = tables[(row0 - begin) / FWD_TOKENS & 1];
     angles.fill(p, s_pos + at, tokens);
     __syncthreads();
     long long q_to = (long long)row0 * p.H * D;
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_fwd_kernel(Para
 template <typename T, int D, bool IL>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_bwd_kernel(Params p) {
   using W = Place<D, IL>;
-  __shared__ __align__(16) Angles<BWD_TOKENS> angles;
+  __shared__ __align__(16) Angles<BWD_TOKENS> tables[2];
   __shared__ int s_pos[LOOKUP];
   __shared__ float sums[THREADS / W::L][D];
   const W w(p);
@@ -307,12 +308,13 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) rotary_bwd_kernel(Para
       }
       row += p.ld;
     });
-    __syncthreads();
     const int at = (row0 - begin) % LOOKUP;
     if (at == 0) {
+      __syncthreads();
       if (threadIdx.x < LOOKUP && row0 + threadIdx.x < end) s_pos[threadIdx.x] = p.positions[row0 + threadIdx.x];
       __syncthreads();
     }
+    Angles<BWD_TOKENS>& angles = tables[(row0 - begin) / BWD_TOKENS & 1];
     angles.fill(p, s_pos + at, tokens);
     __syncthreads();
     uint16_t* out = p.dqkv + (long long)row0 * p.ld + w.head * D;
