@@ -39,8 +39,8 @@ namespace rot {
 constexpr int THREADS = 256;
 constexpr int MAX_D = 128;
 // Tokens of a block's pass, and blocks per SM. Measured together on 16384 tokens
-// forward and backward: 8 tokens / 3 blocks forward with 4 / 3 backward 78.7,
-// 4 / 4 with 2 / 4 75.7, 4 / 5 with 2 / 5 83.3, 2 / 6 with 1 / 5 87.2 us.
+// forward and backward: 8 tokens forward and 4 backward at 3 blocks 73.8, 4 and
+// 2 at 4 blocks 69.7, at 3 77.6, at 5 81.6, 2 and 1 at 6 88.0 us.
 constexpr int FWD_TOKENS = 4, BWD_TOKENS = 2, BLOCKS_PER_SM = 4;
 // Tokens whose positions (and cache rows) a block looks up at once.
 constexpr int LOOKUP = 32;
