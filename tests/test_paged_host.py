@@ -243,3 +243,15 @@ def test_prepared_controls_refuse():
     with pytest.raises(TypeError, match="no further"):
         lg.process_logits(fake((2, 100), "bfloat16"), out=fake((2, 100), "float32"), controls=ready,
                           mask=fake((2, 4), "int32"))
+
+
+def test_packed_calls_refuse():
+    """Integers past their parameter's 32 bits and a missing block are refused, not truncated."""
+    for large in (1 << 31, 1 << 40, (1 << 32) + 2):
+        with pytest.raises(ValueError, match="out of range"):
+            attention_call(max_q=large)
+    with pytest.raises(ValueError, match="out of range"):
+        append_call(heads=16, table=fake((2, 1 << 33), "int32"))
+    for name in ("mfb_qk_rotary_fwd", "mfb_qk_rotary_bwd", "mfb_paged_append", "mfb_paged_attn", "mfb_logits_process"):
+        assert getattr(_lib.lib(), name + "_packed")(None) == _lib.ERR_INVALID
+        assert name in _lib.last_error()
