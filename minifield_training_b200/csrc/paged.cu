@@ -389,8 +389,9 @@ struct PageIds {
   int b, br, nb, end;  // sequence, keys per box, boxes per tile, keys that are needed
   int window, cur, next;
   __device__ __forceinline__ int fetch(const Params& p, int w) const {
-    const int key = (w * 32 + (int)(threadIdx.x & 31)) * br;
-    return key < end ? page_id(p, b, key) : 0;
+    // Unsigned: a window ahead of a sequence that ends just below 2^31 lies above it.
+    const unsigned key = ((unsigned)w * 32u + (threadIdx.x & 31u)) * (unsigned)br;
+    return key < (unsigned)end ? page_id(p, b, (int)key) : 0;
   }
   __device__ __forceinline__ PageIds(const Params& p, int seq, int rows, int boxes, int tile, int keys)
       : b(seq), br(rows), nb(boxes), end(keys), window(tile * boxes >> 5) {

@@ -1,0 +1,43 @@
+"""Edges of the rotary, paged-cache and logit operators on the GPU: the largest sizes, many items, odd values.
+
+Helpers and tolerances are those of tests/test_gpu_paged.py.
+"""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from oracle import paged as op
+from tests.gpu_env import require_gpu
+from tests.test_gpu_paged import NP, U, build, check_attention, dev, normal, run_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("count", [1, 20])
+def test_sequence_that_ends_just_below_2_31(count):
+    """The look-ahead of page ids (4096 keys) passes 2^31; every page of the table is the pool's one page.
+
+    Keys are zeros, so all weights are equal, and the values are 1/2. A row part's sums of n <= 2^31 / 148 ones and
+    halves are exact in FP32 but for the polynomial exponential (2.7e-6), the joins round at most 300 times by
+    2^-24: below 2^-15 in all, where half a step of bf16 under 1/2 is 2^-10.
+    """
+    require_gpu()
+    from minifield_training_b200.device import DeviceArray
+    from minifield_training_b200.kernels import paged
+
+    page, pages = 1024, (1 << 21) - 1
+    length = page * pages - 5
+    keys, values = np.zeros((1, page, 1, 64), NP["bfloat16"]), np.full((1, page, 1, 64), 0.5, NP["bfloat16"])
+    cache = paged.PagedCache(dev(keys, "bfloat16"), dev(values, "bfloat16"))
+    q = dev(np.ones((count, 1, 64), NP["bfloat16"]), "bfloat16")
+    lse = DeviceArray((count, 1), "float32")
+    paged.paged_attention_status()
+    out = paged.paged_attention(q, cache, dev(np.array([0, count], np.int32)), dev(np.array([length], np.int32)),
+                                dev(np.zeros((1, pages), np.int32)), max_q=count, lse=lse)
+    got = out.numpy().astype(np.float32)
+    assert paged.paged_attention_status() == 0
+    np.testing.assert_array_equal(got, 0.5)
+    want = np.log(length - count + 1.0 + np.arange(count))
+    assert np.all(np.abs(lse.numpy()[:, 0] - want) <= 2.0 ** -18 * want)
