@@ -97,23 +97,24 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 // ---------------------------------------------------------------------------
 constexpr int SCHED_THREADS = 1024;
 
-// Exclusive block scan of one int per thread; returns the prefix, total in *sum.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* sum) {
+// Exclusive block scan of one value per thread; returns the prefix, total in *sum.
+template <typename I>
+__device__ __forceinline__ I block_scan(I v, I* warp_sums, I* sum) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = v;
+  I incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    const I y = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += y;
   }
   __syncthreads();  // the previous scan's readers are done with warp_sums
   if (lane == 31) warp_sums[warp] = incl;
   __syncthreads();
   if (warp == 0) {
-    int w = warp_sums[lane];
+    I w = warp_sums[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      const I y = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += y;
     }
     warp_sums[lane] = w;
@@ -163,18 +164,22 @@ __global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
   allow_dependents();
   extern __shared__ int item_base[];  // [B] items before each sequence
   __shared__ int warp_sums[32], s_cuts;
+  __shared__ long long wide_sums[32];
   const int tid = threadIdx.x;
   if (tid == 0) s_cuts = 0;
-  int carry = 0;
+  // Sequences whose cu_q contradict each other may claim the same rows, each all
+  // of them: their items are counted in 64 bits and those past max_items dropped.
+  long long listed = 0;
   for (int b0 = 0; b0 < p.B; b0 += SCHED_THREADS) {
     const int b = b0 + tid;
-    int q0, nq = 0, base, len, sum;
+    int q0, nq = 0, base, len;
+    long long sum;
     if (b < p.B) sequence(p, b, &q0, &nq, &base, &len);
-    const int pre = block_scan(cdiv(nq, p.tok_item) * p.Hk, warp_sums, &sum);
-    if (b < p.B) item_base[b] = carry + pre;
-    carry += sum;
+    const long long pre = block_scan((long long)cdiv(nq, p.tok_item) * p.Hk, wide_sums, &sum);
+    if (b < p.B) item_base[b] = (int)min(listed + pre, (long long)p.max_items);
+    listed += sum;
   }
-  const int items = min(carry, p.max_items);
+  const int items = (int)min(listed, (long long)p.max_items);
   __syncthreads();
   auto make = [&](int i) {
     Item it;
@@ -211,7 +216,7 @@ __global__ void __launch_bounds__(SCHED_THREADS) schedule_kernel(Params p) {
     total += sum;
   }
   Header h = cut(p, total);
-  carry = 0;
+  int carry = 0;
   for (int i0 = 0; i0 < items; i0 += SCHED_THREADS) {
     const int i = i0 + tid;
     if (items > SCHED_THREADS) {

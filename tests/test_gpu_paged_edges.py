@@ -41,3 +41,26 @@ def test_sequence_that_ends_just_below_2_31(count):
     np.testing.assert_array_equal(got, 0.5)
     want = np.log(length - count + 1.0 + np.arange(count))
     assert np.all(np.abs(lse.numpy()[:, 0] - want) <= 2.0 ** -18 * want)
+
+
+def test_sequences_that_claim_the_same_rows_past_2_31_items():
+    """cu_q = 0, N, 0, N, ...: 4096 sequences of all N rows each, 2^31 items in all, are counted and cut at the list."""
+    require_gpu()
+    from minifield_training_b200 import _lib
+    from minifield_training_b200.device import DeviceArray
+    from minifield_training_b200.kernels import paged
+
+    n, batch = 1 << 27, 8192
+    q = DeviceArray((n, 1, 64), "bfloat16")
+    _lib.call("mfb_memset", q.ptr, 0x40, q.nbytes, None)  # 0x4040: 3.0
+    pool = np.full((1, 16, 1, 64), 1.5, NP["bfloat16"])
+    cache = paged.PagedCache(dev(pool, "bfloat16"), dev(pool, "bfloat16"))
+    cu = np.zeros(batch + 1, np.int32)
+    cu[1::2] = n
+    paged.paged_attention_status()
+    paged.paged_attention(q, cache, dev(cu), dev(np.ones(batch, np.int32)), dev(np.zeros((batch, 1), np.int32)),
+                          max_q=n, out=q)
+    assert paged.paged_attention_status() == 1002
+    for at in (0, 1 << 26, n - 1001):  # a sequence's only token is its last row's key
+        assert not np.any(q.view(at * 64, (1000, 64)).numpy().astype(np.float32))
+    np.testing.assert_array_equal(q.view((n - 1) * 64, (64,)).numpy().astype(np.float32), 1.5)
