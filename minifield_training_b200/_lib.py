@@ -81,6 +81,7 @@ SIGNATURES = {
     "mfb_graph_launch": (I, [P, P]),
     "mfb_graph_destroy": (I, [P]),
     "mfb_stream_is_capturing": (I, [P, IP]),
+    "mfb_stream_identity": (I, [P, ctypes.POINTER(ctypes.c_uint64)]),
     "mfb_adamw_workspace_size": (SZ, []),
     "mfb_adamw_commit": (I, [P, P, P, P, LL, LL, LL, P, P, P, P, F, F, F, F, F, F, P, P, SZ, P]),
     "mfb_adamw_shard_pass": (I, [I, P, P, P, P, LL, LL, LL, LL, LL, P, P, P, P, F, F, F, F, F, F, P, P, P, SZ, P]),

@@ -206,6 +206,19 @@ int mfb_stream_is_capturing(void* stream, int* capturing) {
   return MFB_OK;
 }
 
+int mfb_stream_identity(void* stream, uint64_t* identity) {
+  MFB_CHECK_ARG(identity != nullptr, "identity is NULL");
+  int device = 0, capturing = 0;
+  unsigned long long id = 0;
+  MFB_CUDA_TRY(cudaGetDevice(&device));
+  const int st = mfb_stream_is_capturing(stream, &capturing);
+  if (st) return st;
+  if (!capturing) MFB_CUDA_TRY(cudaStreamGetId((cudaStream_t)stream, &id));  // not answered during a capture
+  identity[0] = (uint64_t)device;
+  identity[1] = id;
+  return MFB_OK;
+}
+
 int mfb_graph_destroy(void* graph_exec) {
   if (graph_exec) MFB_CUDA_TRY(cudaGraphExecDestroy((cudaGraphExec_t)graph_exec));
   return MFB_OK;

@@ -9,6 +9,7 @@ plays in the reference. Host NumPy arrays passed to the API are uploaded
 
 import ctypes
 import math
+import threading
 
 import ml_dtypes
 import numpy as np
@@ -202,24 +203,32 @@ def workspace(tag: str, nbytes: int) -> DeviceArray:
 
 
 _STREAM_WORKSPACES = {}
+_LEGACY_STREAM, _PER_THREAD_STREAM = 1, 2  # the handles CUDA reserves
 
 
 def stream_workspace(tag: str, nbytes: int, stream=None) -> DeviceArray:
     """Grow-only scratch of one stream: calls on different streams never share it.
 
+    Kept per device and stream handle (and per thread where the handle names a
+    stream of each), for as long as the handle means the same stream: one that
+    a destroyed stream left to a new one starts afresh.
+
     A call recorded into a CUDA graph must not use it (the graph outlives the
-    call and may replay beside later ones): callers pass
-    ``PACKED_SHARED_WORKSPACE``, and growing is refused here.
+    call and may replay beside later ones): it is refused here.
     """
-    key = (tag, getattr(stream, "value", stream))
+    identity = (ctypes.c_uint64 * 2)()
+    _lib.call("mfb_stream_identity", stream, identity)
+    device, stream_id = identity
+    if not stream_id:
+        raise ValueError(f"a captured {tag} call needs its own workspace (workspace=)")
+    handle = getattr(stream, "value", stream) or _LEGACY_STREAM
+    key = (tag, device, handle, threading.get_ident() if handle == _PER_THREAD_STREAM else None)
     entry = _STREAM_WORKSPACES.get(key)
+    if entry is not None and entry[2] != stream_id:
+        entry = None
     if entry is None or entry[1] < nbytes:
-        flag = ctypes.c_int()
-        _lib.call("mfb_stream_is_capturing", stream, ctypes.byref(flag))
-        if flag.value:
-            raise ValueError(f"a captured {tag} call needs its own workspace (workspace=)")
         size = max(int(nbytes), 2 * entry[1] if entry else 256)
-        entry = _STREAM_WORKSPACES[key] = (DeviceArray((size,), "uint8"), size)
+        entry = _STREAM_WORKSPACES[key] = (DeviceArray((size,), "uint8"), size, stream_id)
     return entry[0]
 
 

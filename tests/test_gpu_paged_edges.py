@@ -64,3 +64,30 @@ def test_sequences_that_claim_the_same_rows_past_2_31_items():
     for at in (0, 1 << 26, n - 1001):  # a sequence's only token is its last row's key
         assert not np.any(q.view(at * 64, (1000, 64)).numpy().astype(np.float32))
     np.testing.assert_array_equal(q.view((n - 1) * 64, (64,)).numpy().astype(np.float32), 1.5)
+
+
+def test_streams_have_identities_of_their_own():
+    """Handles come again after a stream is destroyed, identities do not; the default stream keeps its own."""
+    require_gpu()
+    from minifield_training_b200 import _lib
+
+    def identity(stream):
+        out = (ctypes.c_uint64 * 2)()
+        _lib.call("mfb_stream_identity", stream, out)
+        return out[0], out[1]
+
+    default = identity(None)
+    seen, word = {default}, dev(np.zeros(1, np.int32))
+    for _ in range(20):
+        s = ctypes.c_void_p()
+        _lib.call("mfb_stream_create", ctypes.byref(s))
+        assert identity(s.value) not in seen and identity(s.value) == identity(s.value)
+        seen.add(identity(s.value))
+        _lib.call("mfb_graph_begin", s.value)
+        assert identity(s.value) == (default[0], 0) and identity(None) == default
+        _lib.call("mfb_memset", word.ptr, 0, 4, s.value)
+        g = ctypes.c_void_p()
+        _lib.call("mfb_graph_end", s.value, ctypes.byref(g))
+        _lib.call("mfb_graph_destroy", g.value)
+        _lib.call("mfb_stream_destroy", s.value)
+    assert len(seen) == 21 and identity(None) == default == identity(ctypes.c_void_p(1))
