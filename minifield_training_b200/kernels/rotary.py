@@ -61,7 +61,8 @@ def rotary_frequencies(rotary_dim: int, theta: float, scaling: dict | None = Non
             return r * math.log(length / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
 
         low = max(math.floor(pair_turning(scaling.get("beta_fast", 32.0))), 0)
-        high = min(math.ceil(pair_turning(scaling.get("beta_slow", 1.0))), r // 2 - 1)
+        # May lie behind the last pair, which then turns more than beta_slow times.
+        high = min(math.ceil(pair_turning(scaling.get("beta_slow", 1.0))), r - 1)
         ramp = np.clip((index - low) / max(high - low, 1e-3), 0.0, 1.0)
         return (base * (1.0 - ramp) + base / factor * ramp).astype(np.float32), 1.0 + 0.1 * math.log(factor)
     raise ValueError(f"Unsupported rotary scaling: {kind}")

@@ -9,6 +9,7 @@ import pytest
 
 from minifield_training_b200 import _lib, device
 from minifield_training_b200.device import DeviceArray
+from minifield_training_b200.kernels import paged, rotary
 
 
 class FakeDevice:
@@ -78,3 +79,20 @@ def test_a_reused_stream_handle_gets_a_new_workspace(fake):
     for nbytes in (10, 5000):
         with pytest.raises(ValueError, match="its own workspace"):
             device.stream_workspace("w", nbytes, 64)
+
+
+@pytest.mark.parametrize("length, factor, low, high", [(4096, 16, 10, 23), (65536, 4, 20, 33), (131072, 8, 22, 35)])
+def test_yarn_divides_only_pairs_that_turn_too_seldom(length, factor, low, high):
+    """Rotary 64, theta 1e4: pair i turns length 1e4^(-i / 32) / 2 pi times, 32 and once at the bounds given here.
+
+    The ramp runs between the whole pairs around those bounds, also where the second one lies behind the last pair.
+    """
+    index = np.arange(32)
+    base = 1e4 ** (-index / 32.0)
+    turns = length * base / (2 * math.pi)
+    pair = [32 * math.log(length / (t * 2 * math.pi)) / math.log(1e4) for t in (32.0, 1.0)]
+    assert (math.floor(pair[0]), math.ceil(pair[1])) == (low, high)
+    share = np.array([min(max((i - low) / (high - low), 0.0), 1.0) for i in index])  # of the divided frequency
+    got = rotary.rotary_frequencies(64, 1e4, {"kind": "yarn", "factor": factor, "original_length": length})[0]
+    np.testing.assert_allclose(got, base * ((1 - share) + share / factor), rtol=2.0 ** -22)
+    assert np.all(got[turns > 1.0] > base[turns > 1.0] / factor * (1 + 2.0 ** -20))
