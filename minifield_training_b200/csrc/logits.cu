@@ -95,8 +95,8 @@ struct Row {
 __device__ __forceinline__ float control(float x, uint32_t w, const Row& r) {
   x = w & kSeen ? x * (x > 0.f ? r.inv_rep : r.rep) : x;
   const float made = (float)(w & kMade);
-  x = fmaf(-r.freq, made, x);
-  return made > 0.f ? x - r.pres : x;
+  // Not 0 x frequency elsewhere: an infinite penalty would make a NaN of it.
+  return made > 0.f ? fmaf(-r.freq, made, x) - r.pres : x;
 }
 
 constexpr int AHEAD = 4;  // vectors per thread whose loads precede the table's work

@@ -91,3 +91,19 @@ def test_streams_have_identities_of_their_own():
         _lib.call("mfb_graph_destroy", g.value)
         _lib.call("mfb_stream_destroy", s.value)
     assert len(seen) == 21 and identity(None) == default == identity(ctypes.c_void_p(1))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_infinite_penalties_reach_only_their_tokens(dtype):
+    """A token that was not generated keeps its logit, beside generated ones as anywhere else."""
+    require_gpu()
+    from minifield_training_b200.kernels import logits as lg
+
+    rng = np.random.default_rng(14)
+    x = rng.standard_normal((3, 100), dtype=np.float32).astype(NP[dtype])
+    hist = np.array([[40, 8, 9, 9, 63], [0, 99, 99, 1, 98], [7, 7, 7, 7, 7]], np.int32)
+    inf = np.float32(np.inf)
+    for name, values in (("frequency", [inf, inf, -inf]), ("presence", [inf, -inf, inf])):
+        kw = dict(history=hist, prompt_len=np.array([1, 1, 0], np.int32), **{name: np.array(values, np.float32)})
+        got = lg.process_logits(dev(x, dtype), **{k: dev(v) for k, v in kw.items()}).numpy()
+        np.testing.assert_array_equal(got, op.controlled_logits(x, **kw).astype(np.float32))
