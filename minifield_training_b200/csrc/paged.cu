@@ -261,7 +261,10 @@ __device__ __forceinline__ long long part_at(const Params& p, int slot, int row,
   return ROWS32 ? ((r >> 5) * (D / 4) + d4) * 32 + (r & 31) : r * (D / 4) + d4;
 }
 
-__device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY; }
+// No key: -inf. A NaN sum (a query that is not finite) stays NaN, like the output beside it.
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+}
 
 // Joins the cut items. Each is split by rows over an equal part of the blocks;
 // a block's threads are float4 columns x lanes, a lane taking every lanes-th

@@ -107,3 +107,24 @@ def test_infinite_penalties_reach_only_their_tokens(dtype):
         kw = dict(history=hist, prompt_len=np.array([1, 1, 0], np.int32), **{name: np.array(values, np.float32)})
         got = lg.process_logits(dev(x, dtype), **{k: dev(v) for k, v in kw.items()}).numpy()
         np.testing.assert_array_equal(got, op.controlled_logits(x, **kw).astype(np.float32))
+
+
+@pytest.mark.parametrize("lens, counts, h, hk, dtype", [
+    ([70, 9], [1, 1], 16, 8, "bfloat16"),  # whole items
+    ([9000, 40], [2, 1], 4, 2, "float16"),  # items cut between CTAs
+    ([300, 64], [40, 64], 4, 2, "bfloat16"),  # tiles
+    ([9000, 300], [200, 30], 2, 1, "float16"),  # tiles, cut
+])
+def test_queries_that_are_not_numbers(lens, counts, h, hk, dtype):
+    """A NaN query gives NaN in its output and its lse, not the -inf of a token without keys; the others see nothing."""
+    require_gpu()
+    rng = np.random.default_rng(15)
+    a = build(rng, lens, counts, h, hk, 64, 16, False, dtype, pad=2)
+    good, good_lse = run_attention(*a, False, dtype, max(counts))
+    q, hurt = a[0].copy(), np.zeros(a[0].shape[:2], bool)
+    for t, head in ((0, 0), (int(a[3][1]) - 1, 1), (int(a[3][2]) - 1, h - 1)):
+        q[t, head, 5], hurt[t, head] = np.nan, True
+    got, lse = run_attention(q, *a[1:], False, dtype, max(counts))
+    np.testing.assert_array_equal(got[~hurt], good[~hurt])
+    np.testing.assert_array_equal(lse[~hurt], good_lse[~hurt])
+    assert np.all(np.isnan(got[hurt].astype(np.float32))) and np.all(np.isnan(lse[hurt]))
