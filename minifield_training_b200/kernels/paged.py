@@ -60,7 +60,8 @@ def paged_append(qkv, cache: PagedCache, cu_q, seq_lens, page_table, *, heads, f
 
     Norm and rotation as in ``rotary.qk_rotary_fwd``, at each token's place in
     its sequence. A token without a page (entry outside the pool, or behind
-    the table) is not stored.
+    the table) is not stored. A pool or table of no pages is refused, as
+    ``paged_attention`` refuses it.
     """
     n, ld, d, freqs, wq, wk = projection(qkv, heads, cache.kv_heads, cache.head_dim, freqs, q_weight, k_weight,
                                          stream)
@@ -69,7 +70,7 @@ def paged_append(qkv, cache: PagedCache, cu_q, seq_lens, page_table, *, heads, f
     cu_q, seq_lens, page_table = _sequences(cu_q, seq_lens, page_table, stream)
     q = check_out(out, (n, heads, d), qkv.dtype, "out")
     b, max_pages = page_table.shape
-    if n and b and max_pages and cache.num_pages:
+    if n and b:
         _lib.call_packed("mfb_paged_append", 0, qkv.ptr, ld, wq.ptr if wq is not None else 0,
                   wk.ptr if wk is not None else 0, freqs.ptr, cu_q.ptr, seq_lens.ptr, page_table.ptr, q.ptr,
                   cache.keys.ptr, cache.values.ptr, n, b, max_pages, cache.num_pages, cache.page_size, heads,

@@ -96,3 +96,16 @@ def test_yarn_divides_only_pairs_that_turn_too_seldom(length, factor, low, high)
     got = rotary.rotary_frequencies(64, 1e4, {"kind": "yarn", "factor": factor, "original_length": length})[0]
     np.testing.assert_allclose(got, base * ((1 - share) + share / factor), rtol=2.0 ** -22)
     assert np.all(got[turns > 1.0] > base[turns > 1.0] / factor * (1 + 2.0 ** -20))
+
+
+@pytest.mark.parametrize("pages, columns", [(0, 5), (9, 0), (0, 0)])
+def test_append_and_attention_refuse_a_cache_without_pages(pages, columns):
+    """Both refuse; append once returned a q that nothing had written."""
+    cache = paged.PagedCache(*[array((pages, 16, 8, 64), "bfloat16")] * 2)
+    cu, lens, table = array((3,), "int32"), array((2,), "int32"), array((2, columns), "int32")
+    q = array((4, 16, 64), "bfloat16")
+    with pytest.raises(ValueError, match="pages"):
+        paged.paged_append(array((4, 2048), "bfloat16"), cache, cu, lens, table, heads=16,
+                           freqs=array((32,), "float32"), out=q)
+    with pytest.raises(ValueError, match="pages"):
+        paged.paged_attention(q, cache, cu, lens, table, max_q=2, out=q, workspace=array((1 << 30,), "uint8"))
