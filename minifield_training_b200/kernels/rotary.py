@@ -159,7 +159,7 @@ def qk_rotary_bwd(qkv, positions, freqs, dq, dk, dv, *, head_dim=None, interleav
         raise ValueError("dq, dk and dv must match the projection's heads")
     if wq is None and (weight_grads is not None or accumulate):
         raise ValueError("gain gradients need the gains")
-    if accumulate and weight_grads is None:
+    if accumulate and (weight_grads is None or any(g is None for g in weight_grads)):
         raise ValueError("accumulate needs weight_grads to add to")
     dqkv = check_out(out, qkv.shape, qkv.dtype, "out")
     dwq = dwk = ws = None

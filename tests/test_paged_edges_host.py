@@ -109,3 +109,17 @@ def test_append_and_attention_refuse_a_cache_without_pages(pages, columns):
                            freqs=array((32,), "float32"), out=q)
     with pytest.raises(ValueError, match="pages"):
         paged.paged_attention(q, cache, cu, lens, table, max_q=2, out=q, workspace=array((1 << 30,), "uint8"))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_rotary_backward_adds_only_to_given_gradients(fake, which):
+    """A missing one of the two is a new array, which holds nothing that could be added to."""
+    qkv, w = array((4, 2048), "bfloat16"), array((64,), "float32")
+    args = [qkv, array((4,), "int32"), array((32,), "float32"), array((4, 16, 64), "bfloat16"),
+            array((4, 8, 64), "bfloat16"), array((4, 8, 64), "bfloat16")]
+    grads = [w, w]
+    grads[which] = None
+    with pytest.raises(ValueError, match="to add to"):
+        rotary.qk_rotary_bwd(*args, q_weight=w, k_weight=w, weight_grads=tuple(grads), accumulate=True)
+    got = rotary.qk_rotary_bwd(*args, q_weight=w, k_weight=w, weight_grads=tuple(grads))[1:]
+    assert got[1 - which] is w and got[which] is not w and got[which].shape == (64,)
