@@ -408,7 +408,8 @@ int mfb_qk_rotary_fwd(const void* qkv, int ld_qkv, const float* wq, const float*
                       int interleaved, int dtype, float amplitude, float eps, void* stream);
 /* d_qkv [M, ld_qkv] from dq [M,H,D], dk and dv [M,Hk,D] (norms recomputed from
  * qkv), and the gain gradients dwq, dwk [D] FP32, written or added to
- * (accumulate); both NULL to leave them out. d_qkv may be qkv itself. */
+ * (accumulate); both NULL to leave them out. d_qkv may be qkv itself; its columns
+ * behind the heads are left as they were. */
 size_t mfb_qk_rotary_workspace_size(int D);
 int mfb_qk_rotary_bwd(const void* qkv, int ld_qkv, const float* wq, const float* wk, const int32_t* positions,
                       const float* freqs, const void* dq, const void* dk, const void* dv, void* dqkv, float* dwq,

@@ -144,7 +144,8 @@ def qk_rotary_bwd(qkv, positions, freqs, dq, dk, dv, *, head_dim=None, interleav
 
     The gain gradients (float32 [D]) are new arrays, or ``weight_grads`` =
     (dq_weight, dk_weight), written or (``accumulate``) added to; None without
-    gains. ``out`` may be ``qkv`` itself. A captured call needs its own
+    gains. ``out`` may be ``qkv`` itself. Columns behind the heads have no
+    gradient: zeros in a new dqkv, left as they were in ``out``. A captured call needs its own
     ``workspace`` (``mfb_qk_rotary_workspace_size(head_dim)`` bytes).
     """
     for x in (dq, dk, dv):
@@ -162,6 +163,8 @@ def qk_rotary_bwd(qkv, positions, freqs, dq, dk, dv, *, head_dim=None, interleav
     if accumulate and (weight_grads is None or any(g is None for g in weight_grads)):
         raise ValueError("accumulate needs weight_grads to add to")
     dqkv = check_out(out, qkv.shape, qkv.dtype, "out")
+    if out is None and ld > (heads + 2 * kv_heads) * d:
+        _lib.call("mfb_memset", dqkv.ptr, 0, dqkv.nbytes, stream)
     dwq = dwk = ws = None
     shared = 0
     if wq is not None:

@@ -128,3 +128,23 @@ def test_queries_that_are_not_numbers(lens, counts, h, hk, dtype):
     np.testing.assert_array_equal(got[~hurt], good[~hurt])
     np.testing.assert_array_equal(lse[~hurt], good_lse[~hurt])
     assert np.all(np.isnan(got[hurt].astype(np.float32))) and np.all(np.isnan(lse[hurt]))
+
+
+def test_gradient_of_columns_behind_the_heads():
+    """Zeros in a new array, over memory that held something else."""
+    require_gpu()
+    from minifield_training_b200 import _lib
+    from minifield_training_b200.device import DeviceArray
+    from minifield_training_b200.kernels import rotary
+
+    rng = np.random.default_rng(16)
+    qkv, grads = normal(rng, (50, 2048 + 24), "bfloat16"), [normal(rng, (50, n, 64), "bfloat16") for n in (16, 8, 8)]
+    freqs, pos = dev(rotary.rotary_frequencies(64, 1e4)[0]), dev(np.arange(50, dtype=np.int32))
+    args = [dev(qkv, "bfloat16"), pos, freqs, *(dev(g, "bfloat16") for g in grads)]
+    for _ in range(3):
+        old = DeviceArray(qkv.shape, "bfloat16")
+        _lib.call("mfb_memset", old.ptr, 0x40, old.nbytes, None)
+        _lib.call("mfb_device_sync")
+        del old  # its memory is the likely place of the next array of this size
+        got = rotary.qk_rotary_bwd(*args, head_dim=64)[0].numpy()
+        assert not np.any(got[:, 2048:].astype(np.float32)) and np.all(np.any(got[:, :2048], 1))

@@ -123,3 +123,17 @@ def test_rotary_backward_adds_only_to_given_gradients(fake, which):
         rotary.qk_rotary_bwd(*args, q_weight=w, k_weight=w, weight_grads=tuple(grads), accumulate=True)
     got = rotary.qk_rotary_bwd(*args, q_weight=w, k_weight=w, weight_grads=tuple(grads))[1:]
     assert got[1 - which] is w and got[which] is not w and got[which].shape == (64,)
+
+
+@pytest.mark.parametrize("extra", [0, 8])
+def test_rotary_backward_clears_columns_without_heads(fake, extra):
+    """A projection may be wider than its heads: the gradient of the rest is zero, in a new array or as given."""
+    qkv, out = array((4, 2048 + extra), "bfloat16"), array((4, 2048 + extra), "bfloat16")
+    args = [qkv, array((4,), "int32"), array((32,), "float32"), array((4, 16, 64), "bfloat16"),
+            array((4, 8, 64), "bfloat16"), array((4, 8, 64), "bfloat16")]
+    rotary.qk_rotary_bwd(*args, head_dim=64, out=out, stream=64)
+    assert "mfb_memset" not in fake.names()
+    dqkv = rotary.qk_rotary_bwd(*args, head_dim=64, stream=64)[0]
+    cleared = [a for name, a in fake.calls if name == "mfb_memset"]
+    assert cleared == ([(dqkv.ptr, 0, 4 * 2056 * 2, 64)] if extra else [])
+    assert [name for name, _ in fake.packed] == ["mfb_qk_rotary_bwd"] * 2
