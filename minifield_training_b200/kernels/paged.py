@@ -39,9 +39,13 @@ class PagedCache:
 
     @classmethod
     def zeros(cls, num_pages, page_size, kv_heads, head_dim, dtype="bfloat16", *, head_major=False):
+        """Pools of zeros that any stream may use once this returns."""
         shape = (num_pages, kv_heads, page_size, head_dim) if head_major else (num_pages, page_size, kv_heads,
                                                                                head_dim)
-        return cls(DeviceArray.zeros(shape, dtype), DeviceArray.zeros(shape, dtype), head_major=head_major)
+        cache = cls(DeviceArray.zeros(shape, dtype), DeviceArray.zeros(shape, dtype), head_major=head_major)
+        # Created streams do not wait for the default one: a first append could run before the clearing.
+        _lib.call("mfb_stream_sync", None)
+        return cache
 
 
 def _sequences(cu_q, seq_lens, page_table, stream):

@@ -137,3 +137,11 @@ def test_rotary_backward_clears_columns_without_heads(fake, extra):
     cleared = [a for name, a in fake.calls if name == "mfb_memset"]
     assert cleared == ([(dqkv.ptr, 0, 4 * 2056 * 2, 64)] if extra else [])
     assert [name for name, _ in fake.packed] == ["mfb_qk_rotary_bwd"] * 2
+
+
+def test_a_new_cache_is_clear_before_any_stream_uses_it(fake):
+    """The clearing runs on the default stream, which created streams do not wait for."""
+    cache = paged.PagedCache.zeros(9, 16, 8, 64)
+    assert fake.names()[-3:] == ["mfb_malloc", "mfb_memset", "mfb_stream_sync"]
+    assert [a[0].value for name, a in fake.calls if name == "mfb_memset"] == [cache.keys.ptr, cache.values.ptr]
+    assert fake.calls[-1][1] == (None,)
