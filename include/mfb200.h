@@ -450,6 +450,8 @@ int mfb_paged_append(const void* qkv, int ld_qkv, const float* wq, const float* 
  * blocks x key tiles of the whole table stay below 2^31. The workspace holds the
  * schedule and the partials; calls that share one must not overlap. */
 size_t mfb_paged_attn_workspace_size(int N, int B, int max_q, int H, int Hk, int D);
+/* What mfb_paged_attn refuses of these sizes, for callers that must know before their own work. */
+int mfb_paged_attn_check(int N, int B, int max_q, int max_pages, int num_pages, int page_size, int H, int Hk, int D);
 int mfb_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* cu_q,
                    const int32_t* seq_lens, const int32_t* page_table, void* o, float* lse, int N, int B, int max_q,
                    int max_pages, int num_pages, int page_size, int H, int Hk, int D, int head_major, int dtype,

@@ -121,6 +121,7 @@ SIGNATURES = {
     "mfb_qk_rotary_bwd": (I, [P, I] + [P] * 10 + [I] * 8 + [F, F, P, SZ, P]),
     "mfb_paged_append": (I, [P, I] + [P] * 9 + [I] * 12 + [F, F, P]),
     "mfb_paged_attn_workspace_size": (SZ, [I] * 6),
+    "mfb_paged_attn_check": (I, [I] * 9),
     "mfb_paged_attn": (I, [P] * 8 + [I] * 11 + [F, P, SZ, P]),
     "mfb_paged_attn_status": (I, [IP]),
     "mfb_logits_process": (I, [P, I, P, I] + [P] * 7 + [I, P, P, I, P, I, I, P]),

@@ -1525,11 +1525,8 @@ extern "C" size_t mfb_paged_attn_workspace_size(int N, int B, int max_q, int H, 
   return paged::plan(N, B, max_q, H, Hk, D).bytes;
 }
 
-extern "C" int mfb_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* cu_q,
-                              const int32_t* seq_lens, const int32_t* page_table, void* o, float* lse, int N, int B,
-                              int max_q, int max_pages, int num_pages, int page_size, int H, int Hk, int D,
-                              int head_major, int dtype, float scale, void* workspace, size_t workspace_bytes,
-                              void* stream) {
+extern "C" int mfb_paged_attn_check(int N, int B, int max_q, int max_pages, int num_pages, int page_size, int H, int Hk,
+                                    int D) {
   MFB_CHECK_ARG(N > 0 && B > 0 && max_q > 0 && max_pages > 0 && num_pages > 0,
                 "paged attention needs tokens, sequences and pages (N=%d B=%d max_q=%d)", N, B, max_q);
   MFB_CHECK_ARG(B <= paged::MAX_B, "paged attention batch %d above the supported %d sequences", B, paged::MAX_B);
@@ -1540,17 +1537,26 @@ extern "C" int mfb_paged_attn(const void* q, const void* k_pages, const void* v_
   MFB_CHECK_ARG(page_size >= 8 && (page_size & (page_size - 1)) == 0,
                 "page_size %d must be a power of two of at least 8", page_size);
   MFB_CHECK_ARG((long long)page_size * Hk * D <= 1 << 30, "page of %d tokens too large", page_size);
-  MFB_CHECK_ARG((long long)max_pages * page_size < (1LL << 31) - 128, "page table spans %lld positions (below 2^31 supported)",
-                (long long)max_pages * page_size);
+  const long long span = (long long)max_pages * page_size;
+  MFB_CHECK_ARG(span < (1LL << 31) - 128, "page table spans %lld positions (below 2^31 supported)", span);
+  MFB_CHECK_ARG(paged::plan(N, B, max_q, H, Hk, D).max_weight(B, Hk, span) < 2147483647.0,
+                "paged attention of %d tokens over tables of %lld positions exceeds 2^31 key tiles", N, span);
+  return MFB_OK;
+}
+
+extern "C" int mfb_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* cu_q,
+                              const int32_t* seq_lens, const int32_t* page_table, void* o, float* lse, int N, int B,
+                              int max_q, int max_pages, int num_pages, int page_size, int H, int Hk, int D,
+                              int head_major, int dtype, float scale, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  int st = mfb_paged_attn_check(N, B, max_q, max_pages, num_pages, page_size, H, Hk, D);
+  if (st) return st;
   MFB_CHECK_ARG(dtype == MFB_DTYPE_BF16 || dtype == MFB_DTYPE_F16, "paged attention dtype must be bf16 or fp16");
   MFB_CHECK_ARG(q && k_pages && v_pages && cu_q && seq_lens && page_table && o, "NULL paged attention argument");
   MFB_CHECK_ARG((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o) & 15) == 0,
                 "q, the pages and o must be 16-byte aligned");
   MFB_CHECK_ARG(isfinite(scale) && scale > 0.f, "paged attention scale must be positive and finite");
   const paged::Plan pl = paged::plan(N, B, max_q, H, Hk, D);
-  MFB_CHECK_ARG(pl.max_weight(B, Hk, (long long)max_pages * page_size) < 2147483647.0,
-                "paged attention of %d tokens over tables of %lld positions exceeds 2^31 key tiles", N,
-                (long long)max_pages * page_size);
   if (!workspace || workspace_bytes < pl.bytes)
     return set_error(MFB_ERR_WORKSPACE, "paged attention workspace needs %zu bytes", pl.bytes);
   MFB_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");

@@ -407,11 +407,14 @@ class Decoder:
         if ids.ndim != 2 or ids.shape[0] != len(rows) or ids.shape[1] <= 0:
             raise ValueError("extend input_ids must have shape [rows, tokens] matching the rows of the state")
         b, t = ids.shape
-        if out is not None and (tuple(out.shape) != (b, cfg.vocab) or out.dtype != "float32"):
-            raise ValueError("out must be a float32 [rows, vocab] device array")
+        if out is not None and (not isinstance(out, DeviceArray) or out.shape != (b, cfg.vocab)
+                                or out.dtype != "float32" or out.ptr % 16):
+            raise ValueError("out must be a 16-byte aligned float32 [rows, vocab] device array")
         if graph and (not s or t != 1):
             raise ValueError("graph replay takes single tokens and needs Decoder(stream=...) from mfb_stream_create")
         controls = self._controls(controls, b)
+        _lib.call("mfb_paged_attn_check", b * t, b, t, state.max_pages, state.num_pages, state.page_size, cfg.heads,
+                  cfg.kv_heads, cfg.head_dim)
         fresh = [row for row in rows if state.lengths[row] == 0]
         B = self._extend_buffers(b, t, state.max_pages)
         logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")

@@ -1,6 +1,7 @@
 """Host side of the rotary, paged-cache and logit operators at their edges (no GPU): a library that only records its calls."""
 
 import ctypes
+import dataclasses
 import math
 import threading
 
@@ -21,6 +22,8 @@ class FakeDevice:
 
     def call(self, name, *args):
         self.calls.append((name, args))
+        if name == "mfb_paged_attn_check":  # arithmetic on the host
+            _lib.check(getattr(_lib.lib(), name)(*args), name)
         if name == "mfb_malloc":
             args[0]._obj.value = self.next
             self.next += -(-int(args[1]) // 256) * 256
@@ -145,3 +148,34 @@ def test_a_new_cache_is_clear_before_any_stream_uses_it(fake):
     assert fake.names()[-3:] == ["mfb_malloc", "mfb_memset", "mfb_stream_sync"]
     assert [a[0].value for name, a in fake.calls if name == "mfb_memset"] == [cache.keys.ptr, cache.values.ptr]
     assert fake.calls[-1][1] == (None,)
+
+
+def decoder(stream=None, **changes):
+    """A decoder (conv, attention, conv, attention) on the recorded library, and its config."""
+    from minifield_training_b200 import workloads
+    from minifield_training_b200.models import decode
+    cfg = dataclasses.replace(workloads.DECODER, **{**dict(
+        hidden=256, ffn=512, heads=4, kv_heads=2, vocab=1000,
+        layer_types=("conv", "full_attention", "conv", "full_attention")), **changes})
+    return decode.Decoder(cfg, decode.init_parameters(cfg, 0), stream=stream), cfg, decode
+
+
+def test_extend_refuses_before_anything_runs(fake):
+    dec, cfg, dm = decoder(max_position_embeddings=1 << 26)
+    state = dm.new_paged_state(cfg, 1, 1 << 20, 64)
+    dec.extend(np.zeros((1, 5), np.int32), state)
+    before = list(state.lengths), state.table.copy(), list(state._free), len(fake.packed)
+    ids = np.zeros((1, 3), np.int32)
+    wide = array((1, cfg.vocab), "float32", ptr=(1 << 20) + 4)
+    for match, call in (
+            ("2.31 key tiles", lambda: dec.extend(np.zeros((1, 1 << 18), np.int32), state)),
+            ("16-byte aligned", lambda: dec.extend(ids, state, out=wide)),
+            ("device array", lambda: dec.extend(ids, state, out=np.zeros((1, cfg.vocab), np.float32)))):
+        with pytest.raises(ValueError, match=match):
+            call()
+        assert (list(state.lengths), list(state._free), len(fake.packed)) == (before[0], before[2], before[3])
+        assert np.array_equal(state.table, before[1])
+    state = dm.new_paged_state(cfg, 2, 4, 1 << 24)  # a page of 2^31 elements is more than the kernels take
+    with pytest.raises(ValueError, match="too large"):
+        dec.extend(np.zeros((2, 1), np.int32), state)
+    assert state.lengths == [0, 0] and len(state._free) == 4
