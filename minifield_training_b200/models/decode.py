@@ -134,9 +134,12 @@ class PagedState:
 
     Every attention layer has a ``paged.PagedCache`` of ``num_pages`` pages of
     ``page_size`` tokens; a row takes pages as it grows, the same ones in every
-    layer, up to ``max_pages`` (default: the whole pool), and gives them back on
-    ``release``. ``lengths`` holds each row's tokens; ``history`` the conv
-    layers' two preceding inputs per row.
+    layer, up to ``max_pages`` (default: what the pool and the model's positions
+    allow), and gives them back on ``release``. ``lengths`` holds each row's
+    tokens; ``table`` its pages (-1 behind them), of which ``device_table`` is a
+    copy that ``upload`` keeps up by the pages taken since, so that a step costs
+    no more for a wide table; ``history`` the conv layers' two preceding inputs
+    per row.
     """
 
     def __init__(self, cfg, batch_size: int, num_pages: int, page_size: int = 64, max_pages: int | None = None):
@@ -149,9 +152,11 @@ class PagedState:
         if page_size < 8 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two of at least 8")
         self.cfg, self.batch, self.page_size, self.num_pages = cfg, batch_size, page_size, num_pages
-        self.max_pages = min(max_pages or num_pages, num_pages)
+        self.max_pages = min(max_pages or num_pages, num_pages, self.pages(cfg.max_position_embeddings))
         self.lengths = [0] * batch_size
         self.table = np.full((batch_size, self.max_pages), -1, np.int32)
+        self.device_table = DeviceArray.from_numpy(self.table)
+        self._taken = []  # (row, first, count) of pages that device_table lacks
         self._free = list(range(num_pages - 1, -1, -1))
         self.caches, self.history = [], []
         for kind in cfg.layer_types:
@@ -182,8 +187,18 @@ class PagedState:
             raise DecodeOverflow(f"{sum(need)} pages needed, {len(self._free)} of {self.num_pages} free")
         for row, count in zip(rows, need):
             held = self.pages(self.lengths[row])
-            self.table[row, held:held + count] = [self._free.pop() for _ in range(count)]
             self.lengths[row] += tokens
+            if count:
+                self.table[row, held:held + count] = [self._free.pop() for _ in range(count)]
+                self._taken.append((row, held, count))
+
+    def upload(self, stream=None) -> None:
+        """Brings ``device_table`` up to the pages taken, in the order of ``stream``."""
+        for row, first, count in self._taken:
+            entries = self.table[row, first:first + count]
+            _lib.call("mfb_memcpy_h2d", P(self.device_table.ptr + (row * self.max_pages + first) * entries.itemsize),
+                      entries.ctypes.data_as(P), entries.nbytes, stream)
+        self._taken.clear()
 
     def release(self, row: int) -> None:
         """Empties ``row`` for a new sequence: its pages go back to the pool."""
@@ -416,20 +431,21 @@ class Decoder:
         _lib.call("mfb_paged_attn_check", b * t, b, t, state.max_pages, state.num_pages, state.page_size, cfg.heads,
                   cfg.kv_heads, cfg.head_dim)
         fresh = [row for row in rows if state.lengths[row] == 0]
-        B = self._extend_buffers(b, t, state.max_pages)
+        B = self._extend_buffers(b, t)
         logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")
         state.grow(rows, t)  # what can fail for lack of memory is behind us
         meta = np.concatenate([ids.reshape(-1).astype(np.int32), np.arange(b + 1, dtype=np.int32) * t,
-                               np.asarray(state.lengths[rows.start:rows.stop], np.int32),
-                               state.table[rows.start:rows.stop].reshape(-1)])
+                               np.asarray(state.lengths[rows.start:rows.stop], np.int32)])
         _lib.call("mfb_memcpy_h2d", P(B["meta"].ptr), meta.ctypes.data_as(P), meta.nbytes, s)
+        state.upload(s)
         for history in state.history:
             if history is not None:
                 nbytes = history.nbytes // state.batch
                 for row in fresh:
                     _lib.call("mfb_memset", P(history.ptr + row * nbytes), 0, nbytes, s)
         if graph:
-            key = ("paged", b, rows.start, state.max_pages, state.num_pages, state.page_size) + tuple(
+            key = ("paged", b, rows.start, state.max_pages, state.num_pages, state.page_size,
+                   state.device_table.ptr) + tuple(
                 h.ptr if c is None else (c.keys.ptr, c.values.ptr) for c, h in zip(state.caches, state.history))
             g = self._graphs.get(key)
             if g is None:
@@ -451,7 +467,8 @@ class Decoder:
         c, f, h, hk, hd = cfg.hidden, cfg.ffn, cfg.heads, cfg.kv_heads, cfg.head_dim
         m, nq = b * t, (h + 2 * hk) * hd
         ids_d, cu = B["meta"].view(0, (m,)), B["meta"].view(m, (b + 1,))
-        lens, table = B["meta"].view(m + b + 1, (b,)), B["meta"].view(m + 2 * b + 1, (b, state.max_pages))
+        lens = B["meta"].view(m + b + 1, (b,))
+        table = state.device_table.view(rows.start * state.max_pages, (b, state.max_pages))
 
         def proj(x, w, y, n, k):
             if m <= 64:
@@ -501,12 +518,12 @@ class Decoder:
         else:
             _fwd(B["last"], self.head, B["logits16"], b, cfg.vocab, c, s)
 
-    def _extend_buffers(self, b: int, t: int, max_pages: int):
-        """Scratch of ``extend`` for b x t tokens, kept per batch, power of two that holds t, and table width."""
+    def _extend_buffers(self, b: int, t: int):
+        """Scratch of ``extend`` for b x t tokens, kept per batch and power of two that holds t."""
         cfg, E = self.cfg, DeviceArray
         c, f, h, hk, hd = cfg.hidden, cfg.ffn, cfg.heads, cfg.kv_heads, cfg.head_dim
         bucket = 1 << (t - 1).bit_length()
-        key, n, nq = (b, bucket, max_pages), b * bucket, (h + 2 * hk) * hd
+        key, n, nq = (b, bucket), b * bucket, (h + 2 * hk) * hd
         B = self._extend_scratch.get(key)
         if B is None:
             def bf(cols, rows=n):
@@ -517,7 +534,7 @@ class Decoder:
                 (3 * c, c), (c, c), (nq, c), (c, h * hd), (2 * f, c), (c, f))]
             gemm.append(int(size(min(b, 64), cfg.vocab, c)))
             B = self._extend_scratch[key] = dict(
-                meta=E((n + 2 * b + 1 + b * max_pages,), "int32"), x=bf(c), xb=bf(c), hn=bf(c),
+                meta=E((n + 2 * b + 1,), "int32"), x=bf(c), xb=bf(c), hn=bf(c),
                 proj=E((n * max(3 * c, nq),), "bfloat16"), mixed=bf(c), tail=bf((cfg.conv_kernel - 1) * c, b),
                 r=bf(c), mid=bf(c), h2=bf(c), gu=bf(2 * f), a=bf(f), y=bf(c), q=bf(h * hd), o=bf(h * hd),
                 rstd=E((n,), "float32"), enc=bf(c), last=bf(c, b), logits16=bf(cfg.vocab, b),

@@ -179,3 +179,30 @@ def test_extend_refuses_before_anything_runs(fake):
     with pytest.raises(ValueError, match="too large"):
         dec.extend(np.zeros((2, 1), np.int32), state)
     assert state.lengths == [0, 0] and len(state._free) == 4
+
+
+def test_a_step_uploads_its_tokens_and_the_pages_it_took(fake):
+    """Not the whole table, however wide; rows are no wider than the model's positions."""
+    dec, cfg, dm = decoder(max_position_embeddings=6400)
+    state = dm.new_paged_state(cfg, 4, 1 << 16, 64)
+    assert state.max_pages == 100 and dm.new_paged_state(cfg, 4, 30, 64).max_pages == 30
+
+    def uploads(call):
+        start = len(fake.calls)
+        call()
+        return [(a[0].value, a[2]) for name, a in fake.calls[start:] if name == "mfb_memcpy_h2d"]
+
+    def step(t, rows=None):
+        return uploads(lambda: dec.extend(np.zeros((len(rows or range(4)), t), np.int32), state, rows=rows))
+
+    at = state.device_table.ptr
+    assert step(130)[1:] == [(at + 400 * row, 12) for row in range(4)]  # three pages each
+    first = step(1)
+    assert len(first) == 1 and first[0][1] == 4 * (4 + 5 + 4)  # tokens, offsets, lengths
+    step(60, range(1, 2))
+    assert step(2, range(1, 2))[1:] == [(at + 400 + 12, 4)]  # the 193rd token's page
+    assert at + 400 in fake.packed[-1][1]  # attention reads the rows' part of the table in place
+    state.release(1)
+    assert step(1, range(1, 2))[1:] == [(at + 400, 4)]
+    state.grow(range(2, 3), 126)  # 131 tokens before, 257 now: pages 3 and 4
+    assert uploads(lambda: state.upload(5)) == [(at + 800 + 12, 8)] and uploads(state.upload) == []
