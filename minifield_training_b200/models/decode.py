@@ -431,7 +431,7 @@ class Decoder:
         _lib.call("mfb_paged_attn_check", b * t, b, t, state.max_pages, state.num_pages, state.page_size, cfg.heads,
                   cfg.kv_heads, cfg.head_dim)
         fresh = [row for row in rows if state.lengths[row] == 0]
-        B = self._extend_buffers(b, t)
+        B = self._extend_buffers(b, t, graph)
         logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")
         state.grow(rows, t)  # what can fail for lack of memory is behind us
         meta = np.concatenate([ids.reshape(-1).astype(np.int32), np.arange(b + 1, dtype=np.int32) * t,
@@ -459,7 +459,7 @@ class Decoder:
             _lib.call("mfb_graph_launch", P(g), P(s))
         else:
             self._extend_layers(B, state, rows, t)
-        return self._widen(B["logits16"], logits, controls)
+        return self._widen(B["logits16"].view(0, (b, cfg.vocab)), logits, controls)
 
     def _extend_layers(self, B, state: PagedState, rows, t: int):
         """Every layer over the ``t`` uploaded tokens of ``rows``; bf16 logits of the last ones in B["logits16"]."""
@@ -518,28 +518,38 @@ class Decoder:
         else:
             _fwd(B["last"], self.head, B["logits16"], b, cfg.vocab, c, s)
 
-    def _extend_buffers(self, b: int, t: int):
-        """Scratch of ``extend`` for b x t tokens, kept per batch and power of two that holds t."""
+    def _extend_buffers(self, b: int, t: int, graph: bool = False):
+        """Scratch of ``extend`` for b x t tokens.
+
+        Calls are serial on the decoder's stream, so one set serves them all and
+        grows (by powers of two of tokens and of rows) to the largest. A captured
+        step needs buffers that stay: a set of its own per power of two of rows.
+        """
         cfg, E = self.cfg, DeviceArray
         c, f, h, hk, hd = cfg.hidden, cfg.ffn, cfg.heads, cfg.kv_heads, cfg.head_dim
-        bucket = 1 << (t - 1).bit_length()
-        key, n, nq = (b, bucket), b * bucket, (h + 2 * hk) * hd
+        r, n, nq = 1 << (b - 1).bit_length(), 1 << (b * t - 1).bit_length(), (h + 2 * hk) * hd
+        key = r if graph else None
         B = self._extend_scratch.get(key)
-        if B is None:
+        if B is None or B["rows"] < r or B["tokens"] < n:
+            if B is not None:
+                r, n = max(r, B["rows"]), max(n, B["tokens"])
+                B = None
+                del self._extend_scratch[key]  # before the larger one is allocated
+
             def bf(cols, rows=n):
                 return E((rows, cols), "bfloat16")
 
             size = _lib.lib().mfb_gemm_workspace_size
             gemm = [int(size(min(n, 64), w, k)) for w, k in (
                 (3 * c, c), (c, c), (nq, c), (c, h * hd), (2 * f, c), (c, f))]
-            gemm.append(int(size(min(b, 64), cfg.vocab, c)))
+            gemm.append(int(size(min(r, 64), cfg.vocab, c)))
             B = self._extend_scratch[key] = dict(
-                meta=E((n + 2 * b + 1,), "int32"), x=bf(c), xb=bf(c), hn=bf(c),
-                proj=E((n * max(3 * c, nq),), "bfloat16"), mixed=bf(c), tail=bf((cfg.conv_kernel - 1) * c, b),
+                rows=r, tokens=n, meta=E((n + 2 * r + 1,), "int32"), x=bf(c), xb=bf(c), hn=bf(c),
+                proj=E((n * max(3 * c, nq),), "bfloat16"), mixed=bf(c), tail=bf((cfg.conv_kernel - 1) * c, r),
                 r=bf(c), mid=bf(c), h2=bf(c), gu=bf(2 * f), a=bf(f), y=bf(c), q=bf(h * hd), o=bf(h * hd),
-                rstd=E((n,), "float32"), enc=bf(c), last=bf(c, b), logits16=bf(cfg.vocab, b),
+                rstd=E((n,), "float32"), enc=bf(c), last=bf(c, r), logits16=bf(cfg.vocab, r),
                 gemm_ws=E((max(*gemm, 16),), "uint8"), ws=E((16,), "uint8"))
-        need = paged.paged_attention_workspace_size(b * t, b, t, h, hk, hd)
+        need = paged.paged_attention_workspace_size(n if graph else b * t, r if graph else b, t, h, hk, hd)
         if B["ws"].nbytes < need:
             B["ws"] = E((need,), "uint8")
         return B
@@ -653,11 +663,12 @@ class Decoder:
             _lib.call("mfb_cast_bf16_f32", P(B["logits16"].ptr), P(logits.ptr), b * cfg.vocab, s)
 
     def close(self):
-        """Release the captured decode graphs."""
+        """Release the captured decode graphs and the scratch of ``extend``."""
         graphs, self._graphs = getattr(self, "_graphs", {}), {}
         for g in graphs.values():
             if _lib._lib is not None:
                 _lib.lib().mfb_graph_destroy(P(g))
+        self._extend_scratch = {}
 
     def __del__(self):
         try:

@@ -17,7 +17,7 @@ class FakeDevice:
     """Answers the runtime calls: memory is a counter, streams have the ids given to them, nothing else runs."""
 
     def __init__(self):
-        self.calls, self.packed, self.next, self.freed = [], [], 1 << 20, []
+        self.calls, self.packed, self.next, self.live = [], [], 1 << 20, {}
         self.current, self.ids, self.capturing = 0, {}, set()
 
     def call(self, name, *args):
@@ -26,7 +26,10 @@ class FakeDevice:
             _lib.check(getattr(_lib.lib(), name)(*args), name)
         if name == "mfb_malloc":
             args[0]._obj.value = self.next
+            self.live[self.next] = int(args[1])
             self.next += -(-int(args[1]) // 256) * 256
+        elif name == "mfb_graph_end":
+            args[1]._obj.value = 1
         elif name == "mfb_stream_identity":
             handle = getattr(args[0], "value", args[0])
             args[1][0], args[1][1] = self.current, self.ids.get((self.current, handle), handle or 1)
@@ -45,7 +48,7 @@ def fake(monkeypatch):
     f = FakeDevice()
     monkeypatch.setattr(_lib, "call", f.call)
     monkeypatch.setattr(_lib, "call_packed", f.call_packed)
-    monkeypatch.setattr(DeviceArray, "__del__", lambda self: f.freed.append(self.ptr) if self._owner else None)
+    monkeypatch.setattr(DeviceArray, "__del__", lambda self: f.live.pop(self.ptr) if self._owner else None)
     monkeypatch.setattr(device, "_STREAM_WORKSPACES", {})
     return f
 
@@ -206,3 +209,34 @@ def test_a_step_uploads_its_tokens_and_the_pages_it_took(fake):
     assert step(1, range(1, 2))[1:] == [(at + 400, 4)]
     state.grow(range(2, 3), 126)  # 131 tokens before, 257 now: pages 3 and 4
     assert uploads(lambda: state.upload(5)) == [(at + 800 + 12, 8)] and uploads(state.upload) == []
+
+
+def test_scratch_of_extend_is_bounded(fake):
+    """One set for all calls, as large as the largest needed, and one per power of two of rows for captured steps."""
+    dec, cfg, dm = decoder(stream=64)
+    state = dm.new_paged_state(cfg, 64, 64 * 80, 64)
+    rng = np.random.default_rng(17)
+
+    def call(b, t, graph=False):
+        for row in range(b):
+            state.release(row)
+        dec.extend(np.zeros((b, t), np.int32), state, rows=range(b), graph=graph)
+        return sum(fake.live.values())
+
+    start = sum(fake.live.values())
+    largest = call(64, 512) - start
+    dec.close()
+    assert sum(fake.live.values()) == start
+    for b, t in [(int(b), int(t)) for b, t in zip(rng.integers(1, 65, 60), 2 ** rng.integers(0, 9, 60))]:
+        assert call(b, t) - start <= largest
+    assert call(64, 512) - start == largest
+    for b in range(1, 65):
+        call(b, 1, graph=True)
+    assert len(dec._extend_scratch) == 1 + 7
+    kept = {id(B): {k: getattr(v, "ptr", v) for k, v in B.items()} for B in dec._extend_scratch.values()}
+    for b in (64, 3, 17):
+        call(b, 1, graph=True)  # a captured step's buffers stay where they are
+    assert kept == {id(B): {k: getattr(v, "ptr", v) for k, v in B.items()} for B in dec._extend_scratch.values()}
+    dec._graphs.clear()  # handles of the recorded library
+    dec.close()
+    assert sum(fake.live.values()) == start
