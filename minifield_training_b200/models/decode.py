@@ -430,7 +430,13 @@ class Decoder:
         controls = self._controls(controls, b)
         _lib.call("mfb_paged_attn_check", b * t, b, t, state.max_pages, state.num_pages, state.page_size, cfg.heads,
                   cfg.kv_heads, cfg.head_dim)
-        fresh = [row for row in rows if state.lengths[row] == 0]
+        fresh = []  # [first, count] of neighbouring rows that begin a sequence
+        for row in rows:
+            if state.lengths[row] == 0:
+                if fresh and sum(fresh[-1]) == row:
+                    fresh[-1][1] += 1
+                else:
+                    fresh.append([row, 1])
         B = self._extend_buffers(b, t, graph)
         logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")
         state.grow(rows, t)  # what can fail for lack of memory is behind us
@@ -441,8 +447,8 @@ class Decoder:
         for history in state.history:
             if history is not None:
                 nbytes = history.nbytes // state.batch
-                for row in fresh:
-                    _lib.call("mfb_memset", P(history.ptr + row * nbytes), 0, nbytes, s)
+                for first, count in fresh:
+                    _lib.call("mfb_memset", P(history.ptr + first * nbytes), 0, count * nbytes, s)
         if graph:
             key = ("paged", b, rows.start, state.max_pages, state.num_pages, state.page_size,
                    state.device_table.ptr) + tuple(

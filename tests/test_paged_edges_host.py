@@ -240,3 +240,21 @@ def test_scratch_of_extend_is_bounded(fake):
     dec._graphs.clear()  # handles of the recorded library
     dec.close()
     assert sum(fake.live.values()) == start
+
+
+def test_neighbouring_fresh_rows_are_cleared_together(fake):
+    dec, cfg, dm = decoder()
+    state = dm.new_paged_state(cfg, 8, 64, 64)
+    row = 2 * 256 * 2  # bytes of a row's two conv inputs
+    layers = [h.ptr for h in state.history if h is not None]
+
+    def cleared(rows):
+        start = len(fake.calls)
+        dec.extend(np.zeros((len(rows), 3), np.int32), state, rows=rows)
+        return [(a[0].value, a[2]) for name, a in fake.calls[start:] if name == "mfb_memset"]
+
+    assert cleared(range(0, 8)) == [(p, 8 * row) for p in layers]
+    assert cleared(range(0, 8)) == []
+    for r in (1, 2, 5, 7):
+        state.release(r)
+    assert cleared(range(1, 7)) == [(p + r * row, n * row) for p in layers for r, n in ((1, 2), (5, 1))]
