@@ -581,8 +581,9 @@ class Decoder:
         captured on the first call for this state's caches (needs a created
         stream); the step reads its token ids, positions and lengths from
         device buffers uploaded before each replay, so one graph serves every
-        step. ``controls``: keyword arguments of kernels.logits.process_logits
-        for the returned logits.
+        step (and one every step with controls, which apply behind the replay).
+        ``controls``: keyword arguments of kernels.logits.process_logits for the
+        returned logits.
         """
         cfg, s = self.cfg, self.stream
         if state.cfg != cfg:
@@ -608,13 +609,13 @@ class Decoder:
         _lib.call("mfb_memcpy_h2d", P(B["meta"].ptr), meta.ctypes.data_as(P), meta.nbytes, s)
         logits = out if out is not None else DeviceArray((b, cfg.vocab), "float32")
         if graph:
-            key = (b, state.capacity) + tuple(a.ptr for a in (*state.keys, *state.values, *state.history)
-                                               if a is not None)
+            key = (b, state.capacity, controls is None) + tuple(a.ptr for a in (*state.keys, *state.values, *state.history)
+                                                                if a is not None)
             g = self._graphs.get(key)
             if g is None:
                 _lib.call("mfb_graph_begin", P(s))
                 try:
-                    self._step(B, state, B["logits"])
+                    self._step(B, state, B["logits"] if controls is None else None)
                 finally:
                     g_ = P()
                     _lib.call("mfb_graph_end", P(s), ctypes.byref(g_))

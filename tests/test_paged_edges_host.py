@@ -258,3 +258,19 @@ def test_neighbouring_fresh_rows_are_cleared_together(fake):
     for r in (1, 2, 5, 7):
         state.release(r)
     assert cleared(range(1, 7)) == [(p + r * row, n * row) for p in layers for r, n in ((1, 2), (5, 1))]
+
+
+def test_a_captured_step_with_controls_widens_its_logits_once(fake):
+    dec, cfg, dm = decoder(stream=64)
+    state, ids = dm.new_state(cfg, 2, 16), np.zeros(2, np.int32)
+    bias = dict(bias_ids=array((2, 1), "int32"), bias_values=array((2, 1), "float32"))
+    done = []
+    for controls in (None, bias, bias, None):
+        start = len(fake.calls), len(fake.packed)
+        dec.decode_one(ids, state, graph=True, controls=controls)
+        names = [name for name, _ in fake.calls[start[0]:]]
+        done.append((names.count("mfb_cast_bf16_f32"), names.count("mfb_graph_begin"),
+                     [name for name, _ in fake.packed[start[1]:]]))
+    dec._graphs.clear()  # handles of the recorded library
+    controlled = ["mfb_logits_process"]
+    assert done == [(1, 1, []), (0, 1, controlled), (0, 0, controlled), (0, 0, [])]
