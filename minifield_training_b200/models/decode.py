@@ -174,7 +174,9 @@ class PagedState:
 
     def grow(self, rows, tokens: int) -> None:
         """Takes the pages for ``tokens`` more tokens of each of ``rows``, or none at all (DecodeOverflow)."""
-        need = []
+        rows, need = list(rows), []
+        if tokens <= 0 or len(set(rows)) != len(rows) or any(not 0 <= row < self.batch for row in rows):
+            raise ValueError(f"pages go to distinct rows of the batch of {self.batch}, for a positive number of tokens")
         for row in rows:
             total = self.lengths[row] + tokens
             if total > self.cfg.max_position_embeddings:

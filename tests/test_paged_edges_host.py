@@ -274,3 +274,14 @@ def test_a_captured_step_with_controls_widens_its_logits_once(fake):
     dec._graphs.clear()  # handles of the recorded library
     controlled = ["mfb_logits_process"]
     assert done == [(1, 1, []), (0, 1, controlled), (0, 0, controlled), (0, 0, [])]
+
+
+@pytest.mark.parametrize("rows, tokens", [((0, 0), 10), ((-1,), 3), ((2,), 3), ((0,), 0), ((1,), -2)])
+def test_pages_go_to_distinct_rows(fake, rows, tokens):
+    """A row named twice took the pages of its first growth again and left others with no owner."""
+    _, cfg, dm = decoder()
+    state = dm.new_paged_state(cfg, 2, 8, 8)
+    state.grow((0, 1), 5)
+    with pytest.raises(ValueError, match="distinct rows"):
+        state.grow(rows, tokens)
+    assert state.lengths == [5, 5] and len(state._free) == 6
