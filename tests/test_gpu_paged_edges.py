@@ -148,3 +148,28 @@ def test_gradient_of_columns_behind_the_heads():
         del old  # its memory is the likely place of the next array of this size
         got = rotary.qk_rotary_bwd(*args, head_dim=64)[0].numpy()
         assert not np.any(got[:, 2048:].astype(np.float32)) and np.all(np.any(got[:, :2048], 1))
+
+
+@pytest.mark.parametrize("batch, counts, h, hk, page, dtype", [
+    (1300, (0, 1, 1, 2), 4, 2, 8, "bfloat16"),  # few rows: several items per thread of a CTA's own schedule
+    (700, (1,), 6, 3, 16, "float16"),  # three head groups per sequence
+    (1500, (0, 1, 3, 20), 2, 1, 16, "bfloat16"),  # tiles: more sequences and items than the schedule kernel has threads
+    (131, (129,), 8, 4, 64, "float16"),  # two query blocks per head: 1048 items
+])
+def test_more_items_and_sequences_than_threads(batch, counts, h, hk, page, dtype):
+    """Against float64, and bit for bit the same again (cut items are joined in share order)."""
+    require_gpu()
+    from minifield_training_b200.kernels import paged
+
+    rng = np.random.default_rng(batch)
+    count = rng.choice(counts, batch)
+    lens = count + rng.integers(0, 40, batch) - rng.integers(0, 2, batch) * (count > 1)
+    lens[rng.integers(0, batch, 3)] += 2500  # long ones are cut between CTAs
+    a = build(rng, [int(n) for n in lens], [int(n) for n in count], h, hk, 64, page, False, dtype, pad=3)
+    paged.paged_attention_status()
+    got, lse = run_attention(*a, False, dtype, max(counts))
+    assert paged.paged_attention_status() == 0
+    check_attention(got, lse, *a, False, dtype, 0.125)
+    again, lse2 = run_attention(*a, False, dtype, max(counts))
+    np.testing.assert_array_equal(again.view(np.uint16), got.view(np.uint16))
+    np.testing.assert_array_equal(lse2, lse)

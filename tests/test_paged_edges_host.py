@@ -278,7 +278,7 @@ def test_a_captured_step_with_controls_widens_its_logits_once(fake):
 
 @pytest.mark.parametrize("rows, tokens", [((0, 0), 10), ((-1,), 3), ((2,), 3), ((0,), 0), ((1,), -2)])
 def test_pages_go_to_distinct_rows(fake, rows, tokens):
-    """A row named twice took the pages of its first growth again and left others with no owner."""
+    """The pages of a row named twice were counted from its first length both times: fewer than its tokens need."""
     _, cfg, dm = decoder()
     state = dm.new_paged_state(cfg, 2, 8, 8)
     state.grow((0, 1), 5)
