@@ -530,12 +530,18 @@ class Decoder:
         """Scratch of ``extend`` for b x t tokens.
 
         Calls are serial on the decoder's stream, so one set serves them all and
-        grows (by powers of two of tokens and of rows) to the largest. A captured
-        step needs buffers that stay: a set of its own per power of two of rows.
+        grows to the largest, in steps of an eighth at most. A captured step needs
+        buffers that stay: a set of its own per power of two of rows.
         """
         cfg, E = self.cfg, DeviceArray
         c, f, h, hk, hd = cfg.hidden, cfg.ffn, cfg.heads, cfg.kv_heads, cfg.head_dim
-        r, n, nq = 1 << (b - 1).bit_length(), 1 << (b * t - 1).bit_length(), (h + 2 * hk) * hd
+        nq = (h + 2 * hk) * hd
+
+        def rounded(x):
+            step = max((1 << (x - 1).bit_length()) >> 4, 1)
+            return -(-x // step) * step
+
+        r, n = (rounded(b), rounded(b * t)) if not graph else (1 << (b - 1).bit_length(),) * 2
         key = r if graph else None
         B = self._extend_scratch.get(key)
         if B is None or B["rows"] < r or B["tokens"] < n:

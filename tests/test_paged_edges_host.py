@@ -240,6 +240,11 @@ def test_scratch_of_extend_is_bounded(fake):
     dec._graphs.clear()  # handles of the recorded library
     dec.close()
     assert sum(fake.live.values()) == start
+    for b, t in ((33, 512), (1, 1000), (64, 17), (7, 1)):
+        dec.close()
+        call(b, t)
+        B = dec._extend_scratch[None]
+        assert b * t <= B["tokens"] <= 1.125 * b * t and b <= B["rows"] <= 1.125 * b
 
 
 def test_neighbouring_fresh_rows_are_cleared_together(fake):
