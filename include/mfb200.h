@@ -78,10 +78,11 @@ int mfb_graph_launch(void* graph_exec, void* stream);
 int mfb_graph_destroy(void* graph_exec);
 /* 1 while `stream` records a graph (between mfb_graph_begin and mfb_graph_end, or any other stream capture). */
 int mfb_stream_is_capturing(void* stream, int* capturing);
-/* identity[0]: the current device; identity[1]: the stream's id, which no other stream of the process ever has
- * (a handle comes again: the default streams' on every device and thread, a destroyed stream's on a new one), or 0
- * while the stream records a graph. */
-int mfb_stream_identity(void* stream, uint64_t* identity);
+/* A number for the current device and the stream, which no other stream of the process ever has (a handle comes
+ * again: the default streams' on every device and thread, a destroyed stream's on a new one): the device plus one
+ * from bit 48 up, the stream's id below. 0 while the stream records a graph; MFB_NO_STREAM on an error. */
+#define MFB_NO_STREAM UINT64_MAX
+uint64_t mfb_stream_identity(void* stream);
 
 /* ---- fake quantization ----------------------------------------------------
  * Replaces Quantizer.effective (src/minifield_training/kernels/quantization.py:11-22,

@@ -81,7 +81,7 @@ SIGNATURES = {
     "mfb_graph_launch": (I, [P, P]),
     "mfb_graph_destroy": (I, [P]),
     "mfb_stream_is_capturing": (I, [P, IP]),
-    "mfb_stream_identity": (I, [P, ctypes.POINTER(ctypes.c_uint64)]),
+    "mfb_stream_identity": (ctypes.c_uint64, [P]),
     "mfb_adamw_workspace_size": (SZ, []),
     "mfb_adamw_commit": (I, [P, P, P, P, LL, LL, LL, P, P, P, P, F, F, F, F, F, F, P, P, SZ, P]),
     "mfb_adamw_shard_pass": (I, [I, P, P, P, P, LL, LL, LL, LL, LL, P, P, P, P, F, F, F, F, F, F, P, P, P, SZ, P]),
@@ -132,6 +132,7 @@ SIGNATURES = {
     "mfb_logits_process_packed": (I, [ctypes.c_char_p]),
 }
 PACKED_SHARED_WORKSPACE = 1
+NO_STREAM = (1 << 64) - 1
 # Slot formats of the packed entry points: flags, then the plain one's arguments.
 _SLOTS = {P: "Q", SZ: "Q", I: "q", LL: "q", F: "d"}
 _PACK = {name: struct.Struct("=q" + "".join(_SLOTS[a] for a in SIGNATURES[name][1])).pack
@@ -177,6 +178,14 @@ def call(name: str, *args):
     status = getattr(_lib or lib(), name)(*args)
     if status:
         check(status, name)
+
+
+def stream_identity(stream) -> int:
+    """``mfb_stream_identity``: of the current device and stream, 0 while the stream records a graph."""
+    identity = (_lib or lib()).mfb_stream_identity(stream)
+    if identity == NO_STREAM:
+        check(ERR_CUDA, "mfb_stream_identity")
+    return identity
 
 
 def call_packed(name: str, flags: int, *args, stream=None):

@@ -206,17 +206,18 @@ int mfb_stream_is_capturing(void* stream, int* capturing) {
   return MFB_OK;
 }
 
-int mfb_stream_identity(void* stream, uint64_t* identity) {
-  MFB_CHECK_ARG(identity != nullptr, "identity is NULL");
+uint64_t mfb_stream_identity(void* stream) {
   int device = 0, capturing = 0;
   unsigned long long id = 0;
-  MFB_CUDA_TRY(cudaGetDevice(&device));
-  const int st = mfb_stream_is_capturing(stream, &capturing);
-  if (st) return st;
-  if (!capturing) MFB_CUDA_TRY(cudaStreamGetId((cudaStream_t)stream, &id));  // not answered during a capture
-  identity[0] = (uint64_t)device;
-  identity[1] = id;
-  return MFB_OK;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && mfb_stream_is_capturing(stream, &capturing)) return MFB_NO_STREAM;
+  if (capturing) return 0;
+  if (e == cudaSuccess) e = cudaStreamGetId((cudaStream_t)stream, &id);  // not answered during a capture
+  if (e != cudaSuccess) {
+    mfb::cuda_error(e, "mfb_stream_identity");
+    return MFB_NO_STREAM;
+  }
+  return (uint64_t)(device + 1) << 48 | id;
 }
 
 int mfb_graph_destroy(void* graph_exec) {

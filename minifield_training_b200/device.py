@@ -216,19 +216,17 @@ def stream_workspace(tag: str, nbytes: int, stream=None) -> DeviceArray:
     A call recorded into a CUDA graph must not use it (the graph outlives the
     call and may replay beside later ones): it is refused here.
     """
-    identity = (ctypes.c_uint64 * 2)()
-    _lib.call("mfb_stream_identity", stream, identity)
-    device, stream_id = identity
-    if not stream_id:
+    identity = _lib.stream_identity(stream)
+    if not identity:
         raise ValueError(f"a captured {tag} call needs its own workspace (workspace=)")
     handle = getattr(stream, "value", stream) or _LEGACY_STREAM
-    key = (tag, device, handle, threading.get_ident() if handle == _PER_THREAD_STREAM else None)
+    key = (tag, identity >> 48, handle, threading.get_ident() if handle == _PER_THREAD_STREAM else None)
     entry = _STREAM_WORKSPACES.get(key)
-    if entry is not None and entry[2] != stream_id:
+    if entry is not None and entry[2] != identity:
         entry = None
     if entry is None or entry[1] < nbytes:
         size = max(int(nbytes), 2 * entry[1] if entry else 256)
-        entry = _STREAM_WORKSPACES[key] = (DeviceArray((size,), "uint8"), size, stream_id)
+        entry = _STREAM_WORKSPACES[key] = (DeviceArray((size,), "uint8"), size, identity)
     return entry[0]
 
 

@@ -71,12 +71,9 @@ def test_streams_have_identities_of_their_own():
     require_gpu()
     from minifield_training_b200 import _lib
 
-    def identity(stream):
-        out = (ctypes.c_uint64 * 2)()
-        _lib.call("mfb_stream_identity", stream, out)
-        return out[0], out[1]
-
+    identity = _lib.stream_identity
     default = identity(None)
+    assert default >> 48 == 1  # device 0
     seen, word = {default}, dev(np.zeros(1, np.int32))
     for _ in range(20):
         s = ctypes.c_void_p()
@@ -84,7 +81,7 @@ def test_streams_have_identities_of_their_own():
         assert identity(s.value) not in seen and identity(s.value) == identity(s.value)
         seen.add(identity(s.value))
         _lib.call("mfb_graph_begin", s.value)
-        assert identity(s.value) == (default[0], 0) and identity(None) == default
+        assert identity(s.value) == 0 and identity(None) == default
         _lib.call("mfb_memset", word.ptr, 0, 4, s.value)
         g = ctypes.c_void_p()
         _lib.call("mfb_graph_end", s.value, ctypes.byref(g))

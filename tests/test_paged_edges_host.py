@@ -30,11 +30,11 @@ class FakeDevice:
             self.next += -(-int(args[1]) // 256) * 256
         elif name == "mfb_graph_end":
             args[1]._obj.value = 1
-        elif name == "mfb_stream_identity":
-            handle = getattr(args[0], "value", args[0])
-            args[1][0], args[1][1] = self.current, self.ids.get((self.current, handle), handle or 1)
-            if handle in self.capturing:
-                args[1][1] = 0
+
+    def stream_identity(self, stream):
+        handle = getattr(stream, "value", stream)
+        number = self.ids.get((self.current, handle), handle or 1)
+        return 0 if handle in self.capturing else (self.current + 1 << 48) + number
 
     def call_packed(self, name, flags, *args, stream=None):
         self.packed.append((name, args))
@@ -48,6 +48,7 @@ def fake(monkeypatch):
     f = FakeDevice()
     monkeypatch.setattr(_lib, "call", f.call)
     monkeypatch.setattr(_lib, "call_packed", f.call_packed)
+    monkeypatch.setattr(_lib, "stream_identity", f.stream_identity)
     monkeypatch.setattr(DeviceArray, "__del__", lambda self: f.live.pop(self.ptr) if self._owner else None)
     monkeypatch.setattr(device, "_STREAM_WORKSPACES", {})
     return f
