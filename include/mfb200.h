@@ -457,7 +457,7 @@ int mfb_paged_attn(const void* q, const void* k_pages, const void* v_pages, cons
                    const int32_t* seq_lens, const int32_t* page_table, void* o, float* lse, int N, int B, int max_q,
                    int max_pages, int num_pages, int page_size, int H, int Hk, int D, int head_major, int dtype,
                    float scale, void* workspace, size_t workspace_bytes, void* stream);
-/* Reads (and clears) the paged attention's device status word: 0 = ok, 1001 = a
+/* Reads (and clears) the paged attention's status word, one per device for all its callers: 0 = ok, 1001 = a
  * page id outside the pool, 1002 = lengths that contradict each other, else the
  * id of a bounded pipeline wait that gave up. Synchronous. */
 int mfb_paged_attn_status(int* code);

@@ -75,7 +75,6 @@ struct Params {
   int tok_item;    // query tokens per item
   int hc;          // KV heads per item
   int unit;        // keys per unit
-  int min_share;   // weight a share should hold at least
   int grid, max_items, part_rows;
   float scale_log2;
 };
@@ -124,10 +123,17 @@ __device__ __forceinline__ I block_scan(I v, I* warp_sums, I* sum) {
   return incl - v + (warp ? warp_sums[warp - 1] : 0);
 }
 
+// Weight a share holds at least, in either kernel: a cut costs its partials and
+// their join, a long share leaves SMs idle. Rows, with 1, 2, 4, 8 and 16: one token
+// over 200 keys 12.2, 12.5, 14.3, 18.3, 18.4 us; over 4000 14.5, 14.1, 14.5, 17.7,
+// 22.6; 8 over up to 3000 16.6, 16.6, 16.8, 18.6, 24.6; 64 over up to 4096 58.5 in
+// all. Tiles, with 2, 4, 8 and 16: 64 tokens over 300 keys 18.5, 20.6, 26.8, 43.4;
+// 4 x 64 over 2000 21.7, 20.4, 22.7, 26.6; nine ragged chunks 38.9, 38.8, 38.9, 44.6.
+constexpr int MIN_SHARE = 4;
 __device__ __forceinline__ Header cut(const Params& p, int total) {
   Header h;
   h.total = total;
-  h.shares = max(1, min(p.grid, total / p.min_share));
+  h.shares = max(1, min(p.grid, total / MIN_SHARE));
   h.base = total / h.shares;
   h.rest = total - h.base * h.shares;
   h.cuts = h.pad[0] = h.pad[1] = h.pad[2] = 0;
@@ -376,6 +382,8 @@ __global__ void __launch_bounds__(JOIN_THREADS, 4) join_kernel(Params p) {
   const int rows = w.ntok * p.G * p.hc, per = cdiv(rows, chunks), r0 = chunk * per, r1 = min(rows, r0 + per);
   if (r0 >= r1) return;
   const int c0 = share_of(h, w.first), n = share_of(h, last_weight(w)) - c0 + 1;
+  // The last form for all: 159.5 instead of 155.2 us for two 2048-token chunks, 36.9
+  // instead of 35.0 for 20 ragged ones; without the middle one 154.9 and 37.0.
   if (n <= 2) join_rows<T, D, ROWS32, 4, 2>(p, h, w, c0, n, r0, r1, s_o, s_ml);
   else if (n <= 4) join_rows<T, D, ROWS32, 2, 4>(p, h, w, c0, n, r0, r1, s_o, s_ml);
   else join_rows<T, D, ROWS32, 1, 8>(p, h, w, c0, n, r0, r1, s_o, s_ml);
@@ -856,6 +864,10 @@ __global__ void __launch_bounds__(D_THREADS, D == 64 ? 2 : 1)
 // 44 or 64 with A in TMEM, so whole 128-key tiles: halves of 64 keys, which
 // would double-buffer within the same columns, measured 2076 tensor cycles per
 // unit of two query tiles against 1244.
+// What bounds it is the softmax's latency: two 2048-token chunks over 8192 keys
+// (155 us, 777 TFLOP/s) keep the special-function unit 71 %, the issue slots 51 %
+// and the tensor pipe 40 % of the cycles busy, with two softmax warps on a
+// scheduler that each load scores, take the maximum, weigh and store in turn.
 // Items of more than 128 rows give each group one of the two query tiles;
 // smaller ones give both groups the same queries and alternate key tiles
 // between them; the two accumulators are then joined in the epilogue. Either
@@ -891,8 +903,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^x for two x < 128 on the FMA and integer pipes, for part of a tile: the
-// special-function unit alone would bound the softmax. x = n + f with n the
+// 2^x for two x < 128 on the FMA and integer pipes, for part of a tile: less for
+// the special-function unit, the busiest pipe. x = n + f with n the
 // nearest integer (read off the low bits of x + 1.5 * 2^23 + 127, so that the
 // shifted bits are the FP32 exponent of 2^n) and |f| <= 1/2; 2^f by the degree-4
 // polynomial of least relative error on that interval (Remez exchange on
@@ -1382,7 +1394,12 @@ __global__ void __launch_bounds__(T_THREADS, 1)
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 constexpr size_t MAX_SMEM = 227 * 1024 - 256;  // dynamic part of a CTA's shared memory
-constexpr int FEW_ROWS = 16;  // query rows per KV head the warp-level kernel takes
+// Query rows per KV head the warp-level kernel takes, of any sequence of the call.
+// Rows beyond 8 fill its products' second half; against the tiles they took (16/8
+// heads of 64, with tokens x group = 10 and 16): 16 x 5 tokens over 4096 keys 38.5
+// and 45.3 us, 16 x 8 39.5 and 45.2, 64 x 8 over 256 to 4096 65.9 and 99.0, 8 over
+// 30000 24.8 and 31.6.
+constexpr int FEW_ROWS = 16;
 
 struct Plan {
   bool few;
@@ -1472,6 +1489,9 @@ int run_join(const Params& p, int sms, cudaStream_t s) {
 template <typename T, int D, bool R16>
 int run_few(Params& p, const Plan& pl, const CUtensorMap& tk, const CUtensorMap& tv, int sms, cudaStream_t s) {
   const int rows = p.max_q * p.G;
+  // Two or three units in the ring: 64 single tokens over up to 4096 keys 56.0 and
+  // 58.6 us, 64 x 8 63.3 and 65.9, 16 x 8 over 4096 39.1 and 39.5, but 8 tokens over
+  // 30000 keys 27.1 and 24.8.
   int stages = 3;
   while (stages > 2 && dlayout(D, stages, rows, pl.hc).total > MAX_SMEM) --stages;
   const size_t smem = dlayout(D, stages, rows, pl.hc).total;
@@ -1496,10 +1516,8 @@ int run(Params& p, const Plan& pl, const void* q, const void* kp, const void* vp
   if ((st = make_tmap_pages(&tk, kp, bf, D, page_size, p.Hk, p.num_pages, head_major, br, pl.hc))) return st;
   if ((st = make_tmap_pages(&tv, vp, bf, D, page_size, p.Hk, p.num_pages, head_major, br, pl.hc))) return st;
   if (pl.few) {
-    p.min_share = 4;
     return p.max_q * p.G <= 8 ? run_few<T, D, false>(p, pl, tk, tv, sms, s) : run_few<T, D, true>(p, pl, tk, tv, sms, s);
   }
-  p.min_share = 4;
   const uint64_t dims[3] = {(uint64_t)D, (uint64_t)p.H, (uint64_t)p.N};
   const uint64_t strides[2] = {(uint64_t)D * 2, (uint64_t)p.H * D * 2};
   const uint32_t box[3] = {64, (uint32_t)p.G, (uint32_t)(128 / p.G)};

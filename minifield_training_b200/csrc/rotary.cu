@@ -24,11 +24,14 @@
 // takes a few tokens at a time: their heads' loads are under way while the
 // block computes the tokens' rotary_dim/2 angles each into shared memory; their
 // positions and cache rows, a chain of dependent loads, are looked up for 32
-// tokens at a time. The
-// floor is the bytes; what keeps a kernel of this kind above it is the
-// instructions per byte: with a warp per token that loops over the heads, the
-// same arithmetic took three times the instructions and 84 to 111 us where
-// this takes 70 us (16384 tokens of 32 heads, forward and backward).
+// tokens at a time. The floor is the bytes. With a warp per token that loops
+// over the heads, the same arithmetic took three times the instructions and 84 to
+// 111 us where this takes 70 us (16384 tokens of 32 heads, forward and backward).
+// In those the issue slots are now busy 65 and 63 % of the cycles and the ALUs 44,
+// and of the 11 to 12 cycles between a warp's instructions 3 to 4 pass at a pass's
+// barrier, where the heads' threads wait for the angles: more than anywhere else.
+// Head counts that do not fill a block (32 heads of 64, 16 of 128, or a multiple)
+// leave threads that load the last head and store nothing.
 #include <algorithm>
 
 #include "types16.cuh"

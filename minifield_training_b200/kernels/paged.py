@@ -99,7 +99,12 @@ def paged_attention(q, cache: PagedCache, cu_q, seq_lens, page_table, *, max_q, 
     ``scale`` (positive) defaults to head_dim ** -0.5. ``lse`` (float32 [N, heads], optional) receives the
     natural log-sum-exp of the scaled scores. Calls on one ``workspace``
     (``paged_attention_workspace_size`` bytes) must not overlap; the default
-    one belongs to the stream, and a captured call needs its own.
+    one belongs to the device and stream, and a captured call needs its own.
+
+    A sequence's keys and values must be finite: one that is not reaches the
+    queries of its chunk up to 128 keys before it (behind the sequence anything
+    may lie). What contradicts itself on the device (lengths, page ids) is
+    clamped and recorded for ``paged_attention_status``.
     """
     q = as_device(q, cache.dtype, stream)
     if q.ndim != 3:

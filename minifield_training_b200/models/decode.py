@@ -408,8 +408,9 @@ class Decoder:
         by default), each at its own length: a prompt or a part of one, or one
         decoded token. DecodeOverflow when the pool or a row's table is full,
         like any other refusal, comes before anything runs and leaves the state
-        as it was. ``controls``: keyword arguments of
-        kernels.logits.process_logits for the returned logits. ``out`` (a
+        as it was; what the attention clamps or gives up on while it runs is
+        recorded for kernels.paged.paged_attention_status. ``controls``: keyword
+        arguments of kernels.logits.process_logits for the returned logits. ``out`` (a
         float32 [R, vocab] DeviceArray) receives them. ``graph=True`` replays a
         single-token step (T = 1) as one CUDA graph, captured on the first call
         for these rows of this state (needs a created stream).
