@@ -1291,6 +1291,11 @@ __global__ void __launch_bounds__(T_THREADS, 1)
           tc::tmem_st_wait();
           tc::tc_fence_before();
         }
+        // With three buffers a job's scores do not wait for the product of the
+        // group's job before it, and the epilogue's wait tells this item's last
+        // product only from the one before by the phase's parity: that one has
+        // to be done before the last can start.
+        if (S::NB > 2 && j + 2 >= jobs && mine > 0 && ok) ok = tc::mbar_wait_w(pv_done(grp), (mine - 1) & 1, status, 35);
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(p_full(bj));
         bj += 2;

@@ -170,3 +170,34 @@ def test_more_items_and_sequences_than_threads(batch, counts, h, hk, page, dtype
     again, lse2 = run_attention(*a, False, dtype, max(counts))
     np.testing.assert_array_equal(again.view(np.uint16), got.view(np.uint16))
     np.testing.assert_array_equal(lse2, lse)
+
+
+@pytest.mark.parametrize("lens, counts, h, hk, page, head_major, dtype", [
+    ([147, 2013, 420, 671, 1800, 2692, 908, 1609], [27, 27, 8, 32, 1, 12, 22, 14], 40, 8, 32, True, "bfloat16"),
+    ([2680, 2794, 677, 609, 2711, 984], [4, 2, 6, 3, 6, 1], 48, 3, 8, True, "float16"),
+    ([72, 2645, 5, 2196, 1545, 1927, 341, 1859, 2436], [4, 5, 3, 1, 5, 4, 5, 3, 20], 2, 1, 8, False, "float16"),
+    ([545, 365, 155, 75, 448, 656, 109, 434, 582, 643, 702], [2, 2, 0, 2, 2, 2, 0, 3, 3, 1, 3], 7, 1, 8, False, "bfloat16"),
+])
+def test_tiles_whose_values_come_late(lens, counts, h, hk, page, head_major, dtype):
+    """Many small boxes per tile: an item's last softmax may end before the product of the tile before it starts.
+
+    The outputs are read only behind both; every one of many calls, back to back, gives the same bits.
+    """
+    require_gpu()
+    from minifield_training_b200.device import DeviceArray
+    from minifield_training_b200.kernels import paged
+
+    rng = np.random.default_rng(sum(lens) + h + 64)
+    a = build(rng, lens, counts, h, hk, 64, page, head_major, dtype)
+    q, keys, values, cu, n, table = a
+    first, lse = run_attention(*a, head_major, dtype, max(counts))
+    check_attention(first, lse, *a, head_major, dtype, 0.125)
+    cache = paged.PagedCache(dev(keys, dtype), dev(values, dtype), head_major=head_major)
+    args = [dev(q, dtype), cache, dev(cu), dev(n), dev(table)]
+    outs = [DeviceArray(q.shape, dtype) for _ in range(10)]
+    for _ in range(20):
+        for out in outs:
+            paged.paged_attention(*args, max_q=max(counts), out=out)
+        for out in outs:
+            np.testing.assert_array_equal(out.numpy().view(np.uint16), first.view(np.uint16))
+    assert paged.paged_attention_status() == 0
