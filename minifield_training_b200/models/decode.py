@@ -48,6 +48,7 @@ concatenated rows.
 """
 
 import ctypes
+import weakref
 
 import numpy as np
 
@@ -262,6 +263,7 @@ class Decoder:
             self.layers.append(L)
         _lib.call("mfb_device_sync")
         self._scratch, self._graphs, self._prefill_scratch, self._extend_scratch = {}, {}, {}, {}
+        self._dead_graphs = []  # keys of graphs whose paged state is gone
 
     def _buffers(self, batch: int, capacity: int):
         key = (batch, capacity)
@@ -456,6 +458,10 @@ class Decoder:
             key = ("paged", b, rows.start, state.max_pages, state.num_pages, state.page_size,
                    state.device_table.ptr) + tuple(
                 h.ptr if c is None else (c.keys.ptr, c.values.ptr) for c, h in zip(state.caches, state.history))
+            if self._dead_graphs:
+                _lib.call("mfb_stream_sync", P(s))  # their last replays may still run
+                while self._dead_graphs:
+                    _lib.call("mfb_graph_destroy", P(self._graphs.pop(self._dead_graphs.pop())))
             g = self._graphs.get(key)
             if g is None:
                 _lib.call("mfb_graph_begin", P(s))
@@ -465,6 +471,7 @@ class Decoder:
                     g_ = P()
                     _lib.call("mfb_graph_end", P(s), ctypes.byref(g_))
                 g = self._graphs[key] = g_.value
+                weakref.finalize(state, self._dead_graphs.append, key).atexit = False
             _lib.call("mfb_graph_launch", P(g), P(s))
         else:
             self._extend_layers(B, state, rows, t)
@@ -680,7 +687,7 @@ class Decoder:
 
     def close(self):
         """Release the captured decode graphs and the scratch of ``extend``."""
-        graphs, self._graphs = getattr(self, "_graphs", {}), {}
+        graphs, self._graphs, self._dead_graphs = getattr(self, "_graphs", {}), {}, []
         for g in graphs.values():
             if _lib._lib is not None:
                 _lib.lib().mfb_graph_destroy(P(g))

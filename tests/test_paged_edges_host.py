@@ -291,3 +291,22 @@ def test_pages_go_to_distinct_rows(fake, rows, tokens):
     with pytest.raises(ValueError, match="distinct rows"):
         state.grow(rows, tokens)
     assert state.lengths == [5, 5] and len(state._free) == 6
+
+
+def test_graphs_of_a_state_that_is_gone_are_released(fake):
+    """Behind a synchronise of the stream, by the next captured or replayed step; a living state's stay."""
+    dec, cfg, dm = decoder(stream=64)
+
+    def step(state, rows=None):
+        start = len(fake.calls)
+        dec.extend(np.zeros((len(rows or range(2)), 1), np.int32), state, rows=rows, graph=True)
+        return [n for n in fake.names()[start:] if n in ("mfb_stream_sync", "mfb_graph_destroy", "mfb_graph_end")]
+
+    kept = dm.new_paged_state(cfg, 2, 8, 64)
+    for _ in range(5):
+        state = dm.new_paged_state(cfg, 2, 8, 64)
+        assert step(state)[-1:] == step(state, range(1, 2)) == ["mfb_graph_end"]
+        del state
+    assert step(kept) == ["mfb_stream_sync"] + 2 * ["mfb_graph_destroy"] + ["mfb_graph_end"]
+    assert step(kept) == [] and len(dec._graphs) == 1
+    dec._graphs.clear()  # handles of the recorded library
